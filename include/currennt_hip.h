@@ -1,7 +1,7 @@
 /* C ABI of the gfx950 (MI355X) implementation of CURRENNT's backward hot path.
  *
  * Every entry point takes plain device pointers and sizes; no C++ or PyTorch types cross this
- * boundary.  All buffers are fp32 and use the reference's layouts:
+ * boundary.  All buffers are fp32, where nothing else is said, and use the reference's layouts:
  *   - an activation / error buffer of a layer of size D is a column-major D x (T*S) matrix whose
  *     column index is t*S + s  (time-major, S parallel sequences interleaved);
  *   - patTypes is char[T*S], values 0 none (padding), 1 first, 2 normal, 3 last (Types.hpp:35-38);
@@ -22,6 +22,9 @@ extern "C" {
 #endif
 
 enum { CNT_OK = 0, CNT_ERR_ARG = 1, CNT_ERR_HIP = 2, CNT_ERR_STATE = 3, CNT_ERR_DEVICE = 4 };
+
+/* Element types of the operators over symbols (embedding, log probabilities, gradient norm); everything else is fp32. */
+enum { CNT_F32 = 0, CNT_BF16 = 1, CNT_F16 = 2 };
 
 enum { CNT_ACT_IDENTITY = 0, CNT_ACT_TANH = 1, CNT_ACT_LOGISTIC = 2, CNT_ACT_RELU = 3 };
 
@@ -113,6 +116,55 @@ int cnt_gemm_scratch_buffers(void);
  * GPU (different streams or threads) race; calls on one stream are ordered and safe. */
 int cnt_dense_backward_weights_static(void *stream, int P, int D, int N, float bias, const float *x, const float *err,
                                       float *weight_updates);
+
+/* ---- embedding ---------------------------------------------------------------------------------
+ * The feed-forward layer of a one-hot input without its product: slot n's symbol picks a row of a table of V rows of D
+ * values.  No counterpart in the reference, whose word vectors are data of the input layer.
+ *   out[n] = scale * table[tokens[n]], a row of zeros where tokens[n] is outside 0 .. V-1 (a slot without a symbol).
+ * Row r of a matrix begins at r * stride elements; rows that are read may overlap (stride 0: one row for all), rows that are written
+ * may not (stride >= D).  Bases need the alignment of an element only.  table_type, out_type: CNT_F32, CNT_BF16 or CNT_F16, any two of
+ * them; products are formed in 32 bits and rounded once.  N and D up to a launch of 2^24 workgroups (CNT_ERR_ARG beyond). */
+int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const void *table, long table_stride, const int *tokens,
+                      float scale, int out_type, void *out, long out_stride);
+/* The table's gradient: grad[v] = scale * sum of err[n] over the slots n with tokens[n] = v, for all V rows (rows of zeros where
+ * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
+ * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
+ * cnt_embed_scratch(V, D, N) bytes, aligned to 16, with any content, which the call has for itself until it has run (two captured
+ * graphs that may run at the same time need one each).  N <= 2^30. */
+long cnt_embed_scratch(int V, int D, long N);
+int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
+                       long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,
+                       size_t scratch_bytes);
+
+/* ---- log probabilities of symbols ----------------------------------------------------------------
+ * What the softmax unit of the MDN layer (layers/MDNUnit.cu) does for classes, for vocabularies of any size and with what
+ * scoring, sampling and losses ask for.  Row n of `logits` (V values of `type`, rows `stride` >= 0 elements apart) with
+ * z = scale * logits, scale > 0:
+ *   lse[n]     = log sum_v exp z_v
+ *   logp[n]    = z_t - lse[n], t = tokens[n]; 0 where tokens[n] is outside 0 .. V-1 (a slot without a symbol)
+ *   entropy[n] = - sum_v p_v log p_v, p = exp(z - lse)
+ *   top_logp, top_tokens (N x K, row n at n * K): the K largest, the largest first, the lower token where two logits are equal.
+ * A logit of -inf is a token that is ruled out: its p is 0.  A row with nothing else has lse = -inf, logp = -inf, entropy 0 and the
+ * tokens 0 .. K-1 as alternatives.  A row with a NaN or +inf has NaN in lse, logp, entropy and top_logp; NaN logits are never among the
+ * alternatives (token -1 where fewer than K are left).  Any result may be NULL; K is 0 .. 64 and <= V.  N < 2^24, V <= 2^30.
+ * scratch: device memory of cnt_logprob_scratch(N, V, K) bytes (0 for most sizes: NULL then), any content, the call's own until
+ * it has run. */
+long cnt_logprob_scratch(long N, int V, int K);
+int cnt_logprob_forward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
+                        float *logp, float *lse, float *entropy, int K, float *top_logp, int *top_tokens, void *scratch,
+                        size_t scratch_bytes);
+/* Errors of the logits from the errors of logp and entropy (either may be NULL: zeros):
+ *   err[v] = scale * (logp_err[n] * ([v = t] - p_v) - entropy_err[n] * p_v * (log p_v + entropy[n]))
+ * with the lse and entropy of the forward call, in the logits' type (rows err_stride apart).  err may be the logits themselves, with the
+ * same stride.  Rows where everything is ruled out get zeros, slots without a symbol the entropy's part alone. */
+int cnt_logprob_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
+                         const float *lse, const float *entropy, const float *logp_err, const float *entropy_err, void *err,
+                         long err_stride);
+/* Both in one call, for losses whose errors do not depend on the results (a sum or mean over slots): logp (may be NULL), lse, entropy
+ * and err.  scratch as for the forward call with K = 0. */
+int cnt_logprob_error_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
+                               const float *logp_err, const float *entropy_err, float *logp, float *lse, float *entropy, void *err,
+                               long err_stride, void *scratch, size_t scratch_bytes);
 
 /* ---- SSE post-output layer ---------------------------------------------------------------------
  * SsePostOutputLayer::computeBackwardPass (layers/SsePostOutputLayer.cu:224-267):
@@ -507,6 +559,11 @@ int cnt_network_set_wait_bounds(cnt_network *net, int layer_index, unsigned spin
  * own "learningRate" (layers/TrainableLayer.cu:110-111), the step is one launch per trainable layer instead. */
 int cnt_network_update(cnt_network *net, void *stream, int option, float learning_rate, float momentum,
                        float frac_length);
+/* The same step on gradients clipped to a norm over all weights of the network (see cnt_opt_grad_norm; result: its two floats,
+ * device memory).  The gradients are those of the fraction's sum, as the layers' weight updates hold them: before they are divided by
+ * frac_length.  The first call allocates. */
+int cnt_network_update_clipped(cnt_network *net, void *stream, int option, float learning_rate, float momentum, float frac_length,
+                               float max_norm, float *result);
 /* NeuralNetwork::exportLayers + exportWeights (NeuralNetwork.cpp:2993-3040): the layer objects as they stood in the
  * network file plus the current weights.  *needed receives the size including the terminating 0; nothing is
  * written if cap is smaller (call once with buf = NULL to learn the size). */
@@ -540,6 +597,28 @@ int cnt_opt_step(void *stream, int option, long n, float *weights, const float *
                  float *stats, float *weight_deltas, const float *mask, float frac_length, float beta1_accum,
                  float beta2_accum, float learning_rate, float momentum);
 float cnt_opt_next_beta_accum(float accum, int which);
+
+/* ---- norm of all gradients, and clipping -------------------------------------------------------------
+ * A cnt_gradients handle is a list of tensors: tensor i has sizes[i] elements of types[i] (CNT_F32, CNT_BF16, CNT_F16) at
+ * gradients[i] (device memory, aligned to its elements), and cnt_opt_clip writes to clipped[i] (same size and type; clipped = NULL: in
+ * place).  The three arrays are host memory and copied; the tensors have to stay where they are.  The create call allocates, the
+ * others only enqueue work.  Calls with one handle share its sums: they have to follow each other, also those of captured
+ * graphs.  No counterpart in the reference, which limits single error values only (helpers/limitedError.cuh).
+ *   result[0] = norm = sqrt(sum of all squares), summed in 64 bits in a fixed order
+ *   result[1] = factor = max_norm / norm if norm > max_norm, else 1; 0 if the norm is infinite or NaN
+ * result: two floats of device memory; max_norm > 0.  cnt_opt_grad_norm writes these; cnt_opt_clip also multiplies every element
+ * with the factor (zeros for the factor 0), rounded once. */
+typedef struct cnt_gradients cnt_gradients;
+int cnt_gradients_create(int count, const void *const *gradients, void *const *clipped, const long *sizes, const int *types,
+                         cnt_gradients **out);
+int cnt_gradients_destroy(cnt_gradients *set);
+int cnt_opt_grad_norm(cnt_gradients *set, void *stream, float max_norm, float *result);
+int cnt_opt_clip(cnt_gradients *set, void *stream, float max_norm, float *result);
+/* cnt_opt_step on clip[1] * layer_updates (zeros for the factor 0) with the result of cnt_opt_grad_norm: clipping without a pass over the
+ * gradients of its own. */
+int cnt_opt_step_clipped(void *stream, int option, long n, float *weights, const float *layer_updates, float *cur_updates,
+                         float *stats, float *weight_deltas, const float *mask, float frac_length, float beta1_accum,
+                         float beta2_accum, float learning_rate, float momentum, const float *clip);
 
 /* ---- the .nc data path (NetCDF reader and fraction builder; host memory only) ------------------------
  * data_sets::DataSet's constructor for ONE .nc file (data_sets/DataSet.cpp:1376-1907): reads the

@@ -93,6 +93,18 @@ _SIGNATURES = {
     "cnt_opt_update_weights": (I, [VP, C.c_long, VP, VP, VP, VP, F, F]),
     "cnt_opt_step": (I, [VP, I, C.c_long, VP, VP, VP, VP, VP, VP, F, F, F, F, F]),
     "cnt_opt_next_beta_accum": (F, [F, I]),
+    "cnt_opt_step_clipped": (I, [VP, I, C.c_long, VP, VP, VP, VP, VP, VP, F, F, F, F, F, VP]),
+    "cnt_gradients_create": (I, [I, VP, VP, VP, VP, C.POINTER(VP)]),
+    "cnt_gradients_destroy": (I, [VP]),
+    "cnt_opt_grad_norm": (I, [VP, VP, F, VP]),
+    "cnt_opt_clip": (I, [VP, VP, F, VP]),
+    "cnt_embed_forward": (I, [VP, I, I, C.c_long, I, VP, C.c_long, VP, F, I, VP, C.c_long]),
+    "cnt_embed_scratch": (C.c_long, [I, I, C.c_long]),
+    "cnt_embed_backward": (I, [VP, I, I, C.c_long, VP, F, I, VP, C.c_long, I, VP, C.c_long, I, VP, C.c_size_t]),
+    "cnt_logprob_scratch": (C.c_long, [C.c_long, I, I]),
+    "cnt_logprob_forward": (I, [VP, C.c_long, I, I, VP, C.c_long, F, VP, VP, VP, VP, I, VP, VP, VP, C.c_size_t]),
+    "cnt_logprob_backward": (I, [VP, C.c_long, I, I, VP, C.c_long, F, VP, VP, VP, VP, VP, VP, C.c_long]),
+    "cnt_logprob_error_backward": (I, [VP, C.c_long, I, I, VP, C.c_long, F, VP, VP, VP, VP, VP, VP, VP, C.c_long, VP, C.c_size_t]),
     "cnt_lstm_create": (I, [C.POINTER(LstmDesc), C.POINTER(VP)]),
     "cnt_lstm_destroy": (I, [VP]),
     "cnt_lstm_load_sequences": (I, [VP, VP, VP, I, I]),
@@ -153,6 +165,7 @@ _SIGNATURES = {
     "cnt_network_backward": (I, [VP, VP]),
     "cnt_network_check": (I, [VP, VP]),
     "cnt_network_update": (I, [VP, VP, I, F, F, F]),
+    "cnt_network_update_clipped": (I, [VP, VP, I, F, F, F, F, VP]),
     "cnt_network_export_json": (I, [VP, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)]),
     "cnt_skipadd_forward": (I, [VP, C.c_long, I, C.POINTER(VP), VP, VP, VP]),
     "cnt_skipadd_backward": (I, [VP, C.c_long, VP, VP, I, C.POINTER(VP), C.POINTER(I)]),
@@ -418,6 +431,228 @@ def opt_step(option, weights, layer_updates, cur_updates, stats, deltas, mask, f
                              beta2_accum, learning_rate, momentum))
 
 
+# ---- operators over symbols: tensors of 32 and 16 bits, rows at any stride; every call checks what it is given ----
+
+_ELEMENTS = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_element_codes = {}  # torch.dtype -> code of the library
+
+
+def _element(name, t):
+    code = _element_codes.get(t.dtype)
+    if code is None:
+        code = _ELEMENTS.get(str(t.dtype))
+        if code is None:
+            raise ValueError("%s: float32, bfloat16 or float16 is wanted, not %s" % (name, t.dtype))
+        _element_codes[t.dtype] = code
+    return code
+
+
+def _on_device(name, t, device):
+    if t.device != device or device.type != "cuda":
+        raise ValueError("%s is on %s, the call on %s" % (name, t.device, device))
+
+
+def _matrix(name, t, device, shape=None):
+    """The row stride of a matrix whose rows are contiguous."""
+    _on_device(name, t, device)
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError("%s: a matrix%s is wanted, not %s" % (name, "" if shape is None else " of %d x %d" % shape, tuple(t.shape)))
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("%s: the values of a row have to be contiguous" % name)
+    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def _vector(name, t, dtype, count, device):
+    """A contiguous vector of `count` values (or None)."""
+    if t is None:
+        return
+    _on_device(name, t, device)
+    if str(t.dtype) != "torch." + dtype or t.numel() != count or not t.is_contiguous():
+        raise ValueError("%s: %d contiguous values of %s are wanted, not %s of %s" % (name, count, dtype, tuple(t.shape), t.dtype))
+
+
+def _enqueue(device, stream, call):
+    """call(stream pointer) on `stream`, or on the device's current one."""
+    import torch
+
+    if stream is not None and stream.device != device:
+        raise ValueError("the stream is on %s, the tensors are on %s" % (stream.device, device))
+    if torch.cuda.current_device() == device.index:
+        check(call(stream_ptr(stream)))
+    else:
+        with torch.cuda.device(device):
+            check(call(stream_ptr(stream)))
+
+
+def _scratch(scratch, need, device, stream):
+    """`scratch`, or memory of the calling stream's pool where there is none."""
+    import torch
+
+    if need < 0:
+        raise ValueError("sizes out of range")
+    if scratch is not None:
+        _on_device("scratch", scratch, device)
+        if not scratch.is_contiguous():
+            raise ValueError("scratch: contiguous memory is wanted")
+        return scratch
+    if need == 0:
+        return None
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _bytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def embed_forward(table, tokens, out, scale=1.0, stream=None):
+    """out[n] = scale * table[tokens[n]]; zeros where tokens[n] is no row of the table (see cnt_embed_forward)."""
+    device, (V, D), N = table.device, table.shape, tokens.numel()
+    ts, os_ = _matrix("table", table, device), _matrix("out", out, device, (N, D))
+    _vector("tokens", tokens, "int32", N, device)
+    args = (V, D, N, _element("table", table), ptr(table), ts, ptr(tokens), scale, _element("out", out), ptr(out), os_)
+    _enqueue(device, stream, lambda s: lib().cnt_embed_forward(s, *args))
+
+
+def embed_scratch(V, D, N):
+    """Bytes of scratch memory that embed_backward needs."""
+    need = lib().cnt_embed_scratch(V, D, N)
+    if need < 0:
+        raise ValueError("sizes out of range")
+    return need
+
+
+def embed_backward(tokens, err, grad, scale=1.0, accumulate=False, scratch=None, stream=None):
+    """grad[v] = scale * sum of err[n] over the slots with tokens[n] = v, added to what grad holds if asked (see cnt_embed_backward)."""
+    device, (V, D), N = grad.device, grad.shape, tokens.numel()
+    gs, es = _matrix("grad", grad, device), _matrix("err", err, device, (N, D))
+    _vector("tokens", tokens, "int32", N, device)
+    scratch = _scratch(scratch, lib().cnt_embed_scratch(V, D, N), device, stream)
+    args = (V, D, N, ptr(tokens), scale, _element("err", err), ptr(err), es, _element("grad", grad), ptr(grad), gs, int(accumulate),
+            ptr(scratch), _bytes(scratch))
+    _enqueue(device, stream, lambda s: lib().cnt_embed_backward(s, *args))
+
+
+def logprob_scratch(N, V, K=0):
+    """Bytes of scratch memory that logprob_forward (logprob_error_backward: K = 0) needs; none for most sizes."""
+    need = lib().cnt_logprob_scratch(N, V, K)
+    if need < 0:
+        raise ValueError("sizes out of range")
+    return need
+
+
+def _row_results(device, N, tokens, **vectors):
+    _vector("tokens", tokens, "int32", N, device)
+    for name, t in vectors.items():
+        _vector(name, t, "float32", N, device)
+
+
+def logprob_forward(logits, tokens=None, logp=None, lse=None, entropy=None, top_logp=None, top_tokens=None, scale=1.0, scratch=None,
+                    stream=None):
+    """Log probabilities of given tokens, log sums, entropies and the most probable alternatives of every row, into the tensors
+    that are given (see cnt_logprob_forward); top_logp and top_tokens are N x K."""
+    device, (N, V) = logits.device, logits.shape
+    stride = _matrix("logits", logits, device)
+    _row_results(device, N, tokens, logp=logp, lse=lse, entropy=entropy)
+    K = 0
+    for name, t, dtype in (("top_logp", top_logp, "float32"), ("top_tokens", top_tokens, "int32")):
+        if t is not None:
+            if t.dim() != 2 or t.shape[0] != N or (K and t.shape[1] != K):
+                raise ValueError("%s: a row of alternatives for each of %d rows is wanted, not %s" % (name, N, tuple(t.shape)))
+            K = t.shape[1]
+            _vector(name, t, dtype, N * K, device)
+    scratch = _scratch(scratch, lib().cnt_logprob_scratch(N, V, K) if K <= 64 else 0, device, stream)
+    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(logp), ptr(lse), ptr(entropy), K,
+            ptr(top_logp), ptr(top_tokens), ptr(scratch), _bytes(scratch))
+    _enqueue(device, stream, lambda s: lib().cnt_logprob_forward(s, *args))
+
+
+def _error_rows(logits, err):
+    device, (N, V) = logits.device, logits.shape
+    if err.dtype != logits.dtype:
+        raise ValueError("err: the errors have the logits' type, %s, not %s" % (logits.dtype, err.dtype))
+    return _matrix("logits", logits, device), _matrix("err", err, device, (N, V))
+
+
+def logprob_backward(logits, tokens, lse, entropy, logp_err, entropy_err, err, scale=1.0, stream=None):
+    """Errors of the logits from those of logp and entropy, either of which may be None (see cnt_logprob_backward)."""
+    device, (N, V) = logits.device, logits.shape
+    stride, err_stride = _error_rows(logits, err)
+    _row_results(device, N, tokens, lse=lse, entropy=entropy, logp_err=logp_err, entropy_err=entropy_err)
+    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(lse), ptr(entropy), ptr(logp_err),
+            ptr(entropy_err), ptr(err), err_stride)
+    _enqueue(device, stream, lambda s: lib().cnt_logprob_backward(s, *args))
+
+
+def logprob_error_backward(logits, tokens, logp_err, entropy_err, logp, lse, entropy, err, scale=1.0, scratch=None, stream=None):
+    """logprob_forward and logprob_backward in one call, for errors that are known before (see cnt_logprob_error_backward)."""
+    device, (N, V) = logits.device, logits.shape
+    stride, err_stride = _error_rows(logits, err)
+    _row_results(device, N, tokens, logp_err=logp_err, entropy_err=entropy_err, logp=logp, lse=lse, entropy=entropy)
+    scratch = _scratch(scratch, lib().cnt_logprob_scratch(N, V, 0), device, stream)
+    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(logp_err), ptr(entropy_err), ptr(logp),
+            ptr(lse), ptr(entropy), ptr(err), err_stride, ptr(scratch), _bytes(scratch))
+    _enqueue(device, stream, lambda s: lib().cnt_logprob_error_backward(s, *args))
+
+
+class GradientSet:
+    """Thin owner of a cnt_gradients handle: a list of contiguous gradient tensors and of those that the clipped gradients go to (None:
+    in place).  Holds on to the tensors; a gradient that is replaced by another tensor needs another set."""
+
+    def __init__(self, gradients, clipped=None):
+        import torch
+
+        self.handle = VP()
+        self.gradients, self.clipped = list(gradients), None if clipped is None else list(clipped)
+        n = len(self.gradients)
+        if self.clipped is not None and len(self.clipped) != n:
+            raise ValueError("%d gradients and %d places for them" % (n, len(self.clipped)))
+        self.device = self.gradients[0].device if n else torch.device("cuda", torch.cuda.current_device())
+        for i, g in enumerate(self.gradients):
+            to = g if self.clipped is None else self.clipped[i]
+            for name, t in (("gradient", g), ("clipped gradient", to)):
+                _on_device("%s %d" % (name, i), t, self.device)
+                if not t.is_contiguous() or t.shape != g.shape or t.dtype != g.dtype:
+                    raise ValueError("%s %d: contiguous %s of shape %s is wanted" % (name, i, g.dtype, tuple(g.shape)))
+        sizes = (C.c_long * n)(*[g.numel() for g in self.gradients])
+        types = (I * n)(*[_element("gradient %d" % i, g) for i, g in enumerate(self.gradients)])
+        to = None if self.clipped is None else _ptr_array(self.clipped)
+        with torch.cuda.device(self.device):
+            check(lib().cnt_gradients_create(n, _ptr_array(self.gradients), to, sizes, types, C.byref(self.handle)))
+
+    def close(self):
+        if self.handle:
+            lib().cnt_gradients_destroy(self.handle)
+            self.handle = VP()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def opt_grad_norm(gradient_set, max_norm, result, stream=None):
+    """result = [norm of all gradients of the set, factor that brings it down to max_norm] (see cnt_opt_grad_norm)."""
+    _vector("result", result, "float32", 2, gradient_set.device)
+    _enqueue(gradient_set.device, stream, lambda s: lib().cnt_opt_grad_norm(gradient_set.handle, s, max_norm, ptr(result)))
+
+
+def opt_clip(gradient_set, max_norm, result, stream=None):
+    """opt_grad_norm, and the gradients multiplied with the factor (see cnt_opt_clip)."""
+    _vector("result", result, "float32", 2, gradient_set.device)
+    _enqueue(gradient_set.device, stream, lambda s: lib().cnt_opt_clip(gradient_set.handle, s, max_norm, ptr(result)))
+
+
+def opt_step_clipped(option, weights, layer_updates, cur_updates, stats, deltas, mask, frac_length, beta1_accum, beta2_accum,
+                     learning_rate, momentum, clip, stream=None):
+    """opt_step on clip[1] * layer_updates, clip as opt_grad_norm has left it."""
+    _vector("clip", clip, "float32", 2, weights.device)
+    check(lib().cnt_opt_step_clipped(stream_ptr(stream), option, weights.numel(), ptr(weights), ptr(layer_updates),
+                                     ptr(cur_updates), ptr(stats), ptr(deltas), ptr(mask), frac_length, beta1_accum,
+                                     beta2_accum, learning_rate, momentum, ptr(clip)))
+
+
 def opt_next_beta_accum(accum, which):
     return float(lib().cnt_opt_next_beta_accum(accum, which))
 
@@ -665,6 +900,12 @@ class Network:
 
     def update(self, option, learning_rate, momentum, frac_length, stream=None):
         check(lib().cnt_network_update(self.handle, stream_ptr(stream), option, learning_rate, momentum, frac_length))
+
+    def update_clipped(self, option, learning_rate, momentum, frac_length, max_norm, result, stream=None):
+        """`update` with the gradients clipped to max_norm; result (two floats on the device) receives their norm and the factor."""
+        _vector("result", result, "float32", 2, result.device)
+        check(lib().cnt_network_update_clipped(self.handle, stream_ptr(stream), option, learning_rate, momentum, frac_length, max_norm,
+                                               ptr(result)))
 
     def export_json(self):
         need = C.c_size_t()

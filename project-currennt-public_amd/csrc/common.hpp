@@ -357,10 +357,11 @@ int gemm_simple(hipStream_t stream, float *C, int m, int n, int k, const float *
                 const float *B, bool transB, bool accumulate);
 
 // cnt_opt_step with a device flag in front of it: when *veto is non-zero at the time the kernel runs (a recursion of
-// the pass that produced the gradients gave up), the step changes nothing.
+// the pass that produced the gradients gave up), the step changes nothing.  clip: see cnt_opt_step_clipped, may be NULL.
 int opt_step_guarded(hipStream_t stream, int option, long n, float *weights, const float *layer_updates, float *cur_updates,
                      float *stats, float *weight_deltas, const float *mask, float frac_length, float beta1_accum,
-                     float beta2_accum, float learning_rate, float momentum, const int *veto, const float *accum_dev);
+                     float beta2_accum, float learning_rate, float momentum, const int *veto, const float *accum_dev,
+                     const float *clip);
 // Adam's bias-correction products (two floats in device memory, both 1 before the first step) advanced by one step,
 // unless *veto is non-zero; opt_step_guarded reads them in place of its two float arguments when accum_dev is given.
 int opt_adam_advance(hipStream_t stream, float *accum_dev, const int *veto);

@@ -1,0 +1,73 @@
+// Elements of 32 and 16 bits: what the operators over symbols read and write.  All of them compute in 32 bits and round a result once.
+#pragma once
+
+#include "common.hpp"
+
+namespace cnt {
+
+inline bool known_type(int type) { return type == CNT_F32 || type == CNT_BF16 || type == CNT_F16; }
+inline size_t element_size(int type) { return type == CNT_F32 ? 4 : 2; }
+
+template <typename T>
+struct Tag {
+    using type = T;
+};
+// f(Tag<T>()) for the element type T that `type` names; the caller has checked it
+template <typename F>
+inline void with_type(int type, F f) {
+    if (type == CNT_F32) f(Tag<float>());
+    else if (type == CNT_BF16) f(Tag<__bf16>());
+    else f(Tag<_Float16>());
+}
+
+// N neighbouring elements at any address that an element may have: rows of odd lengths begin anywhere, and the hardware takes 16-byte
+// accesses at any address.
+template <typename T, int N>
+struct Packed {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T, int N>
+__device__ __forceinline__ void fetch_elements(const T *p, float (&v)[N]) {
+    const typename Packed<T, N>::type x = *reinterpret_cast<const typename Packed<T, N>::type *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)x[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void put_elements(T *p, const float (&v)[N]) {
+    typename Packed<T, N>::type x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = (T)v[i];
+    *reinterpret_cast<typename Packed<T, N>::type *>(p) = x;
+}
+// the first `count` of N, 0 <= count <= N
+template <typename T, int N>
+__device__ __forceinline__ void fetch_some(const T *p, int count, float (&v)[N], float rest) {
+    if (count == N) {
+        fetch_elements<T, N>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < count ? (float)p[i] : rest;
+}
+template <typename T, int N>
+__device__ __forceinline__ void put_some(T *p, int count, const float (&v)[N]) {
+    if (count == N) {
+        put_elements<T, N>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < count) p[i] = (T)v[i];
+}
+
+// elements of a 16-byte access
+template <typename T>
+constexpr int kWide = 16 / (int)sizeof(T);
+
+inline int power_of_two_from(long n) {
+    int p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+}  // namespace cnt

@@ -1,0 +1,436 @@
+// Rows of a table looked up by token and scaled, and the table's gradient.
+//
+//   out[n] = scale * table[token[n]]                       (zero where slot n has no token)
+//   grad[v] = scale * sum over the slots n of token v of err[n]    (+ what grad held, if asked)
+//
+// Both move rows and are bounded by memory.  The gradient is formed by sorted tokens: a stable counting sort of the slots' tokens (one or
+// two passes of at most ten bits) makes a token's slots neighbours in ascending order, so a row's sum has one order, is formed in 32 bits
+// and written once, without atomics and without clearing the table first.  Tokens are as skewed as in any text: a run that covers
+// whole pieces of the sorted list is added up piece by piece by workgroups of their own first.
+#include "elements.hpp"
+
+#include <algorithm>
+
+namespace cnt {
+namespace {
+
+// ----- lookup ---------------------------------------------------------------------------------------------------------------
+struct LookupArgs {
+    const void *table;
+    void *out;
+    const int *tokens;
+    long N, table_stride, out_stride;
+    int V, D, lanes;  // lanes: threads that share a row
+    float scale;
+};
+
+template <typename T, typename O>
+__global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
+    constexpr int W = 8;
+    const long n = (long)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    if (n >= a.N) return;
+    const int token = a.tokens[n];
+    const bool held = token >= 0 && token < a.V;
+    const T *from = static_cast<const T *>(a.table) + (held ? token : 0) * a.table_stride;
+    O *to = static_cast<O *>(a.out) + n * a.out_stride;
+    for (int d = (threadIdx.x % a.lanes) * W; d < a.D; d += a.lanes * W) {
+        const int count = min(W, a.D - d);
+        float v[W];
+        if (held) fetch_some<T, W>(from + d, count, v, 0.0f);
+#pragma unroll
+        for (int q = 0; q < W; ++q) v[q] = held ? v[q] * a.scale : 0.0f;
+        put_some<O, W>(to + d, count, v);
+    }
+}
+
+// ----- sort of the slots by token ---------------------------------------------------------------------------------------------
+constexpr int kMostBits = 10, kMostBins = 1 << kMostBits, kMostSortBlocks = 512;
+
+// Scratch of a gradient: two lists of (token, slot), counts of every block and digit, the number of slots with a token, partial sums.
+struct SortPlan {
+    int bits, passes, block, blocks, piece;  // slots per block, blocks; piece: entries of the sorted list that are added up together
+    size_t keys[2], slots[2], counts, total, partial, bytes;
+};
+SortPlan sort_plan(long V, int D, long N) {
+    SortPlan p = {};
+    int all = 0;
+    while ((1L << all) < V) ++all;
+    p.passes = std::max(1, (all + kMostBits - 1) / kMostBits);
+    p.bits = std::max(1, (all + p.passes - 1) / p.passes);
+    // a wave takes its quarter of a block in steps of 64 slots
+    p.block = (int)((std::max(1024L, (N + kMostSortBlocks - 1) / kMostSortBlocks) + 255) / 256 * 256);
+    p.blocks = (int)std::max(1L, (N + p.block - 1) / p.block);
+    p.piece = 64;
+    while (16L * p.piece * p.piece < N) p.piece *= 2;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t list = (size_t)N * sizeof(int);
+    p.keys[0] = take(list); p.slots[0] = take(list);
+    p.keys[1] = p.passes > 1 ? take(list) : 0; p.slots[1] = p.passes > 1 ? take(list) : 0;
+    p.counts = take((size_t)p.blocks * (1 << p.bits) * sizeof(int));
+    p.total = take(sizeof(int));
+    p.partial = take((size_t)(N / p.piece) * D * sizeof(float));
+    p.bytes = at;
+    return p;
+}
+
+struct SortArgs {
+    const int *keys, *slots;  // the list before the pass; first pass: keys are the tokens, slots NULL
+    int *keys_out, *slots_out, *counts, *total;
+    int N, V, shift, bits, block;
+};
+
+// First pass: a slot without a token has no place in the list.  Later ones: `total` entries are in it.
+template <bool FIRST>
+__device__ __forceinline__ int entries(const SortArgs &a) { return FIRST ? a.N : *a.total; }
+template <bool FIRST>
+__device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIRST || (key >= 0 && key < a.V); }
+
+// how often every digit occurs in a block of the list
+template <bool FIRST>
+__global__ __launch_bounds__(256) void token_count_kernel(const SortArgs a) {
+    __shared__ int bins[kMostBins];
+    const int n_bins = 1 << a.bits, n = entries<FIRST>(a);
+    for (int d = threadIdx.x; d < n_bins; d += 256) bins[d] = 0;
+    __syncthreads();
+    const long begin = (long)blockIdx.x * a.block, end = min((long)n, begin + a.block);
+    for (long i = begin + threadIdx.x; i < end; i += 256) {
+        const int key = a.keys[i];
+        if (listed<FIRST>(a, key)) atomicAdd(&bins[(key >> a.shift) & (n_bins - 1)], 1);
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < n_bins; d += 256) a.counts[blockIdx.x * n_bins + d] = bins[d];
+}
+
+// Puts a block's entries to their places.  Every block adds the blocks' counts up for itself, which saves a launch.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void token_place_kernel(const SortArgs a) {
+    __shared__ int next[4][kMostBins];  // counts of a wave's entries, then the next place for every wave and digit
+    __shared__ int totals[kMostBins];
+    __shared__ int wave_totals[4];
+    const int n_bins = 1 << a.bits, n = entries<FIRST>(a), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int d = tid; d < n_bins; d += 256) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) next[w][d] = 0;
+    }
+    __syncthreads();
+    const int quarter = a.block / 4;
+    const long begin = (long)blockIdx.x * a.block + (long)wave * quarter, end = min((long)n, begin + quarter);
+    for (long i = begin + lane; i < end; i += 64) {
+        const int key = a.keys[i];
+        if (listed<FIRST>(a, key)) atomicAdd(&next[wave][(key >> a.shift) & (n_bins - 1)], 1);
+    }
+    int before[kMostBins / 256];
+#pragma unroll
+    for (int q = 0; q < kMostBins / 256; ++q) {
+        const int d = tid + q * 256;
+        int all = 0, earlier = 0;
+        if (d < n_bins) {
+#pragma unroll 8
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const int c = a.counts[b * n_bins + d];
+                all += c;
+                earlier += b < (int)blockIdx.x ? c : 0;
+            }
+            totals[d] = all;
+        }
+        before[q] = earlier;
+    }
+    __syncthreads();
+    // places of the digits: four neighbouring ones per thread
+    int four[4], sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int d = tid * 4 + q;
+        four[q] = d < n_bins ? totals[d] : 0;
+        sum += four[q];
+    }
+    int upto = sum;
+    for (int o = 1; o < 64; o *= 2) {
+        const int other = __shfl_up(upto, o);
+        if (lane >= o) upto += other;
+    }
+    if (lane == 63) wave_totals[wave] = upto;
+    __syncthreads();
+    int place = upto - sum;
+    for (int w = 0; w < wave; ++w) place += wave_totals[w];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int d = tid * 4 + q;
+        if (d < n_bins) totals[d] = place;
+        place += four[q];
+    }
+    if (FIRST && blockIdx.x == 0 && tid == 255) *a.total = place;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kMostBins / 256; ++q) {
+        const int d = tid + q * 256;
+        if (d < n_bins) {
+            int at = totals[d] + before[q];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int c = next[w][d];
+                next[w][d] = at;
+                at += c;
+            }
+        }
+    }
+    __syncthreads();
+    // In steps of 64 entries, in order: lanes of one digit find each other by one ballot per bit.  Every lane reads its digit's
+    // next place before the first lane of the digit moves it on (the accesses of one wave to LDS are performed in order).
+    volatile int *mine = next[wave];
+    for (long i0 = begin; i0 < end; i0 += 64) {
+        const long i = i0 + lane;
+        const int key = i < end ? a.keys[i] : -1;
+        const bool in = i < end && listed<FIRST>(a, key);
+        const int digit = in ? (key >> a.shift) & (n_bins - 1) : 0;
+        unsigned long long same = __ballot(in);
+        for (int bit = 0; bit < a.bits; ++bit) {
+            const bool set = (digit >> bit) & 1;
+            const unsigned long long b = __ballot(set);
+            same &= set ? b : ~b;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        const int at = mine[digit] + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (in && rank == 0) mine[digit] = at + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+        if (in) {
+            a.keys_out[at] = key;
+            a.slots_out[at] = FIRST ? (int)i : a.slots[i];
+        }
+    }
+}
+
+// ----- sums of the runs -------------------------------------------------------------------------------------------------------
+struct SumArgs {
+    const int *keys, *slots, *total;
+    const void *err;
+    void *grad;
+    float *partial;
+    long err_stride, grad_stride;
+    int V, D, lanes, piece, accumulate;
+    float scale;
+};
+
+constexpr int kShortRun = 32;
+
+// sum of entries first, first + step, ... < end of the sorted list, W columns from `column` on
+template <typename E, int W>
+__device__ __forceinline__ void add_entries(const SumArgs &a, int first, int end, int step, int column, int count, float (&sum)[W]) {
+    const E *err = static_cast<const E *>(a.err) + column;
+    int i = first;
+    for (; i + 3 * step < end; i += 4 * step) {
+        float v[4][W];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) fetch_some<E, W>(err + a.slots[i + u * step] * a.err_stride, count, v[u], 0.0f);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+    }
+    for (; i < end; i += step) {
+        float v[W];
+        fetch_some<E, W>(err + a.slots[i] * a.err_stride, count, v, 0.0f);
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum[q] += v[q];
+    }
+}
+
+// the sums of a workgroup's groups, in the first group
+template <int W>
+__device__ __forceinline__ void join_groups(int lanes, float (&sum)[W]) {
+    __shared__ float parts[256 * W];
+    const int x = threadIdx.x % lanes, g = threadIdx.x / lanes, groups = 256 / lanes;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < W; ++q) parts[(g * W + q) * lanes + x] = sum[q];
+    __syncthreads();
+    if (g == 0)
+        for (int o = 1; o < groups; ++o)
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] += parts[(o * W + q) * lanes + x];
+}
+
+// Pieces of the sorted list that lie within one token's run: their sums.  blockIdx.x: the piece, blockIdx.y: the columns.
+template <typename E, int W>
+__global__ __launch_bounds__(256) void embed_piece_kernel(const SumArgs a) {
+    const int begin = blockIdx.x * a.piece, end = begin + a.piece;
+    if (end > *a.total || a.keys[begin] != a.keys[end - 1]) return;
+    const int x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
+    const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    float sum[W] = {};
+    if (count > 0) add_entries<E, W>(a, begin + g, end, 256 / a.lanes, column, count, sum);
+    join_groups<W>(a.lanes, sum);
+    if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)blockIdx.x * a.D + column, count, sum);
+}
+
+template <typename G, int W>
+__device__ __forceinline__ void write_row(const SumArgs &a, int row, bool any, int column, int count, float (&sum)[W]) {
+    if (count <= 0 || (a.accumulate && !any)) return;
+    G *to = static_cast<G *>(a.grad) + row * a.grad_stride + column;
+    float old[W];
+    if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
+#pragma unroll
+    for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + sum[q] * a.scale : sum[q] * a.scale;
+    put_some<G, W>(to, count, sum);
+}
+
+// first entry of the sorted list whose token is not below v
+__device__ __forceinline__ int lower_bound(const int *keys, int n, int v) {
+    int lo = 0;
+    for (int len = n; len > 0;) {
+        const int half = len / 2;
+        if (keys[lo + half] < v) {
+            lo += half + 1;
+            len -= half + 1;
+        } else {
+            len = half;
+        }
+    }
+    return lo;
+}
+
+// The table's rows.  A workgroup holds as many rows as it has groups of `lanes` threads: short runs are added up by a group each, long ones
+// by all groups, whole pieces by their sums.
+template <typename E, typename G, int W>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
+    __shared__ int bounds[257];
+    const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
+    const long base = (long)blockIdx.x * groups;
+    const int n = *a.total;
+    for (int i = threadIdx.x; i <= groups; i += 256) bounds[i] = base + i >= a.V ? n : lower_bound(a.keys, n, (int)(base + i));
+    __syncthreads();
+    const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    {
+        const int begin = bounds[g], end = bounds[g + 1];
+        if (base + g < a.V && end - begin <= kShortRun) {
+            float sum[W] = {};
+            if (count > 0) add_entries<E, W>(a, begin, end, 1, column, count, sum);
+            write_row<G, W>(a, (int)(base + g), end > begin, column, count, sum);
+        }
+    }
+    for (int r = 0; r < groups && base + r < a.V; ++r) {
+        const int begin = bounds[r], end = bounds[r + 1];
+        if (end - begin <= kShortRun) continue;
+        float sum[W] = {};
+        const int first = (begin + a.piece - 1) / a.piece, behind = end / a.piece;  // the whole pieces
+        if (count > 0) {
+            if (first >= behind) {
+                add_entries<E, W>(a, begin + g, end, groups, column, count, sum);
+            } else {
+                add_entries<E, W>(a, begin + g, first * a.piece, groups, column, count, sum);
+                for (int p = first + g; p < behind; p += groups) {
+                    float v[W];
+                    fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
+#pragma unroll
+                    for (int q = 0; q < W; ++q) sum[q] += v[q];
+                }
+                add_entries<E, W>(a, behind * a.piece + g, end, groups, column, count, sum);
+            }
+        }
+        join_groups<W>(a.lanes, sum);
+        if (g == 0) write_row<G, W>(a, (int)(base + r), true, column, count, sum);
+    }
+}
+
+template <typename E, typename G>
+int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
+    constexpr int W = kWide<E>;
+    SumArgs a = args;
+    a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
+    const unsigned tiles = (unsigned)((a.D + a.lanes * W - 1) / (a.lanes * W));
+    const long pieces = N / a.piece;
+    if (pieces > 0) hipLaunchKernelGGL((embed_piece_kernel<E, W>), dim3((unsigned)pieces, tiles), dim3(256), 0, stream, a);
+    const long rows = (a.V + 256L / a.lanes - 1) / (256 / a.lanes);
+    CNT_REQUIRE(rows < 1L << 24 && tiles < 1u << 16, "embed_backward: the table is too large");
+    hipLaunchKernelGGL((embed_rows_kernel<E, G, W>), dim3((unsigned)rows, tiles), dim3(256), 0, stream, a);
+    CNT_HIP(hipGetLastError());
+    return CNT_OK;
+}
+
+}  // namespace
+}  // namespace cnt
+
+extern "C" {
+
+int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const void *table, long table_stride, const int *tokens,
+                      float scale, int out_type, void *out, long out_stride) {
+    using namespace cnt;
+    CNT_REQUIRE(V > 0 && D > 0 && N >= 0, "embed_forward: bad sizes");
+    CNT_REQUIRE(known_type(table_type) && known_type(out_type), "embed_forward: unknown element type");
+    CNT_REQUIRE(table_stride >= 0 && out_stride >= D, "embed_forward: rows of the output overlap, or a negative stride");
+    CNT_REQUIRE(table && (N == 0 || (tokens && out)), "embed_forward: null argument");
+    if (N == 0) return CNT_OK;
+    LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + 7) / 8)), scale};
+    const long blocks = (N + 256 / a.lanes - 1) / (256 / a.lanes);
+    CNT_REQUIRE(blocks < 1L << 24, "embed_forward: too many slots");
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    ProfileScope prof(stream, "embed_forward");
+    with_type(table_type, [&](auto t) {
+        with_type(out_type, [&](auto o) {
+            hipLaunchKernelGGL((embed_lookup_kernel<typename decltype(t)::type, typename decltype(o)::type>), dim3((unsigned)blocks),
+                               dim3(256), 0, stream, a);
+        });
+    });
+    CNT_HIP(hipGetLastError());
+    return CNT_OK;
+}
+
+long cnt_embed_scratch(int V, int D, long N) {
+    if (V <= 0 || D <= 0 || N < 0 || N > 0x3fffffffL) return -1;
+    return (long)cnt::sort_plan(V, D, N).bytes;
+}
+
+int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
+                       long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,
+                       size_t scratch_bytes) {
+    using namespace cnt;
+    CNT_REQUIRE(V > 0 && D > 0 && N >= 0 && N <= 0x3fffffffL, "embed_backward: bad sizes");
+    CNT_REQUIRE(known_type(err_type) && known_type(grad_type), "embed_backward: unknown element type");
+    CNT_REQUIRE(err_stride >= 0 && grad_stride >= D, "embed_backward: rows of the gradient overlap, or a negative stride");
+    CNT_REQUIRE(grad && scratch && (N == 0 || (tokens && err)), "embed_backward: null argument");
+    const SortPlan plan = sort_plan(V, D, N);
+    CNT_REQUIRE(scratch_bytes >= plan.bytes, "embed_backward: %zu bytes of scratch memory, %zu are needed", scratch_bytes, plan.bytes);
+    CNT_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embed_backward: the scratch memory is not aligned to 16 bytes");
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    ProfileScope prof(stream, "embed_backward");
+    char *mem = static_cast<char *>(scratch);
+    auto ints = [&](size_t at) { return reinterpret_cast<int *>(mem + at); };
+    SortArgs s = {};
+    s.counts = ints(plan.counts); s.total = ints(plan.total);
+    s.N = (int)N; s.V = V; s.bits = plan.bits; s.block = plan.block;
+    for (int pass = 0; pass < plan.passes; ++pass) {
+        const int to = pass & 1;
+        s.keys = pass ? ints(plan.keys[1 - to]) : tokens;
+        s.slots = pass ? ints(plan.slots[1 - to]) : nullptr;
+        s.keys_out = ints(plan.keys[to]); s.slots_out = ints(plan.slots[to]);
+        s.shift = pass * plan.bits;
+        const dim3 grid((unsigned)plan.blocks), block(256);
+        if (pass == 0) {
+            hipLaunchKernelGGL(token_count_kernel<true>, grid, block, 0, stream, s);
+            hipLaunchKernelGGL(token_place_kernel<true>, grid, block, 0, stream, s);
+        } else {
+            hipLaunchKernelGGL(token_count_kernel<false>, grid, block, 0, stream, s);
+            hipLaunchKernelGGL(token_place_kernel<false>, grid, block, 0, stream, s);
+        }
+        CNT_HIP(hipGetLastError());
+    }
+    const int last = (plan.passes - 1) & 1;
+    SumArgs a = {};
+    a.keys = ints(plan.keys[last]); a.slots = ints(plan.slots[last]); a.total = s.total;
+    a.err = err; a.grad = grad; a.partial = reinterpret_cast<float *>(mem + plan.partial);
+    a.err_stride = err_stride; a.grad_stride = grad_stride;
+    a.V = V; a.D = D; a.piece = plan.piece; a.accumulate = accumulate; a.scale = scale;
+    int status = CNT_OK;
+    with_type(err_type, [&](auto e) {
+        with_type(grad_type, [&](auto g) { status = sum_runs<typename decltype(e)::type, typename decltype(g)::type>(stream, a, N); });
+    });
+    return status;
+}
+
+}  // extern "C"

@@ -488,6 +488,11 @@ std::string get_str(const json::Value &o, const char *key) {
 }  // namespace
 }  // namespace cnt
 
+namespace cnt {
+// cnt_network_update; clip: norm of the gradients and the factor to multiply them with (device), or NULL
+int network_update(cnt_network *net, void *stream, int option, float learning_rate, float momentum, float frac_length, const float *clip);
+}  // namespace cnt
+
 struct cnt_network {
     std::vector<cnt::NetLayer> layers;
     int S = 0, maxT = 0, T = 0, Tmin = 0;
@@ -524,6 +529,7 @@ struct cnt_network {
     int stats_option = -1;
     float *block_sums = nullptr;  // of wavenet_block_weights, whose launches go to one stream one after the other
     float *adam_accum = nullptr;  // beta1^t, beta2^t of Adam's bias correction (device)
+    cnt_gradients *gradients = nullptr;  // all weight updates, for clipped updates (made by the first one)
     int mdn_target_start = 0, mdn_classes = 0;
     // set on the device by an LSTM recursion that gives up; the optimizer step looks at it and leaves the weights alone
     int *veto = nullptr;
@@ -1220,6 +1226,7 @@ int cnt_network_destroy(cnt_network *net) {
         if (L.mdn) cnt_mdn_destroy(L.mdn);
         if (L.dft) cnt_dft_destroy(L.dft);
     }
+    cnt_gradients_destroy(net->gradients);
     for (void *p : net->allocations) (void)hipFree(p);
     if (net->side_user) cnt::release_side(net);
     if (net->own_side) {
@@ -2331,8 +2338,27 @@ int cnt_network_set_wait_bounds(cnt_network *net, int layer_index, unsigned spin
     return cnt_lstm_set_wait_bounds(net->layers[(size_t)layer_index].lstm, spin_limit, poll_delay_backward, poll_delay_forward);
 }
 
-int cnt_network_update(cnt_network *net, void *stream_, int option, float learning_rate, float momentum,
-                       float frac_length) {
+int cnt_network_update(cnt_network *net, void *stream, int option, float learning_rate, float momentum, float frac_length) {
+    return cnt::network_update(net, stream, option, learning_rate, momentum, frac_length, nullptr);
+}
+
+int cnt_network_update_clipped(cnt_network *net, void *stream, int option, float learning_rate, float momentum, float frac_length,
+                               float max_norm, float *result) {
+    using namespace cnt;
+    CNT_REQUIRE(net && result, "network_update_clipped: null argument");
+    CNT_REQUIRE(max_norm > 0, "network_update_clipped: the largest norm has to be positive");
+    if (!net->gradients) {
+        const void *updates = net->updates;
+        const long n = net->n_weights;
+        const int type = CNT_F32;
+        CNT_TRY(cnt_gradients_create(1, &updates, nullptr, &n, &type, &net->gradients));
+    }
+    CNT_TRY(cnt_opt_grad_norm(net->gradients, stream, max_norm, result));
+    return network_update(net, stream, option, learning_rate, momentum, frac_length, result);
+}
+
+extern "C++" int cnt::network_update(cnt_network *net, void *stream_, int option, float learning_rate, float momentum,
+                                     float frac_length, const float *clip) {
     using namespace cnt;
     CNT_REQUIRE(net, "network_update: null handle");
     // A pass whose recursion gave up must not reach the weights.  Two nets: launches that have already ended are
@@ -2372,7 +2398,7 @@ int cnt_network_update(cnt_network *net, void *stream_, int option, float learni
     if (!own_rates)
         return opt_step_guarded(static_cast<hipStream_t>(stream_), option, (long)n, net->weights, net->updates, net->cur_updates,
                                 net->stats, net->deltas, nullptr, frac_length, 0.0f, 0.0f, learning_rate, momentum, net->veto,
-                                accum_dev);
+                                accum_dev, clip);
     // a layer's own "learningRate" replaces the optimizer's (optimizers/SteepestDescentOptimizer.cu:402-403, :425-426): one
     // launch per trainable layer
     for (const auto &L : net->layers) {
@@ -2382,7 +2408,8 @@ int cnt_network_update(cnt_network *net, void *stream_, int option, float learni
         float *st = net->stats ? net->stats + (adam ? 2 * o : o) : nullptr;
         CNT_TRY(opt_step_guarded(static_cast<hipStream_t>(stream_), option, c, net->weights + o, net->updates + o,
                                  net->cur_updates + o, st, net->deltas + o, nullptr, frac_length, 0.0f, 0.0f,
-                                 L.learning_rate > -0.5f ? L.learning_rate : learning_rate, momentum, net->veto, accum_dev));
+                                 L.learning_rate > -0.5f ? L.learning_rate : learning_rate, momentum, net->veto, accum_dev,
+                                 clip));
     }
     return CNT_OK;
 }

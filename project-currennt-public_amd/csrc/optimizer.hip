@@ -32,6 +32,7 @@ struct OptArgs {
     float frac_length, beta1_accum, beta2_accum, learning_rate, momentum;
     const int *veto;             // optional device flag: non-zero means the gradients are invalid, nothing is touched
     const float *accum_dev;      // optional: Adam's two bias-correction products in device memory (replace the two floats)
+    const float *clip;           // optional: norm of all gradients and the factor to multiply this fraction's gradient with
 };
 
 __device__ __forceinline__ bool bad(float g) { return isnan(g) || isinf(g); }
@@ -103,6 +104,11 @@ __device__ __forceinline__ void optimize(const OptArgs &a, size_t i) {
     }
     if (UPDATE) { fetch<N>(a.deltas + i, delta); fetch<N>(a.weights + i, w); }
     if (a.mask) fetch<N>(a.mask + i, mask);
+    if (LAYER && a.clip) {
+        const float factor = a.clip[1];
+#pragma unroll
+        for (int q = 0; q < N; ++q) g[q] = factor == 0.0f ? 0.0f : g[q] * factor;
+    }
 #pragma unroll
     for (int q = 0; q < N; ++q) {
         float x = !LAYER ? cur[q] : a.add ? g[q] + cur[q] : g[q];
@@ -210,7 +216,16 @@ int cnt_opt_step(void *stream, int option, long n, float *weights, const float *
                  float beta2_accum, float learning_rate, float momentum) {
     return cnt::opt_step_guarded(static_cast<hipStream_t>(stream), option, n, weights, layer_updates, cur_updates, stats,
                                  weight_deltas, mask, frac_length, beta1_accum, beta2_accum, learning_rate, momentum, nullptr,
-                                 nullptr);
+                                 nullptr, nullptr);
+}
+
+int cnt_opt_step_clipped(void *stream, int option, long n, float *weights, const float *layer_updates, float *cur_updates,
+                         float *stats, float *weight_deltas, const float *mask, float frac_length, float beta1_accum,
+                         float beta2_accum, float learning_rate, float momentum, const float *clip) {
+    using namespace cnt;
+    CNT_REQUIRE(clip, "opt_step_clipped: null argument");
+    return opt_step_guarded(static_cast<hipStream_t>(stream), option, n, weights, layer_updates, cur_updates, stats, weight_deltas,
+                            mask, frac_length, beta1_accum, beta2_accum, learning_rate, momentum, nullptr, nullptr, clip);
 }
 
 extern "C++" int cnt::opt_adam_advance(hipStream_t stream, float *accum_dev, const int *veto) {
@@ -222,7 +237,7 @@ extern "C++" int cnt::opt_adam_advance(hipStream_t stream, float *accum_dev, con
 extern "C++" int cnt::opt_step_guarded(hipStream_t stream, int option, long n, float *weights, const float *layer_updates,
                                        float *cur_updates, float *stats, float *weight_deltas, const float *mask,
                                        float frac_length, float beta1_accum, float beta2_accum, float learning_rate,
-                                       float momentum, const int *veto, const float *accum_dev) {
+                                       float momentum, const int *veto, const float *accum_dev, const float *clip) {
     using namespace cnt;
     CNT_REQUIRE(n >= 0 && (n == 0 || (weights && layer_updates && cur_updates && weight_deltas)), "opt_step: bad argument");
     CNT_REQUIRE(known_option(option), "opt_step: unknown optimizer option %d", option);
@@ -236,6 +251,7 @@ extern "C++" int cnt::opt_step_guarded(hipStream_t stream, int option, long n, f
     a.learning_rate = learning_rate; a.momentum = momentum;
     a.veto = veto;
     a.accum_dev = accum_dev;
+    a.clip = clip;
     ProfileScope prof(stream, "opt_step");
     return launch_optimizer<3>(stream, a);
 }
