@@ -431,87 +431,109 @@ def opt_step(option, weights, layer_updates, cur_updates, stats, deltas, mask, f
                              beta2_accum, learning_rate, momentum))
 
 
-# ---- operators over symbols: tensors of 32 and 16 bits, rows at any stride; every call checks what it is given ----
+# ---- operators over symbols: tensors of 32 and 16 bits, rows at any stride; every call checks what it is given.  A call of a few rows
+# takes a few microseconds on the device, so the checks below are spared what costs as much (torch's device objects, names of types).
 
-_ELEMENTS = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
-_element_codes = {}  # torch.dtype -> code of the library
+class _Types:
+    """torch and its types once the first call has imported it"""
+
+    torch = float32 = int32 = None
+    codes = {}
+
+    @classmethod
+    def load(cls):
+        import torch
+
+        cls.float32, cls.int32 = torch.float32, torch.int32
+        cls.codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        cls.torch = torch
 
 
 def _element(name, t):
-    code = _element_codes.get(t.dtype)
+    code = _Types.codes.get(t.dtype)
     if code is None:
-        code = _ELEMENTS.get(str(t.dtype))
+        _Types.load()
+        code = _Types.codes.get(t.dtype)
         if code is None:
             raise ValueError("%s: float32, bfloat16 or float16 is wanted, not %s" % (name, t.dtype))
-        _element_codes[t.dtype] = code
     return code
 
 
-def _on_device(name, t, device):
-    if t.device != device or device.type != "cuda":
-        raise ValueError("%s is on %s, the call on %s" % (name, t.device, device))
+def _index(name, t):
+    """number of the device that a call runs on: that of its first tensor"""
+    if _Types.torch is None:
+        _Types.load()
+    i = t.get_device()
+    if i < 0:
+        raise ValueError("%s is on %s, a GPU is wanted" % (name, t.device))
+    return i
 
 
-def _matrix(name, t, device, shape=None):
+def _matrix(name, t, index, rows=None, columns=None):
     """The row stride of a matrix whose rows are contiguous."""
-    _on_device(name, t, device)
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError("%s: a matrix%s is wanted, not %s" % (name, "" if shape is None else " of %d x %d" % shape, tuple(t.shape)))
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if t.get_device() != index:
+        raise ValueError("%s is on %s, the call on cuda:%d" % (name, t.device, index))
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and (shape[0] != rows or shape[1] != columns)):
+        raise ValueError("%s: a matrix%s is wanted, not %s" % (name, "" if rows is None else " of %d x %d" % (rows, columns), tuple(shape)))
+    stride = t.stride()
+    if shape[1] > 1 and stride[1] != 1:
         raise ValueError("%s: the values of a row have to be contiguous" % name)
-    return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+    return stride[0] if shape[0] > 1 else max(1, shape[1])
 
 
-def _vector(name, t, dtype, count, device):
-    """A contiguous vector of `count` values (or None)."""
+def _vector(name, t, dtype, count, index):
+    """Address of a contiguous vector of `count` values (None: of none)."""
     if t is None:
-        return
-    _on_device(name, t, device)
-    if str(t.dtype) != "torch." + dtype or t.numel() != count or not t.is_contiguous():
+        return None
+    if t.get_device() != index:
+        raise ValueError("%s is on %s, the call on cuda:%d" % (name, t.device, index))
+    if t.dtype is not dtype or t.numel() != count or not t.is_contiguous():
         raise ValueError("%s: %d contiguous values of %s are wanted, not %s of %s" % (name, count, dtype, tuple(t.shape), t.dtype))
+    return t.data_ptr()
 
 
-def _enqueue(device, stream, call):
-    """call(stream pointer) on `stream`, or on the device's current one."""
-    import torch
-
-    if stream is not None and stream.device != device:
-        raise ValueError("the stream is on %s, the tensors are on %s" % (stream.device, device))
-    if torch.cuda.current_device() == device.index:
-        check(call(stream_ptr(stream)))
+def _enqueue(index, stream, function, *args):
+    """The call on `stream`, or on the device's current one."""
+    torch = _Types.torch
+    if stream is None:
+        raw = torch._C._cuda_getCurrentRawStream(index)
+    elif stream.device_index != index:
+        raise ValueError("the stream is on %s, the tensors are on cuda:%d" % (stream.device, index))
     else:
-        with torch.cuda.device(device):
-            check(call(stream_ptr(stream)))
+        raw = stream.cuda_stream
+    if torch._C._cuda_getDevice() == index:
+        status = function(raw, *args)
+    else:
+        with torch.cuda.device(index):
+            status = function(raw, *args)
+    if status != CNT_OK:
+        check(status)
 
 
-def _scratch(scratch, need, device, stream):
-    """`scratch`, or memory of the calling stream's pool where there is none."""
-    import torch
-
+def _scratch(scratch, need, index, stream):
+    """(address, bytes) of scratch memory: the caller's, or some of the calling stream's pool; and what keeps it."""
     if need < 0:
         raise ValueError("sizes out of range")
-    if scratch is not None:
-        _on_device("scratch", scratch, device)
-        if not scratch.is_contiguous():
-            raise ValueError("scratch: contiguous memory is wanted")
-        return scratch
-    if need == 0:
-        return None
-    with torch.cuda.device(device), torch.cuda.stream(stream):
-        return torch.empty(need, dtype=torch.uint8, device=device)
-
-
-def _bytes(t):
-    return 0 if t is None else t.numel() * t.element_size()
+    if scratch is None:
+        if need == 0:
+            return None, 0, None
+        torch = _Types.torch
+        with torch.cuda.device(index), torch.cuda.stream(stream):
+            scratch = torch.empty(need, dtype=torch.uint8, device="cuda")
+    elif scratch.get_device() != index or not scratch.is_contiguous():
+        raise ValueError("scratch: contiguous memory on cuda:%d is wanted" % index)
+    return scratch.data_ptr(), scratch.numel() * scratch.element_size(), scratch
 
 
 def embed_forward(table, tokens, out, scale=1.0, stream=None):
     """out[n] = scale * table[tokens[n]]; zeros where tokens[n] is no row of the table (see cnt_embed_forward)."""
-    device, (V, D), N = table.device, table.shape, tokens.numel()
-    ts, os_ = _matrix("table", table, device), _matrix("out", out, device, (N, D))
-    _vector("tokens", tokens, "int32", N, device)
-    args = (V, D, N, _element("table", table), ptr(table), ts, ptr(tokens), scale, _element("out", out), ptr(out), os_)
-    _enqueue(device, stream, lambda s: lib().cnt_embed_forward(s, *args))
+    index, N = _index("table", table), tokens.numel()
+    table_stride = _matrix("table", table, index)
+    V, D = table.shape
+    out_stride = _matrix("out", out, index, N, D)
+    _enqueue(index, stream, lib().cnt_embed_forward, V, D, N, _element("table", table), table.data_ptr(), table_stride,
+             _vector("tokens", tokens, _Types.int32, N, index), scale, _element("out", out), out.data_ptr(), out_stride)
 
 
 def embed_scratch(V, D, N):
@@ -524,13 +546,14 @@ def embed_scratch(V, D, N):
 
 def embed_backward(tokens, err, grad, scale=1.0, accumulate=False, scratch=None, stream=None):
     """grad[v] = scale * sum of err[n] over the slots with tokens[n] = v, added to what grad holds if asked (see cnt_embed_backward)."""
-    device, (V, D), N = grad.device, grad.shape, tokens.numel()
-    gs, es = _matrix("grad", grad, device), _matrix("err", err, device, (N, D))
-    _vector("tokens", tokens, "int32", N, device)
-    scratch = _scratch(scratch, lib().cnt_embed_scratch(V, D, N), device, stream)
-    args = (V, D, N, ptr(tokens), scale, _element("err", err), ptr(err), es, _element("grad", grad), ptr(grad), gs, int(accumulate),
-            ptr(scratch), _bytes(scratch))
-    _enqueue(device, stream, lambda s: lib().cnt_embed_backward(s, *args))
+    index, N = _index("grad", grad), tokens.numel()
+    grad_stride = _matrix("grad", grad, index)
+    V, D = grad.shape
+    err_stride = _matrix("err", err, index, N, D)
+    address, size, keep = _scratch(scratch, lib().cnt_embed_scratch(V, D, N), index, stream)
+    _enqueue(index, stream, lib().cnt_embed_backward, V, D, N, _vector("tokens", tokens, _Types.int32, N, index), scale,
+             _element("err", err), err.data_ptr(), err_stride, _element("grad", grad), grad.data_ptr(), grad_stride, int(accumulate),
+             address, size)
 
 
 def logprob_scratch(N, V, K=0):
@@ -541,58 +564,58 @@ def logprob_scratch(N, V, K=0):
     return need
 
 
-def _row_results(device, N, tokens, **vectors):
-    _vector("tokens", tokens, "int32", N, device)
-    for name, t in vectors.items():
-        _vector(name, t, "float32", N, device)
-
-
 def logprob_forward(logits, tokens=None, logp=None, lse=None, entropy=None, top_logp=None, top_tokens=None, scale=1.0, scratch=None,
                     stream=None):
     """Log probabilities of given tokens, log sums, entropies and the most probable alternatives of every row, into the tensors
     that are given (see cnt_logprob_forward); top_logp and top_tokens are N x K."""
-    device, (N, V) = logits.device, logits.shape
-    stride = _matrix("logits", logits, device)
-    _row_results(device, N, tokens, logp=logp, lse=lse, entropy=entropy)
+    index = _index("logits", logits)
+    stride = _matrix("logits", logits, index)
+    N, V = logits.shape
+    float32, int32 = _Types.float32, _Types.int32
     K = 0
-    for name, t, dtype in (("top_logp", top_logp, "float32"), ("top_tokens", top_tokens, "int32")):
+    for name, t in (("top_logp", top_logp), ("top_tokens", top_tokens)):
         if t is not None:
-            if t.dim() != 2 or t.shape[0] != N or (K and t.shape[1] != K):
-                raise ValueError("%s: a row of alternatives for each of %d rows is wanted, not %s" % (name, N, tuple(t.shape)))
-            K = t.shape[1]
-            _vector(name, t, dtype, N * K, device)
-    scratch = _scratch(scratch, lib().cnt_logprob_scratch(N, V, K) if K <= 64 else 0, device, stream)
-    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(logp), ptr(lse), ptr(entropy), K,
-            ptr(top_logp), ptr(top_tokens), ptr(scratch), _bytes(scratch))
-    _enqueue(device, stream, lambda s: lib().cnt_logprob_forward(s, *args))
+            shape = t.shape
+            if len(shape) != 2 or shape[0] != N or (K and shape[1] != K):
+                raise ValueError("%s: a row of alternatives for each of %d rows is wanted, not %s" % (name, N, tuple(shape)))
+            K = shape[1]
+    address, size, keep = _scratch(scratch, lib().cnt_logprob_scratch(N, V, K) if K <= 64 else 0, index, stream)
+    _enqueue(index, stream, lib().cnt_logprob_forward, N, V, _element("logits", logits), logits.data_ptr(), stride, scale,
+             _vector("tokens", tokens, int32, N, index), _vector("logp", logp, float32, N, index), _vector("lse", lse, float32, N, index),
+             _vector("entropy", entropy, float32, N, index), K, _vector("top_logp", top_logp, float32, N * K, index),
+             _vector("top_tokens", top_tokens, int32, N * K, index), address, size)
 
 
-def _error_rows(logits, err):
-    device, (N, V) = logits.device, logits.shape
-    if err.dtype != logits.dtype:
+def _error_rows(logits, err, index):
+    if err.dtype is not logits.dtype:
         raise ValueError("err: the errors have the logits' type, %s, not %s" % (logits.dtype, err.dtype))
-    return _matrix("logits", logits, device), _matrix("err", err, device, (N, V))
+    return _matrix("logits", logits, index), _matrix("err", err, index, *logits.shape)
 
 
 def logprob_backward(logits, tokens, lse, entropy, logp_err, entropy_err, err, scale=1.0, stream=None):
     """Errors of the logits from those of logp and entropy, either of which may be None (see cnt_logprob_backward)."""
-    device, (N, V) = logits.device, logits.shape
-    stride, err_stride = _error_rows(logits, err)
-    _row_results(device, N, tokens, lse=lse, entropy=entropy, logp_err=logp_err, entropy_err=entropy_err)
-    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(lse), ptr(entropy), ptr(logp_err),
-            ptr(entropy_err), ptr(err), err_stride)
-    _enqueue(device, stream, lambda s: lib().cnt_logprob_backward(s, *args))
+    index = _index("logits", logits)
+    stride, err_stride = _error_rows(logits, err, index)
+    N, V = logits.shape
+    float32 = _Types.float32
+    _enqueue(index, stream, lib().cnt_logprob_backward, N, V, _element("logits", logits), logits.data_ptr(), stride, scale,
+             _vector("tokens", tokens, _Types.int32, N, index), _vector("lse", lse, float32, N, index),
+             _vector("entropy", entropy, float32, N, index), _vector("logp_err", logp_err, float32, N, index),
+             _vector("entropy_err", entropy_err, float32, N, index), err.data_ptr(), err_stride)
 
 
 def logprob_error_backward(logits, tokens, logp_err, entropy_err, logp, lse, entropy, err, scale=1.0, scratch=None, stream=None):
     """logprob_forward and logprob_backward in one call, for errors that are known before (see cnt_logprob_error_backward)."""
-    device, (N, V) = logits.device, logits.shape
-    stride, err_stride = _error_rows(logits, err)
-    _row_results(device, N, tokens, logp_err=logp_err, entropy_err=entropy_err, logp=logp, lse=lse, entropy=entropy)
-    scratch = _scratch(scratch, lib().cnt_logprob_scratch(N, V, 0), device, stream)
-    args = (N, V, _element("logits", logits), ptr(logits), stride, scale, ptr(tokens), ptr(logp_err), ptr(entropy_err), ptr(logp),
-            ptr(lse), ptr(entropy), ptr(err), err_stride, ptr(scratch), _bytes(scratch))
-    _enqueue(device, stream, lambda s: lib().cnt_logprob_error_backward(s, *args))
+    index = _index("logits", logits)
+    stride, err_stride = _error_rows(logits, err, index)
+    N, V = logits.shape
+    float32 = _Types.float32
+    address, size, keep = _scratch(scratch, lib().cnt_logprob_scratch(N, V, 0), index, stream)
+    _enqueue(index, stream, lib().cnt_logprob_error_backward, N, V, _element("logits", logits), logits.data_ptr(), stride, scale,
+             _vector("tokens", tokens, _Types.int32, N, index), _vector("logp_err", logp_err, float32, N, index),
+             _vector("entropy_err", entropy_err, float32, N, index), _vector("logp", logp, float32, N, index),
+             _vector("lse", lse, float32, N, index), _vector("entropy", entropy, float32, N, index), err.data_ptr(), err_stride,
+             address, size)
 
 
 class GradientSet:
@@ -600,24 +623,22 @@ class GradientSet:
     in place).  Holds on to the tensors; a gradient that is replaced by another tensor needs another set."""
 
     def __init__(self, gradients, clipped=None):
-        import torch
-
         self.handle = VP()
+        if _Types.torch is None:
+            _Types.load()
         self.gradients, self.clipped = list(gradients), None if clipped is None else list(clipped)
         n = len(self.gradients)
         if self.clipped is not None and len(self.clipped) != n:
             raise ValueError("%d gradients and %d places for them" % (n, len(self.clipped)))
-        self.device = self.gradients[0].device if n else torch.device("cuda", torch.cuda.current_device())
+        self.index = _index("gradient 0", self.gradients[0]) if n else _Types.torch.cuda.current_device()
         for i, g in enumerate(self.gradients):
-            to = g if self.clipped is None else self.clipped[i]
-            for name, t in (("gradient", g), ("clipped gradient", to)):
-                _on_device("%s %d" % (name, i), t, self.device)
-                if not t.is_contiguous() or t.shape != g.shape or t.dtype != g.dtype:
-                    raise ValueError("%s %d: contiguous %s of shape %s is wanted" % (name, i, g.dtype, tuple(g.shape)))
+            for name, t in (("gradient", g), ("clipped gradient", g if self.clipped is None else self.clipped[i])):
+                if t.get_device() != self.index or not t.is_contiguous() or t.shape != g.shape or t.dtype != g.dtype:
+                    raise ValueError("%s %d: contiguous %s of shape %s on cuda:%d is wanted" % (name, i, g.dtype, tuple(g.shape), self.index))
         sizes = (C.c_long * n)(*[g.numel() for g in self.gradients])
         types = (I * n)(*[_element("gradient %d" % i, g) for i, g in enumerate(self.gradients)])
         to = None if self.clipped is None else _ptr_array(self.clipped)
-        with torch.cuda.device(self.device):
+        with _Types.torch.cuda.device(self.index):
             check(lib().cnt_gradients_create(n, _ptr_array(self.gradients), to, sizes, types, C.byref(self.handle)))
 
     def close(self):
@@ -634,20 +655,23 @@ class GradientSet:
 
 def opt_grad_norm(gradient_set, max_norm, result, stream=None):
     """result = [norm of all gradients of the set, factor that brings it down to max_norm] (see cnt_opt_grad_norm)."""
-    _vector("result", result, "float32", 2, gradient_set.device)
-    _enqueue(gradient_set.device, stream, lambda s: lib().cnt_opt_grad_norm(gradient_set.handle, s, max_norm, ptr(result)))
+    index = gradient_set.index
+    address = _vector("result", result, _Types.float32, 2, index)
+    _enqueue(index, stream, lambda raw: lib().cnt_opt_grad_norm(gradient_set.handle, raw, max_norm, address))
 
 
 def opt_clip(gradient_set, max_norm, result, stream=None):
     """opt_grad_norm, and the gradients multiplied with the factor (see cnt_opt_clip)."""
-    _vector("result", result, "float32", 2, gradient_set.device)
-    _enqueue(gradient_set.device, stream, lambda s: lib().cnt_opt_clip(gradient_set.handle, s, max_norm, ptr(result)))
+    index = gradient_set.index
+    address = _vector("result", result, _Types.float32, 2, index)
+    _enqueue(index, stream, lambda raw: lib().cnt_opt_clip(gradient_set.handle, raw, max_norm, address))
 
 
 def opt_step_clipped(option, weights, layer_updates, cur_updates, stats, deltas, mask, frac_length, beta1_accum, beta2_accum,
                      learning_rate, momentum, clip, stream=None):
     """opt_step on clip[1] * layer_updates, clip as opt_grad_norm has left it."""
-    _vector("clip", clip, "float32", 2, weights.device)
+    index = _index("weights", weights)
+    _vector("clip", clip, _Types.float32, 2, index)
     check(lib().cnt_opt_step_clipped(stream_ptr(stream), option, weights.numel(), ptr(weights), ptr(layer_updates),
                                      ptr(cur_updates), ptr(stats), ptr(deltas), ptr(mask), frac_length, beta1_accum,
                                      beta2_accum, learning_rate, momentum, ptr(clip)))
@@ -903,7 +927,8 @@ class Network:
 
     def update_clipped(self, option, learning_rate, momentum, frac_length, max_norm, result, stream=None):
         """`update` with the gradients clipped to max_norm; result (two floats on the device) receives their norm and the factor."""
-        _vector("result", result, "float32", 2, result.device)
+        index = _index("result", result)
+        _vector("result", result, _Types.float32, 2, index)
         check(lib().cnt_network_update_clipped(self.handle, stream_ptr(stream), option, learning_rate, momentum, frac_length, max_norm,
                                                ptr(result)))
 

@@ -26,33 +26,37 @@ template <typename T, int N>
 struct Packed {
     typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
-template <typename T, int N>
+// ONCE: data that is not read again soon, or not at all, goes past the caches (512 MB: reads 6.3 -> 6.9 TB/s, copies 5.6 -> 6.2).
+template <typename T, int N, bool ONCE = false>
 __device__ __forceinline__ void fetch_elements(const T *p, float (&v)[N]) {
-    const typename Packed<T, N>::type x = *reinterpret_cast<const typename Packed<T, N>::type *>(p);
+    const auto *from = reinterpret_cast<const typename Packed<T, N>::type *>(p);
+    const typename Packed<T, N>::type x = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)x[i];
 }
-template <typename T, int N>
+template <typename T, int N, bool ONCE = false>
 __device__ __forceinline__ void put_elements(T *p, const float (&v)[N]) {
     typename Packed<T, N>::type x;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = (T)v[i];
-    *reinterpret_cast<typename Packed<T, N>::type *>(p) = x;
+    auto *to = reinterpret_cast<typename Packed<T, N>::type *>(p);
+    if (ONCE) __builtin_nontemporal_store(x, to);
+    else *to = x;
 }
 // the first `count` of N, 0 <= count <= N
-template <typename T, int N>
+template <typename T, int N, bool ONCE = false>
 __device__ __forceinline__ void fetch_some(const T *p, int count, float (&v)[N], float rest) {
     if (count == N) {
-        fetch_elements<T, N>(p, v);
+        fetch_elements<T, N, ONCE>(p, v);
         return;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = i < count ? (float)p[i] : rest;
 }
-template <typename T, int N>
+template <typename T, int N, bool ONCE = false>
 __device__ __forceinline__ void put_some(T *p, int count, const float (&v)[N]) {
     if (count == N) {
-        put_elements<T, N>(p, v);
+        put_elements<T, N, ONCE>(p, v);
         return;
     }
 #pragma unroll

@@ -44,12 +44,16 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
 }
 
 // ----- sort of the slots by token ---------------------------------------------------------------------------------------------
-constexpr int kMostBits = 10, kMostBins = 1 << kMostBits, kMostSortBlocks = 512;
+constexpr int kMostBits = 10, kMostBins = 1 << kMostBits, kMostSortBlocks = 512, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+// Up to here every workgroup counts the whole list's digits for itself, which takes less than a launch of its own for the counts.
+constexpr long kCountedTwice = 32768;
 
-// Scratch of a gradient: two lists of (token, slot), counts of every block and digit, the number of slots with a token, partial sums.
+// Scratch of a gradient: two lists of (token, slot), counts of every block and digit, the number of slots with a token, where the rows' runs
+// begin, partial sums.
 struct SortPlan {
     int bits, passes, block, blocks, piece;  // slots per block, blocks; piece: entries of the sorted list that are added up together
-    size_t keys[2], slots[2], counts, total, partial, bytes;
+    bool counted;                            // the counts are made by a launch of their own
+    size_t keys[2], slots[2], counts, total, starts, partial, bytes;
 };
 SortPlan sort_plan(long V, int D, long N) {
     SortPlan p = {};
@@ -57,10 +61,11 @@ SortPlan sort_plan(long V, int D, long N) {
     while ((1L << all) < V) ++all;
     p.passes = std::max(1, (all + kMostBits - 1) / kMostBits);
     p.bits = std::max(1, (all + p.passes - 1) / p.passes);
-    // a wave takes its quarter of a block in steps of 64 slots
-    p.block = (int)((std::max(1024L, (N + kMostSortBlocks - 1) / kMostSortBlocks) + 255) / 256 * 256);
+    p.block = (int)((std::max(1L, (N + kMostSortBlocks - 1) / kMostSortBlocks) + kSortThreads - 1) / kSortThreads * kSortThreads);
     p.blocks = (int)std::max(1L, (N + p.block - 1) / p.block);
-    p.piece = 64;
+    p.counted = N > kCountedTwice;
+    // partial sums of pieces: about as many entries in a piece as pieces in the longest runs
+    p.piece = 32;
     while (16L * p.piece * p.piece < N) p.piece *= 2;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -71,8 +76,9 @@ SortPlan sort_plan(long V, int D, long N) {
     const size_t list = (size_t)N * sizeof(int);
     p.keys[0] = take(list); p.slots[0] = take(list);
     p.keys[1] = p.passes > 1 ? take(list) : 0; p.slots[1] = p.passes > 1 ? take(list) : 0;
-    p.counts = take((size_t)p.blocks * (1 << p.bits) * sizeof(int));
+    p.counts = take(p.counted ? (size_t)p.blocks * (1 << p.bits) * sizeof(int) : 0);
     p.total = take(sizeof(int));
+    p.starts = take(((size_t)V + 1) * sizeof(int));
     p.partial = take((size_t)(N / p.piece) * D * sizeof(float));
     p.bytes = at;
     return p;
@@ -90,93 +96,85 @@ __device__ __forceinline__ int entries(const SortArgs &a) { return FIRST ? a.N :
 template <bool FIRST>
 __device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIRST || (key >= 0 && key < a.V); }
 
-// how often every digit occurs in a block of the list
+// how often every digit occurs among entries begin .. end, added to bins
 template <bool FIRST>
-__global__ __launch_bounds__(256) void token_count_kernel(const SortArgs a) {
-    __shared__ int bins[kMostBins];
-    const int n_bins = 1 << a.bits, n = entries<FIRST>(a);
-    for (int d = threadIdx.x; d < n_bins; d += 256) bins[d] = 0;
-    __syncthreads();
-    const long begin = (long)blockIdx.x * a.block, end = min((long)n, begin + a.block);
-    for (long i = begin + threadIdx.x; i < end; i += 256) {
+__device__ __forceinline__ void count_digits(const SortArgs &a, long begin, long end, int first, int step, int *bins) {
+    for (long i = begin + first; i < end; i += step) {
         const int key = a.keys[i];
-        if (listed<FIRST>(a, key)) atomicAdd(&bins[(key >> a.shift) & (n_bins - 1)], 1);
+        if (listed<FIRST>(a, key)) atomicAdd(&bins[(key >> a.shift) & ((1 << a.bits) - 1)], 1);
     }
-    __syncthreads();
-    for (int d = threadIdx.x; d < n_bins; d += 256) a.counts[blockIdx.x * n_bins + d] = bins[d];
 }
 
-// Puts a block's entries to their places.  Every block adds the blocks' counts up for itself, which saves a launch.
 template <bool FIRST>
-__global__ __launch_bounds__(256) void token_place_kernel(const SortArgs a) {
-    __shared__ int next[4][kMostBins];  // counts of a wave's entries, then the next place for every wave and digit
-    __shared__ int totals[kMostBins];
-    __shared__ int wave_totals[4];
-    const int n_bins = 1 << a.bits, n = entries<FIRST>(a), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int d = tid; d < n_bins; d += 256) {
+__global__ __launch_bounds__(kSortThreads) void token_count_kernel(const SortArgs a) {
+    __shared__ int bins[kMostBins];
+    const int n_bins = 1 << a.bits, n = entries<FIRST>(a), d = threadIdx.x;
+    bins[d] = 0;
+    __syncthreads();
+    const long begin = (long)blockIdx.x * a.block;
+    count_digits<FIRST>(a, begin, min((long)n, begin + a.block), d, kSortThreads, bins);
+    __syncthreads();
+    if (d < n_bins) a.counts[blockIdx.x * n_bins + d] = bins[d];
+}
+
+// Puts a block's entries to their places, a thread per digit and entry.  COUNTED: every block adds the blocks' counts up for itself, which
+// saves a launch; else it counts the whole list.
+template <bool FIRST, bool COUNTED>
+__global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArgs a) {
+    static_assert(kSortThreads == kMostBins, "a thread per digit");
+    __shared__ int next[kSortWaves][kMostBins];  // counts of a wave's entries, then the next place for every wave and digit
+    __shared__ int earlier[kMostBins], others[kMostBins];
+    __shared__ int wave_totals[kSortWaves];
+    const int n_bins = 1 << a.bits, n = entries<FIRST>(a), d = threadIdx.x, lane = d & 63, wave = d >> 6;
+    if (d < n_bins) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) next[w][d] = 0;
+        for (int w = 0; w < kSortWaves; ++w) next[w][d] = 0;
+        earlier[d] = others[d] = 0;
     }
     __syncthreads();
-    const int quarter = a.block / 4;
-    const long begin = (long)blockIdx.x * a.block + (long)wave * quarter, end = min((long)n, begin + quarter);
-    for (long i = begin + lane; i < end; i += 64) {
-        const int key = a.keys[i];
-        if (listed<FIRST>(a, key)) atomicAdd(&next[wave][(key >> a.shift) & (n_bins - 1)], 1);
-    }
-    int before[kMostBins / 256];
-#pragma unroll
-    for (int q = 0; q < kMostBins / 256; ++q) {
-        const int d = tid + q * 256;
-        int all = 0, earlier = 0;
+    const long block_begin = min((long)n, (long)blockIdx.x * a.block), block_end = min((long)n, block_begin + a.block);
+    const int share = a.block / kSortWaves;
+    const long begin = min((long)n, (long)blockIdx.x * a.block + (long)wave * share), end = min((long)n, begin + share);
+    count_digits<FIRST>(a, begin, end, lane, 64, next[wave]);
+    int before = 0, all = 0;
+    if (COUNTED) {
         if (d < n_bins) {
 #pragma unroll 8
             for (int b = 0; b < (int)gridDim.x; ++b) {
                 const int c = a.counts[b * n_bins + d];
                 all += c;
-                earlier += b < (int)blockIdx.x ? c : 0;
+                before += b < (int)blockIdx.x ? c : 0;
             }
-            totals[d] = all;
         }
-        before[q] = earlier;
+    } else {
+        count_digits<FIRST>(a, 0, block_begin, d, kSortThreads, earlier);
+        count_digits<FIRST>(a, block_end, n, d, kSortThreads, others);
     }
     __syncthreads();
-    // places of the digits: four neighbouring ones per thread
-    int four[4], sum = 0;
+    if (!COUNTED && d < n_bins) {
+        before = earlier[d];
+        all = before + others[d];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int d = tid * 4 + q;
-        four[q] = d < n_bins ? totals[d] : 0;
-        sum += four[q];
+        for (int w = 0; w < kSortWaves; ++w) all += next[w][d];
     }
-    int upto = sum;
+    // places of the digits
+    int upto = all;
     for (int o = 1; o < 64; o *= 2) {
         const int other = __shfl_up(upto, o);
         if (lane >= o) upto += other;
     }
     if (lane == 63) wave_totals[wave] = upto;
     __syncthreads();
-    int place = upto - sum;
-    for (int w = 0; w < wave; ++w) place += wave_totals[w];
+    int at = upto - all;
+    for (int w = 0; w < wave; ++w) at += wave_totals[w];
+    if (FIRST && blockIdx.x == 0 && d == kSortThreads - 1) *a.total = at + all;
+    at += before;
+    if (d < n_bins) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int d = tid * 4 + q;
-        if (d < n_bins) totals[d] = place;
-        place += four[q];
-    }
-    if (FIRST && blockIdx.x == 0 && tid == 255) *a.total = place;
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kMostBins / 256; ++q) {
-        const int d = tid + q * 256;
-        if (d < n_bins) {
-            int at = totals[d] + before[q];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const int c = next[w][d];
-                next[w][d] = at;
-                at += c;
-            }
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int c = next[w][d];
+            next[w][d] = at;
+            at += c;
         }
     }
     __syncthreads();
@@ -195,13 +193,13 @@ __global__ __launch_bounds__(256) void token_place_kernel(const SortArgs a) {
             same &= set ? b : ~b;
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
-        const int at = mine[digit] + rank;
+        const int place = mine[digit] + rank;
         __builtin_amdgcn_wave_barrier();
-        if (in && rank == 0) mine[digit] = at + __popcll(same);
+        if (in && rank == 0) mine[digit] = place + __popcll(same);
         __builtin_amdgcn_wave_barrier();
         if (in) {
-            a.keys_out[at] = key;
-            a.slots_out[at] = FIRST ? (int)i : a.slots[i];
+            a.keys_out[place] = key;
+            a.slots_out[place] = FIRST ? (int)i : a.slots[i];
         }
     }
 }
@@ -211,13 +209,13 @@ struct SumArgs {
     const int *keys, *slots, *total;
     const void *err;
     void *grad;
+    int *starts;  // V + 1: where the rows' runs begin in the sorted list
     float *partial;
     long err_stride, grad_stride;
     int V, D, lanes, piece, accumulate;
+    int first_blocks;  // workgroups of the first kind of a launch, in front of those of the second
     float scale;
 };
-
-constexpr int kShortRun = 32;
 
 // sum of entries first, first + step, ... < end of the sorted list, W columns from `column` on
 template <typename E, int W>
@@ -256,17 +254,42 @@ __device__ __forceinline__ void join_groups(int lanes, float (&sum)[W]) {
             for (int q = 0; q < W; ++q) sum[q] += parts[(o * W + q) * lanes + x];
 }
 
-// Pieces of the sorted list that lie within one token's run: their sums.  blockIdx.x: the piece, blockIdx.y: the columns.
+// Where the runs of the rows key(i - 1) + 1 .. key(i) begin: at entry i.  A wave for 64 entries; long gaps between two keys are filled
+// by the whole wave.
+__device__ __forceinline__ void find_starts(const SumArgs &a) {
+    const int lane = threadIdx.x & 63, n = *a.total;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    int from = 0, to = -1;  // rows whose runs begin at entry i
+    if (i <= n) {
+        from = i == 0 ? 0 : a.keys[i - 1] + 1;
+        to = i == n ? a.V : a.keys[i];
+    }
+    unsigned long long far = __ballot(to - from >= 64);
+    if (to - from < 64)
+        for (int v = from; v <= to; ++v) a.starts[v] = (int)i;
+    for (; far; far &= far - 1) {
+        const int owner = __builtin_ctzll(far), first = __builtin_amdgcn_readlane(from, owner), last = __builtin_amdgcn_readlane(to, owner);
+        const int entry = __builtin_amdgcn_readlane((int)i, owner);
+        for (long v = (long)first + lane; v <= last; v += 64) a.starts[v] = entry;
+    }
+}
+
+// First workgroups: where the runs begin.  The others: sums of the pieces of the sorted list that lie within one run.
+// blockIdx.y: the columns.
 template <typename E, int W>
-__global__ __launch_bounds__(256) void embed_piece_kernel(const SumArgs a) {
-    const int begin = blockIdx.x * a.piece, end = begin + a.piece;
+__global__ __launch_bounds__(256) void embed_pieces_kernel(const SumArgs a) {
+    if ((int)blockIdx.x < a.first_blocks) {
+        if (blockIdx.y == 0) find_starts(a);
+        return;
+    }
+    const int piece = blockIdx.x - a.first_blocks, begin = piece * a.piece, end = begin + a.piece;
     if (end > *a.total || a.keys[begin] != a.keys[end - 1]) return;
     const int x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
     const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
     float sum[W] = {};
     if (count > 0) add_entries<E, W>(a, begin + g, end, 256 / a.lanes, column, count, sum);
     join_groups<W>(a.lanes, sum);
-    if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)blockIdx.x * a.D + column, count, sum);
+    if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)piece * a.D + column, count, sum);
 }
 
 template <typename G, int W>
@@ -280,75 +303,56 @@ __device__ __forceinline__ void write_row(const SumArgs &a, int row, bool any, i
     put_some<G, W>(to, count, sum);
 }
 
-// first entry of the sorted list whose token is not below v
-__device__ __forceinline__ int lower_bound(const int *keys, int n, int v) {
-    int lo = 0;
-    for (int len = n; len > 0;) {
-        const int half = len / 2;
-        if (keys[lo + half] < v) {
-            lo += half + 1;
-            len -= half + 1;
-        } else {
-            len = half;
-        }
-    }
-    return lo;
-}
-
-// The table's rows.  A workgroup holds as many rows as it has groups of `lanes` threads: short runs are added up by a group each, long ones
-// by all groups, whole pieces by their sums.
+// First workgroups: rows whose run holds the first entry of a piece, by all groups of the workgroup of the first such piece; whole pieces go
+// by their sums.  The others: the other rows, a group of `lanes` threads for each, which have fewer entries than a piece.
 template <typename E, typename G, int W>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
-    __shared__ int bounds[257];
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
-    const long base = (long)blockIdx.x * groups;
-    const int n = *a.total;
-    for (int i = threadIdx.x; i <= groups; i += 256) bounds[i] = base + i >= a.V ? n : lower_bound(a.keys, n, (int)(base + i));
-    __syncthreads();
     const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
-    {
-        const int begin = bounds[g], end = bounds[g + 1];
-        if (base + g < a.V && end - begin <= kShortRun) {
-            float sum[W] = {};
-            if (count > 0) add_entries<E, W>(a, begin, end, 1, column, count, sum);
-            write_row<G, W>(a, (int)(base + g), end > begin, column, count, sum);
-        }
-    }
-    for (int r = 0; r < groups && base + r < a.V; ++r) {
-        const int begin = bounds[r], end = bounds[r + 1];
-        if (end - begin <= kShortRun) continue;
-        float sum[W] = {};
-        const int first = (begin + a.piece - 1) / a.piece, behind = end / a.piece;  // the whole pieces
+    float sum[W] = {};
+    if ((int)blockIdx.x < a.first_blocks) {
+        const int here = blockIdx.x * a.piece;
+        if (here >= *a.total) return;
+        const int row = a.keys[here], begin = a.starts[row], end = a.starts[row + 1];
+        if (here - begin >= a.piece) return;
+        const int whole = end / a.piece * a.piece;  // >= here
         if (count > 0) {
-            if (first >= behind) {
-                add_entries<E, W>(a, begin + g, end, groups, column, count, sum);
-            } else {
-                add_entries<E, W>(a, begin + g, first * a.piece, groups, column, count, sum);
-                for (int p = first + g; p < behind; p += groups) {
-                    float v[W];
-                    fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
+            add_entries<E, W>(a, begin + g, here, groups, column, count, sum);
+            for (int p = blockIdx.x + g; p < whole / a.piece; p += groups) {
+                float v[W];
+                fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
 #pragma unroll
-                    for (int q = 0; q < W; ++q) sum[q] += v[q];
-                }
-                add_entries<E, W>(a, behind * a.piece + g, end, groups, column, count, sum);
+                for (int q = 0; q < W; ++q) sum[q] += v[q];
             }
+            add_entries<E, W>(a, whole + g, end, groups, column, count, sum);
         }
         join_groups<W>(a.lanes, sum);
-        if (g == 0) write_row<G, W>(a, (int)(base + r), true, column, count, sum);
+        if (g == 0) write_row<G, W>(a, row, true, column, count, sum);
+        return;
     }
+    const long row = (long)(blockIdx.x - a.first_blocks) * groups + g;
+    if (row >= a.V || count <= 0) return;
+    const int begin = a.starts[row], end = a.starts[row + 1];
+    if (end > begin && (end - 1) / a.piece * a.piece >= begin) return;  // holds the first entry of a piece
+    add_entries<E, W>(a, begin, end, 1, column, count, sum);
+    write_row<G, W>(a, (int)row, end > begin, column, count, sum);
 }
+
+// what a launch has workgroups for
+bool gradient_sizes(int V, int D, long N) { return V > 0 && V <= 1 << 23 && D > 0 && D <= 1 << 21 && N >= 0 && N <= 1L << 30; }
 
 template <typename E, typename G>
 int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
     constexpr int W = kWide<E>;
     SumArgs a = args;
     a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
-    const unsigned tiles = (unsigned)((a.D + a.lanes * W - 1) / (a.lanes * W));
-    const long pieces = N / a.piece;
-    if (pieces > 0) hipLaunchKernelGGL((embed_piece_kernel<E, W>), dim3((unsigned)pieces, tiles), dim3(256), 0, stream, a);
-    const long rows = (a.V + 256L / a.lanes - 1) / (256 / a.lanes);
-    CNT_REQUIRE(rows < 1L << 24 && tiles < 1u << 16, "embed_backward: the table is too large");
-    hipLaunchKernelGGL((embed_rows_kernel<E, G, W>), dim3((unsigned)rows, tiles), dim3(256), 0, stream, a);
+    const long tiles = (a.D + (long)a.lanes * W - 1) / (a.lanes * W), rows = (a.V + 256L / a.lanes - 1) / (256 / a.lanes);
+    const long pieces = N / a.piece, starters = (N + a.piece - 1) / a.piece;
+    a.first_blocks = (int)(N / 256 + 1);
+    hipLaunchKernelGGL((embed_pieces_kernel<E, W>), dim3((unsigned)(a.first_blocks + pieces), (unsigned)tiles), dim3(256), 0, stream, a);
+    CNT_HIP(hipGetLastError());
+    a.first_blocks = (int)starters;
+    hipLaunchKernelGGL((embed_rows_kernel<E, G, W>), dim3((unsigned)(starters + rows), (unsigned)tiles), dim3(256), 0, stream, a);
     CNT_HIP(hipGetLastError());
     return CNT_OK;
 }
@@ -382,7 +386,7 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
 }
 
 long cnt_embed_scratch(int V, int D, long N) {
-    if (V <= 0 || D <= 0 || N < 0 || N > 0x3fffffffL) return -1;
+    if (!cnt::gradient_sizes(V, D, N)) return -1;
     return (long)cnt::sort_plan(V, D, N).bytes;
 }
 
@@ -390,7 +394,7 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
                        long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,
                        size_t scratch_bytes) {
     using namespace cnt;
-    CNT_REQUIRE(V > 0 && D > 0 && N >= 0 && N <= 0x3fffffffL, "embed_backward: bad sizes");
+    CNT_REQUIRE(gradient_sizes(V, D, N), "embed_backward: bad sizes");
     CNT_REQUIRE(known_type(err_type) && known_type(grad_type), "embed_backward: unknown element type");
     CNT_REQUIRE(err_stride >= 0 && grad_stride >= D, "embed_backward: rows of the gradient overlap, or a negative stride");
     CNT_REQUIRE(grad && scratch && (N == 0 || (tokens && err)), "embed_backward: null argument");
@@ -410,19 +414,21 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
         s.slots = pass ? ints(plan.slots[1 - to]) : nullptr;
         s.keys_out = ints(plan.keys[to]); s.slots_out = ints(plan.slots[to]);
         s.shift = pass * plan.bits;
-        const dim3 grid((unsigned)plan.blocks), block(256);
-        if (pass == 0) {
-            hipLaunchKernelGGL(token_count_kernel<true>, grid, block, 0, stream, s);
-            hipLaunchKernelGGL(token_place_kernel<true>, grid, block, 0, stream, s);
-        } else {
-            hipLaunchKernelGGL(token_count_kernel<false>, grid, block, 0, stream, s);
-            hipLaunchKernelGGL(token_place_kernel<false>, grid, block, 0, stream, s);
+        const dim3 grid((unsigned)plan.blocks), block(kSortThreads);
+        auto count = pass == 0 ? token_count_kernel<true> : token_count_kernel<false>;
+        auto place = plan.counted ? (pass == 0 ? token_place_kernel<true, true> : token_place_kernel<false, true>)
+                                  : (pass == 0 ? token_place_kernel<true, false> : token_place_kernel<false, false>);
+        if (plan.counted) {
+            hipLaunchKernelGGL(count, grid, block, 0, stream, s);
+            CNT_HIP(hipGetLastError());
         }
+        hipLaunchKernelGGL(place, grid, block, 0, stream, s);
         CNT_HIP(hipGetLastError());
     }
     const int last = (plan.passes - 1) & 1;
     SumArgs a = {};
     a.keys = ints(plan.keys[last]); a.slots = ints(plan.slots[last]); a.total = s.total;
+    a.starts = ints(plan.starts);
     a.err = err; a.grad = grad; a.partial = reinterpret_cast<float *>(mem + plan.partial);
     a.err_stride = err_stride; a.grad_stride = grad_stride;
     a.V = V; a.D = D; a.piece = plan.piece; a.accumulate = accumulate; a.scale = scale;

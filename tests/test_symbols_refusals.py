@@ -38,7 +38,7 @@ def test_embedding():
         a.update(changes)
         return g(*a.values())
 
-    for changes, what in (({"V": 0}, "sizes"), ({"N": -1}, "sizes"), ({"N": 2 ** 31}, "sizes"), ({"et": 7}, "element type"),
+    for changes, what in (({"V": 0}, "sizes"), ({"N": -1}, "sizes"), ({"N": 2 ** 31}, "sizes"), ({"V": 2 ** 23 + 1}, "sizes"), ({"D": 2 ** 21 + 1}, "sizes"), ({"et": 7}, "element type"),
                           ({"gt": 7}, "element type"), ({"es": -1}, "stride"), ({"gs": 7}, "overlap"), ({"err": None}, "null"),
                           ({"grad": None}, "null"), ({"scratch": None}, "null"), ({"bytes": need - 1}, "scratch"),
                           ({"scratch": C.c_void_p(4100)}, "aligned")):
