@@ -9,12 +9,14 @@
 #include "elements.hpp"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace cnt {
 namespace {
 
-constexpr int kMostTop = 64;
+constexpr int kMostTop = 64, kMostJoined = 1024;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kMinusInfinity = -__builtin_inff();
 
@@ -35,6 +37,32 @@ struct RowArgs {
     long err_stride;
 };
 
+// ----- sums and maxima over the lanes that share a row: 16 (a row of the data-parallel permutations) or a wave ----------------
+template <int ROTATE>
+__device__ __forceinline__ int rotated(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x120 + ROTATE, 0xf, 0xf, false); }
+template <int ROTATE>
+__device__ __forceinline__ float rotated(float v) { return __int_as_float(rotated<ROTATE>(__float_as_int(v))); }
+__device__ __forceinline__ float of_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
+template <int LANES, typename V, typename F>
+__device__ __forceinline__ V over_lanes(V v, F f) {
+    v = f(v, rotated<8>(v));
+    v = f(v, rotated<4>(v));
+    v = f(v, rotated<2>(v));
+    v = f(v, rotated<1>(v));
+    if (LANES == 16) return v;
+    auto at = [&](int lane) {
+        if constexpr (sizeof(V) == 4 && !std::is_integral<V>::value) return of_lane(v, lane);
+        else return (V)__builtin_amdgcn_readlane(v, lane);
+    };
+    return f(f(at(0), at(16)), f(at(32), at(48)));
+}
+template <int LANES>
+__device__ __forceinline__ float max_of(float v) { return over_lanes<LANES>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int LANES>
+__device__ __forceinline__ float sum_of(float v) { return over_lanes<LANES>(v, [](float a, float b) { return a + b; }); }
+template <int LANES>
+__device__ __forceinline__ int min_of(int v) { return over_lanes<LANES>(v, [](int a, int b) { return a < b ? a : b; }); }
+
 // ----- a wave's view of a row: chunks of NV vectors of W logits per lane -----------------------------------------------------
 template <typename T, int NV>
 struct Chunk {
@@ -42,7 +70,7 @@ struct Chunk {
     float x[COUNT];
 };
 // logits begin .. begin + SPAN of a row, those from `end` on are -inf
-template <typename T, int NV>
+template <bool ONCE, typename T, int NV>
 __device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int lane, Chunk<T, NV> &c) {
     constexpr int W = Chunk<T, NV>::W;
     const bool whole = begin + Chunk<T, NV>::SPAN <= end;
@@ -50,8 +78,8 @@ __device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int
     for (int j = 0; j < NV; ++j) {
         const int at = begin + (j * 64 + lane) * W;
         float v[W];
-        if (whole) fetch_elements<T, W>(row + at, v);
-        else fetch_some<T, W>(row + at, max(0, min(W, end - at)), v, kMinusInfinity);
+        if (whole) fetch_elements<T, W, ONCE>(row + at, v);
+        else fetch_some<T, W, ONCE>(row + at, max(0, min(W, end - at)), v, kMinusInfinity);
 #pragma unroll
         for (int i = 0; i < W; ++i) c.x[j * W + i] = v[i];
     }
@@ -75,12 +103,13 @@ __device__ __forceinline__ void shift_stats(Stats &a, float m, float ref, float 
     a.s *= f;
     a.m = m;
 }
+// (hands back the lane's largest of the chunk; NaN are no numbers to it)
 template <typename T, int NV>
-__device__ __forceinline__ void fold(Stats &a, const Chunk<T, NV> &x, float c) {
-    float m = a.m;
+__device__ __forceinline__ float fold(Stats &a, const Chunk<T, NV> &x, float c) {
+    float largest = x.x[0];
 #pragma unroll
-    for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) m = fmaxf(m, x.x[i]);
-    const float ref = m == kMinusInfinity ? 0.0f : m;
+    for (int i = 1; i < Chunk<T, NV>::COUNT; ++i) largest = fmaxf(largest, x.x[i]);
+    const float m = fmaxf(a.m, largest), ref = m == kMinusInfinity ? 0.0f : m;
     shift_stats(a, m, ref, c);
 #pragma unroll
     for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) {
@@ -88,6 +117,7 @@ __device__ __forceinline__ void fold(Stats &a, const Chunk<T, NV> &x, float c) {
         a.s += e;
         a.w = __builtin_fmaf(e, at_least(t), a.w);
     }
+    return largest;
 }
 __device__ __forceinline__ Stats join(Stats a, Stats b, float c) {
     const float m = fmaxf(a.m, b.m), ref = m == kMinusInfinity ? 0.0f : m;
@@ -117,7 +147,6 @@ __device__ __forceinline__ void begin_best(Best &b) {
     b.token = -1;
     b.count = 0;
 }
-__device__ __forceinline__ float of_lane(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
 // puts an entry to place `rank` < K; the others from there on move one lane up
 __device__ __forceinline__ void insert(Best &b, float value, int token, int rank, int K, int lane) {
     const float below_value = __shfl_up(b.value, 1);
@@ -126,10 +155,6 @@ __device__ __forceinline__ void insert(Best &b, float value, int token, int rank
     b.token = lane == rank ? token : lane > rank ? below_token : b.token;
     b.count = min(b.count + 1, K);
     b.least = of_lane(b.value, K - 1);
-}
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return of_lane(v, 0);
 }
 // A chunk's logits that belong into the list, largest first: at most K rounds, each of which takes one logit out of the chunk (c is used
 // up).  Most chunks of a long row end in the first test.  Tokens of later chunks are higher, so an equal logit goes behind.
@@ -155,7 +180,7 @@ __device__ __forceinline__ void take_best(Best &b, Chunk<T, NV> &c, int begin, i
     while (true) {
         const bool full = b.count == K;
         if (full && __ballot(best > b.least) == 0) break;
-        const float m = wave_max(best);
+        const float m = max_of<64>(best);
         if (m != m) break;
         unsigned long long holders = 0;
         int vec = 0;
@@ -210,97 +235,321 @@ __device__ __forceinline__ float logp_of(float x, const Stats &a, float scale, f
 __device__ __forceinline__ float entropy_of(const Stats &a, float log_s) {
     return a.m == kMinusInfinity && a.s == 0.0f ? 0.0f : log_s - kLn2 * (a.w / a.s);
 }
+// by one lane
 template <typename T>
-__device__ __forceinline__ void write_results(const RowArgs &a, long n, const Stats &s, const Best &b, int lane) {
-    const float log_s = logf(s.s);
-    const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-    if (lane == 0) {
-        if (a.logp) {
-            const int token = a.tokens ? a.tokens[n] : -1;
-            a.logp[n] = token >= 0 && token < a.V ? logp_of((float)row[token], s, a.scale, log_s) : 0.0f;
-        }
-        if (a.lse) a.lse[n] = s.m * a.scale + log_s;
-        if (a.entropy) a.entropy[n] = entropy_of(s, log_s);
+__device__ __forceinline__ void write_stats(const RowArgs &a, long n, const Stats &s, float log_s) {
+    if (a.logp) {
+        const int token = a.tokens ? a.tokens[n] : -1;
+        const T *row = static_cast<const T *>(a.logits) + n * a.stride;
+        a.logp[n] = token >= 0 && token < a.V ? logp_of((float)row[token], s, a.scale, log_s) : 0.0f;
     }
-    if (lane < a.K) {
-        if (a.top_logp) a.top_logp[n * a.K + lane] = b.token < 0 ? __builtin_nanf("") : logp_of(b.value, s, a.scale, log_s);
-        if (a.top_tokens) a.top_tokens[n * a.K + lane] = b.token;
+    if (a.lse) a.lse[n] = s.m * a.scale + log_s;
+    if (a.entropy) a.entropy[n] = entropy_of(s, log_s);
+}
+// alternative `rank` of a row; token -1: there is none
+__device__ __forceinline__ void write_top(const RowArgs &a, long n, int rank, float value, int token, const Stats &s, float log_s) {
+    if (a.top_logp) a.top_logp[n * a.K + rank] = token < 0 ? __builtin_nanf("") : logp_of(value, s, a.scale, log_s);
+    if (a.top_tokens) a.top_tokens[n * a.K + rank] = token;
+}
+
+// ----- short rows: LANES lanes hold a row, COUNT logits each ---------------------------------------------------------------------
+// The row is read once and stays in registers, so the maximum is known before the first exponential.  16 lanes per row and not a wave
+// where they can hold it: a row's steps across lanes and the rounds of its alternatives are then taken for four rows at a time.
+template <typename T, int COUNT, int LANES>
+struct ShortRow {
+    static constexpr int W = kWide<T> < COUNT ? kWide<T> : COUNT, NV = COUNT / W;
+    float x[COUNT];
+    static __device__ __forceinline__ int index(int i, int l) { return (i / W * LANES + l) * W + i % W; }
+    __device__ __forceinline__ void load(const T *row, int V, int l) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * LANES + l) * W;
+            float v[W];
+            fetch_some<T, W, true>(row + at, max(0, min(W, V - at)), v, kMinusInfinity);
+#pragma unroll
+            for (int i = 0; i < W; ++i) x[j * W + i] = v[i];
+        }
+    }
+    __device__ __forceinline__ float largest() const {
+        float m = x[0];
+#pragma unroll
+        for (int i = 1; i < COUNT; ++i) m = fmaxf(m, x[i]);
+        return m;
+    }
+    __device__ __forceinline__ Stats stats(float c) const {
+        const float m = max_of<LANES>(largest());
+        Stats a = {m == m ? m : kMinusInfinity, 0.0f, 0.0f};  // (all NaN)
+        const float ref = a.m == kMinusInfinity ? 0.0f : a.m;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) {
+            const float t = (x[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+            a.s += e;
+            a.w = __builtin_fmaf(e, at_least(t), a.w);
+        }
+        a.s = sum_of<LANES>(a.s);
+        a.w = sum_of<LANES>(a.w);
+        return a;
+    }
+};
+
+template <typename T, int COUNT, int LANES, bool TOP>
+__global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
+    const int l = threadIdx.x % LANES;
+    const long n = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const bool here = n < a.N;  // (whole groups of lanes)
+    const T *row = static_cast<const T *>(a.logits) + (here ? n : 0) * a.stride;
+    ShortRow<T, COUNT, LANES> x;
+    x.load(row, here ? a.V : 0, l);
+    const Stats s = x.stats(a.scale * kLog2e);
+    const float log_s = logf(s.s);
+    if (here && l == 0) write_stats<T>(a, n, s, log_s);
+    if (!TOP) return;
+    // K rounds: the largest of what is left, the lowest token where several hold it; its place is taken by a NaN, which is never the largest
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+        if (x.index(i, l) >= a.V) x.x[i] = __builtin_nanf("");
+    for (int k = 0; k < a.K; ++k) {
+        const float best = x.largest();
+        int at = 0;
+#pragma unroll
+        for (int i = COUNT - 1; i >= 0; --i) at = x.x[i] == best ? i : at;
+        const float m = max_of<LANES>(best);
+        const int token = min_of<LANES>(best == m ? x.index(at, l) : INT_MAX);
+        const int taken = best == m && x.index(at, l) == token ? at : -1;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) x.x[i] = i == taken ? __builtin_nanf("") : x.x[i];
+        if (here && l == 0) write_top(a, n, k, m, token == INT_MAX ? -1 : token, s, log_s);
     }
 }
 
-// A row, or a part of one, by WAVES waves of a workgroup of four: their chunks alternate.
-template <typename T, int NV, int WAVES, bool TOP>
+// ----- long rows: a workgroup of four waves for a row or a part of one ------------------------------------------------------------
+// The best K without keeping them up to date on the way, which at K = 16 took longer than everything else (2047 rows of 100003: 200 us, of
+// which a list per wave 130): a lane remembers the largest logit of its best two chunks, and of which chunks, and that of its third.  The
+// K-th largest of the lanes' largest is a bound that K logits reach.  Only the remembered chunks' logits of their lanes
+// that reach it are read again, some 16 K of them, unless a lane's third chunk reaches it too, or ties make
+// them too many: then the row is read once more with lists.
+struct Cells {
+    float first, second, third;
+    int first_at, second_at;
+};
+__device__ __forceinline__ void remember(Cells &c, float largest, int at) {
+    const bool a = largest > c.first, b = largest > c.second;
+    c.third = b ? c.second : fmaxf(c.third, largest);
+    c.second_at = a ? c.first_at : b ? at : c.second_at;
+    c.second = a ? c.first : b ? largest : c.second;
+    c.first_at = a ? at : c.first_at;
+    c.first = a ? largest : c.first;
+}
+// whole numbers in the order of floats, -0 the same as 0; no number is 0
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned u = __float_as_uint(v + 0.0f);
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+// the K-th largest of a wave's keys, up to COUNT per lane, `entries` in all; 0: there are fewer, keys of 0 being none
+template <int COUNT>
+__device__ __forceinline__ unsigned kth_largest(const unsigned (&key)[COUNT], int entries, int K) {
+    unsigned t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned more = t | 1u << bit;
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < COUNT; ++q)
+            if (q * 64 < entries) count += __popcll(__ballot(key[q] >= more));
+        t = count >= K ? more : t;
+    }
+    return t;
+}
+
+constexpr int kMostCells = 64, kMostCandidates = 256;
+struct Shared {
+    Stats stats[4];
+    float first[256], second[256], third[4];
+    int first_at[256], second_at[256];
+    int cell_lane[kMostCells], cell_at[kMostCells];
+    unsigned least;
+    int cells, candidates;
+    float value[kMostCandidates];
+    int token[kMostCandidates];
+};
+
+// entry i of a list, at its rank if that is among the first K: f(rank)
+template <typename F>
+__device__ __forceinline__ void rank_entry(const float *value, const int *token, int count, int i, int K, F f) {
+    const float v = value[i];
+    const int t = token[i];
+    int rank = 0;
+    for (int k = 0; k < count; ++k) rank += value[k] > v || (value[k] == v && token[k] < t);
+    if (rank < K) f(rank, v, t);
+}
+
+template <typename T, int NV, bool TOP>
 __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
-    constexpr int SPAN = Chunk<T, NV>::SPAN;
+    using X = Chunk<T, NV>;
+    constexpr int SPAN = X::SPAN, W = X::W;
+    __shared__ Shared sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = WAVES == 1 ? (long)blockIdx.x * 4 + wave : (long)blockIdx.x;
-    if (n >= a.N) return;  // (a workgroup of one row never)
+    const long n = blockIdx.x;
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-    const int begin = WAVES == 1 ? 0 : (int)blockIdx.y * a.part, end = WAVES == 1 ? a.V : min(a.V, begin + a.part);
+    const int begin = (int)blockIdx.y * a.part, end = min(a.V, begin + a.part);
     Stats s;
-    Best b;
     begin_stats(s);
-    begin_best(b);
-    for (int at = begin + (WAVES == 1 ? 0 : wave * SPAN); at < end; at += WAVES * SPAN) {
-        Chunk<T, NV> x;
-        load_chunk(row, at, end, lane, x);
-        fold(s, x, c);
-        if (TOP) take_best(b, x, at, end, a.K, lane);
+    Cells cells = {kMinusInfinity, kMinusInfinity, kMinusInfinity, -1, -1};
+    for (int at = begin + wave * SPAN; at < end; at += 4 * SPAN) {
+        X x;
+        load_chunk<true>(row, at, end, lane, x);
+        const float largest = fold(s, x, c);
+        if (TOP) remember(cells, largest, at);
     }
     s = join_lanes(s, c);
-    if (WAVES > 1) {
-        __shared__ Stats stats[4];
-        __shared__ float values[4][kMostTop];
-        __shared__ int tokens[4][kMostTop];
-        if (lane == 0) stats[wave] = s;
-        if (TOP) {
-            values[wave][lane] = b.value;
-            tokens[wave][lane] = lane < b.count ? b.token : -1;
-        }
-        __syncthreads();
-        if (wave != 0) return;
+    if (lane == 0) sh.stats[wave] = s;
+    if (TOP) {
+        sh.first[threadIdx.x] = cells.first;
+        sh.second[threadIdx.x] = cells.second;
+        sh.first_at[threadIdx.x] = cells.first_at;
+        sh.second_at[threadIdx.x] = cells.second_at;
+        const float third = max_of<64>(cells.third);
+        if (lane == 0) sh.third[wave] = third;
+    }
+    __syncthreads();
+    s = sh.stats[0];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) {
-            s = join(s, stats[w], c);
-            if (TOP) merge_best(b, values[w][lane], tokens[w][lane], a.K, lane);
-        }
-        if (a.parts > 1) {
-            const long p = n * a.parts + blockIdx.y;
-            if (lane == 0) {
-                a.part_stats[p * 3] = s.m;
-                a.part_stats[p * 3 + 1] = s.s;
-                a.part_stats[p * 3 + 2] = s.w;
-            }
-            if (TOP && lane < a.K) {
-                a.part_values[p * a.K + lane] = b.value;
-                a.part_tokens[p * a.K + lane] = b.token;
-            }
-            return;
+    for (int w = 1; w < 4; ++w) s = join(s, sh.stats[w], c);
+    const float log_s = logf(s.s);
+    const bool shared_row = a.parts > 1;
+    const long p = n * a.parts + blockIdx.y;
+    if (threadIdx.x == 0) {
+        if (shared_row) {
+            a.part_stats[p * 3] = s.m;
+            a.part_stats[p * 3 + 1] = s.s;
+            a.part_stats[p * 3 + 2] = s.w;
+        } else {
+            write_stats<T>(a, n, s, log_s);
         }
     }
-    write_results<T>(a, n, s, b, lane);
+    if (!TOP) return;
+    auto put = [&](int rank, float value, int token) {
+        if (shared_row) {
+            a.part_values[p * a.K + rank] = value;
+            a.part_tokens[p * a.K + rank] = token;
+        } else {
+            write_top(a, n, rank, value, token, s, log_s);
+        }
+    };
+    if (wave == 0) {
+        unsigned key[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) key[w] = ordered(sh.first[w * 64 + lane]);
+        const unsigned least = kth_largest<4>(key, 256, a.K);
+        bool plain = ordered(fmaxf(fmaxf(sh.third[0], sh.third[1]), fmaxf(sh.third[2], sh.third[3]))) < least;
+        int count = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int from = q % 4 * 64 + lane;
+            const bool in = ordered(q < 4 ? sh.first[from] : sh.second[from]) >= least;
+            const unsigned long long b = __ballot(in);
+            const int place = count + __popcll(b & ((1ull << lane) - 1));
+            if (plain && in && place < kMostCells) {
+                sh.cell_lane[place] = lane;
+                sh.cell_at[place] = q < 4 ? sh.first_at[from] : sh.second_at[from];
+            }
+            count += __popcll(b);
+        }
+        if (lane == 0) {
+            sh.least = least;
+            sh.cells = plain && count <= kMostCells ? count : -1;
+            sh.candidates = 0;
+        }
+    }
+    __syncthreads();
+    const int n_cells = sh.cells;
+    bool listed = n_cells < 0;
+    if (!listed) {
+        const unsigned least = sh.least;
+        for (int i = threadIdx.x; i < n_cells * NV; i += 256) {
+            const int cell = i / NV, first = sh.cell_at[cell] + (i % NV * 64 + sh.cell_lane[cell]) * W;
+            float v[W];
+            fetch_some<T, W>(row + first, max(0, min(W, end - first)), v, __builtin_nanf(""));
+#pragma unroll
+            for (int q = 0; q < W; ++q) {
+                if (v[q] == v[q] && ordered(v[q]) >= least) {
+                    const int place = atomicAdd(&sh.candidates, 1);
+                    if (place < kMostCandidates) {
+                        sh.value[place] = v[q];
+                        sh.token[place] = first + q;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        listed = sh.candidates > kMostCandidates;
+        if (!listed && (int)threadIdx.x < sh.candidates) rank_entry(sh.value, sh.token, sh.candidates, threadIdx.x, a.K, put);
+    }
+    if (!listed) return;
+    // the row again, with a list per wave
+    Best b;
+    begin_best(b);
+    for (int at = begin + wave * SPAN; at < end; at += 4 * SPAN) {
+        X x;
+        load_chunk<false>(row, at, end, lane, x);
+        take_best(b, x, at, end, a.K, lane);
+    }
+    __syncthreads();
+    float *values = sh.first;  // 64 of each wave
+    int *tokens = sh.first_at;
+    values[threadIdx.x] = b.value;
+    tokens[threadIdx.x] = lane < b.count ? b.token : -1;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) merge_best(b, values[w * 64 + lane], tokens[w * 64 + lane], a.K, lane);
+    if (lane < a.K) put(lane, b.value, lane < b.count ? b.token : -1);
 }
 
-// the parts of a row, by a wave
+// The parts of a row, by a wave: up to 16 * 64 alternatives of all parts.
 template <typename T>
 __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
+    __shared__ float value[kMostJoined];
+    __shared__ int token[kMostJoined];
     const long n = blockIdx.x;
     const int lane = threadIdx.x;
     const float c = a.scale * kLog2e;
     Stats s;
-    Best b;
     begin_stats(s);
-    begin_best(b);
     const long p = n * a.parts;
     if (lane < a.parts) s = {a.part_stats[(p + lane) * 3], a.part_stats[(p + lane) * 3 + 1], a.part_stats[(p + lane) * 3 + 2]};
+    float v[kMostJoined / 64];
+    int t[kMostJoined / 64];
+    const int entries = a.parts * a.K;
+#pragma unroll
+    for (int q = 0; q < kMostJoined / 64; ++q) {
+        const int i = q * 64 + lane;
+        v[q] = i < entries ? a.part_values[p * a.K + i] : 0.0f;
+        t[q] = i < entries ? a.part_tokens[p * a.K + i] : -1;
+    }
     s = join_lanes(s, c);
-    if (a.K > 0)
-        for (int i = 0; i < a.parts; ++i) {
-            const long at = (p + i) * a.K + lane;
-            merge_best(b, lane < a.K ? a.part_values[at] : 0.0f, lane < a.K ? a.part_tokens[at] : -1, a.K, lane);
+    const float log_s = logf(s.s);
+    if (lane == 0) write_stats<T>(a, n, s, log_s);
+    if (a.K == 0) return;
+    unsigned key[kMostJoined / 64];
+#pragma unroll
+    for (int q = 0; q < kMostJoined / 64; ++q) key[q] = t[q] >= 0 ? ordered(v[q]) : 0u;
+    const unsigned least = max(1u, kth_largest<kMostJoined / 64>(key, entries, a.K));
+    int count = 0;
+#pragma unroll
+    for (int q = 0; q < kMostJoined / 64; ++q) {
+        const unsigned long long b = __ballot(key[q] >= least);
+        const int place = count + __popcll(b & ((1ull << lane) - 1));
+        if (key[q] >= least) {
+            value[place] = v[q];
+            token[place] = t[q];
         }
-    write_results<T>(a, n, s, b, lane);
+        count += __popcll(b);
+    }
+    __syncthreads();
+    for (int i = lane; i < count; i += 64)
+        rank_entry(value, token, count, i, a.K, [&](int rank, float x, int y) { write_top(a, n, rank, x, y, s, log_s); });
+    for (int i = count + lane; i < a.K; i += 64) write_top(a, n, i, 0.0f, -1, s, log_s);  // NaN took the others' places
 }
 
 // ----- gradient ----------------------------------------------------------------------------------------------------------------
@@ -321,23 +570,33 @@ __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse,
     if (lse != lse) s.first = lse;
     return s;
 }
+// W errors of a row from logit `at` on in the place of log2 of the probabilities
+template <int W>
+__device__ __forceinline__ void errors_of(int at, const Slopes &s, float (&t)[W]) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float u = at_least(t[i]);
+        t[i] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(s.second, u, s.first);
+    }
+    if ((unsigned)(s.token - at) < (unsigned)W) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] += s.token - at == i ? s.given : 0.0f;
+    }
+}
+template <typename T, int W>
+__device__ __forceinline__ void put_errors(T *row, int at, int end, const Slopes &s, float (&t)[W]) {
+    errors_of<W>(at, s, t);
+    put_some<T, W, true>(row + at, max(0, min(W, end - at)), t);
+}
 template <typename T, int NV>
 __device__ __forceinline__ void put_gradient(T *row, int begin, int end, int lane, const Slopes &s, const Chunk<T, NV> &t) {
     constexpr int W = Chunk<T, NV>::W;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int at = begin + (j * 64 + lane) * W;
         float v[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const float u = at_least(t.x[j * W + i]);
-            v[i] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(s.second, u, s.first);
-        }
-        if ((unsigned)(s.token - at) < (unsigned)W) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] += s.token - at == i ? s.given : 0.0f;
-        }
-        put_some<T, W>(row + at, max(0, min(W, end - at)), v);
+        for (int i = 0; i < W; ++i) v[i] = t.x[j * W + i];
+        put_errors<T, W>(row, begin + (j * 64 + lane) * W, end, s, v);
     }
 }
 
@@ -354,50 +613,183 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) 
     const float ref = lse == kMinusInfinity ? 0.0f : lse;
     for (int at = (blockIdx.y * 4 + wave) * SPAN; at < a.V; at += gridDim.y * 4 * SPAN) {
         Chunk<T, NV> x;
-        load_chunk(row, at, a.V, lane, x);
+        load_chunk<true>(row, at, a.V, lane, x);
 #pragma unroll
-        for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = (x.x[i] * a.scale - ref) * kLog2e;
+        for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = __builtin_fmaf(x.x[i], a.scale, -ref) * kLog2e;
         put_gradient(to, at, a.V, lane, s, x);
     }
 }
 
-// statistics and gradient of a row by WAVES waves of a workgroup of four
-template <typename T, int NV, int WAVES>
-__global__ __launch_bounds__(256) void logprob_error_kernel(const RowArgs a) {
-    constexpr int SPAN = Chunk<T, NV>::SPAN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = WAVES == 1 ? (long)blockIdx.x * 4 + wave : (long)blockIdx.x;
-    if (n >= a.N) return;
+template <typename T, int COUNT, int LANES>
+__global__ __launch_bounds__(256) void logprob_short_error_kernel(const RowArgs a) {
+    using X = ShortRow<T, COUNT, LANES>;
+    constexpr int W = X::W;
+    const int l = threadIdx.x % LANES;
+    const long n = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const bool here = n < a.N;
+    const float c = a.scale * kLog2e;
+    X x;
+    x.load(static_cast<const T *>(a.logits) + (here ? n : 0) * a.stride, here ? a.V : 0, l);
+    const Stats s = x.stats(c);
+    if (!here) return;
+    const float log_s = logf(s.s), log2_s = log_s * kLog2e;
+    if (l == 0) write_stats<T>(a, n, s, log_s);
+    const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
+    const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
+    T *to = static_cast<T *>(a.err) + n * a.err_stride;
+#pragma unroll
+    for (int j = 0; j < X::NV; ++j) {
+        float t[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = (x.x[j * W + i] - ref) * c - log2_s;
+        put_errors<T, W>(to, (j * LANES + l) * W, a.V, slopes, t);
+    }
+}
+
+// 16 bytes of a row as they stand in memory.  renewed() hides that nothing has changed: the compiler would keep the 32-bit values from one use
+// to the next otherwise, which takes twice the registers of 16-bit logits.
+template <typename T>
+struct Raw {
+    typedef typename Packed<T, kWide<T>>::type vec;
+    typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
+    words x;
+    __device__ __forceinline__ void load(const T *p, bool whole) {
+        vec v;
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) v[i] = (T)kMinusInfinity;
+        x = __builtin_bit_cast(words, v);
+        if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
+    }
+    __device__ __forceinline__ void renewed() {
+        unsigned a = x[0], b = x[1], c = x[2], d = x[3];
+        asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+        x = words{a, b, c, d};
+    }
+    __device__ __forceinline__ void values(float (&v)[kWide<T>]) const {
+        const vec y = __builtin_bit_cast(vec, x);
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) v[i] = (float)y[i];
+    }
+};
+
+// A long row that a workgroup of THREADS holds in registers, NV vectors per thread: read once, written once.  GROUPS: workgroups that a compute
+// unit has registers for, so that one's loads and stores go on while another computes.
+template <typename T, int NV, int THREADS, int GROUPS>
+__global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_error_kernel(const RowArgs a) {
+    constexpr int W = kWide<T>, WAVES = THREADS / 64;
+    __shared__ float maxima[WAVES], sums[WAVES], means[WAVES], given;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long n = blockIdx.x;
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
-    const int first = WAVES == 1 ? 0 : wave * SPAN;
+    const int token = a.tokens ? a.tokens[n] : -1;
+    // the row's whole vectors, and what is left behind them, one logit for each of the first threads
+    Raw<T> x[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int at = (j * THREADS + (int)threadIdx.x) * W;
+        x[j].load(row + at, at + W <= a.V);
+    }
+    const int behind = a.V / W * W + (int)threadIdx.x;
+    const float rest = behind < a.V ? (float)row[behind] : kMinusInfinity;
+    float m = rest;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float v[W];
+        x[j].values(v);
+#pragma unroll
+        for (int i = 0; i < W; ++i) m = fmaxf(m, v[i]);
+        x[j].renewed();
+        __builtin_amdgcn_sched_barrier(0);  // (one vector's values at a time)
+    }
+    m = max_of<64>(m);
+    if (lane == 0) maxima[wave] = m;
+    // the errors may take the logits' place: the given token's logit is kept before any of them is written
+    if (threadIdx.x == 0 && token >= 0 && token < a.V) given = (float)row[token];
+    __syncthreads();
+    const int w = lane % 16;  // every 16 lanes add the waves up
+    m = max_of<16>(w < WAVES ? maxima[w] : kMinusInfinity);
+    m = m == m ? m : kMinusInfinity;  // (all NaN)
+    const float ref = m == kMinusInfinity ? 0.0f : m, t_rest = (rest - ref) * c, e_rest = __builtin_amdgcn_exp2f(t_rest);
+    Stats s = {m, e_rest, e_rest * at_least(t_rest)};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float v[W];
+        x[j].values(v);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float t = (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+            s.s += e;
+            s.w = __builtin_fmaf(e, at_least(t), s.w);
+        }
+        x[j].renewed();
+        __builtin_amdgcn_sched_barrier(0);  // (one vector's values at a time)
+    }
+    s.s = sum_of<64>(s.s);
+    s.w = sum_of<64>(s.w);
+    if (lane == 0) {
+        sums[wave] = s.s;
+        means[wave] = s.w;
+    }
+    __syncthreads();
+    s.s = sum_of<16>(w < WAVES ? sums[w] : 0.0f);
+    s.w = sum_of<16>(w < WAVES ? means[w] : 0.0f);
+    const float log_s = logf(s.s), log2_s = log_s * kLog2e, entropy = entropy_of(s, log_s), lse = s.m * a.scale + log_s;
+    if (threadIdx.x == 0) {
+        if (a.logp) a.logp[n] = token >= 0 && token < a.V ? logp_of(given, s, a.scale, log_s) : 0.0f;
+        a.lse[n] = lse;
+        a.entropy[n] = entropy;
+    }
+    const Slopes slopes = slopes_of(a, n, lse, entropy);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        float t[W];
+        x[j].values(t);
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = (t[i] - ref) * c - log2_s;
+        const int at = (j * THREADS + (int)threadIdx.x) * W;
+        errors_of<W>(at, slopes, t);
+        if (at + W <= a.V) put_elements<T, W, true>(to + at, t);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (behind < a.V) {
+        float t[1] = {t_rest - log2_s};
+        errors_of<1>(behind, slopes, t);
+        to[behind] = (T)t[0];
+    }
+}
+
+// Longer rows: a workgroup of 16 waves reads the row twice, the second time mostly from the caches.
+template <typename T, int NV>
+__global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs a) {
+    constexpr int SPAN = Chunk<T, NV>::SPAN, WAVES = 16;
+    __shared__ Stats stats[WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long n = blockIdx.x;
+    const float c = a.scale * kLog2e;
+    const T *row = static_cast<const T *>(a.logits) + n * a.stride;
+    T *to = static_cast<T *>(a.err) + n * a.err_stride;
     Stats s;
-    Best none;
     begin_stats(s);
-    begin_best(none);
     Chunk<T, NV> x;
-    for (int at = first; at < a.V; at += WAVES * SPAN) {
-        load_chunk(row, at, a.V, lane, x);
+    for (int at = wave * SPAN; at < a.V; at += WAVES * SPAN) {
+        load_chunk<false>(row, at, a.V, lane, x);
         fold(s, x, c);
     }
     s = join_lanes(s, c);
-    if (WAVES > 1) {
-        __shared__ Stats stats[4];
-        if (lane == 0) stats[wave] = s;
-        __syncthreads();
-        s = stats[0];
+    if (lane == 0) stats[wave] = s;
+    __syncthreads();
+    s = stats[0];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s = join(s, stats[w], c);
-    }
-    if (WAVES == 1 || wave == 0) write_results<T>(a, n, s, none, lane);
-    // the errors may take the logits' place: the token's logit has been read before any of the workgroup's errors is written
-    if (WAVES > 1) __syncthreads();
+    for (int w = 1; w < WAVES; ++w) s = join(s, stats[w], c);
     const float log_s = logf(s.s), log2_s = log_s * kLog2e;
+    if (threadIdx.x == 0) write_stats<T>(a, n, s, log_s);
+    __syncthreads();  // the errors may take the logits' place: the given token's logit has been read
     const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
-    for (int at = first; at < a.V; at += WAVES * SPAN) {
-        if (WAVES > 1) load_chunk(row, at, a.V, lane, x);
+    for (int at = wave * SPAN; at < a.V; at += WAVES * SPAN) {
+        load_chunk<true>(row, at, a.V, lane, x);
 #pragma unroll
         for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = (x.x[i] - ref) * c - log2_s;
         put_gradient(to, at, a.V, lane, slopes, x);
@@ -405,24 +797,27 @@ __global__ __launch_bounds__(256) void logprob_error_kernel(const RowArgs a) {
 }
 
 // ----- launches ------------------------------------------------------------------------------------------------------------------
-// Logits of a wave's chunk: 32 per lane.  A row that fits into one is a wave's.
+// Logits of a wave's chunk: 32 per lane.  A row that fits into one stays in the registers of a wave or of 16 lanes.
 constexpr int kSpan = 64 * 32;
 // Parts of a row: enough workgroups for the card where there are few rows, each with a chunk per wave at least, as many as a wave can join.
-int parts_of(long N, int V) {
+int parts_of(long N, int V, int K) {
     if (V <= kSpan || N == 0 || N >= 512) return 1;
-    return (int)std::min({64L, (V + 4L * kSpan - 1) / (4 * kSpan), (1023 + N) / N});
+    return (int)std::min({64L, (V + 4L * kSpan - 1) / (4 * kSpan), (1023 + N) / N, K > 0 ? (long)kMostJoined / K : 64L});
 }
 
-template <typename T, int NV, int WAVES>
-void launch_rows(hipStream_t stream, const RowArgs &a) {
-    const dim3 grid((unsigned)(WAVES == 1 ? (a.N + 3) / 4 : a.N), (unsigned)a.parts), block(256);
-    if (a.K > 0) hipLaunchKernelGGL((logprob_kernel<T, NV, WAVES, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((logprob_kernel<T, NV, WAVES, false>), grid, block, 0, stream, a);
-    if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, stream, a);
+// f(COUNT, LANES) for a short row
+template <typename F>
+void with_lanes(int V, F f) {
+    using std::integral_constant;
+    if (V <= 128) f(integral_constant<int, 8>(), integral_constant<int, 16>());
+    else if (V <= 256) f(integral_constant<int, 16>(), integral_constant<int, 16>());
+    else if (V <= 512) f(integral_constant<int, 32>(), integral_constant<int, 16>());
+    else if (V <= 1024) f(integral_constant<int, 16>(), integral_constant<int, 64>());
+    else f(integral_constant<int, 32>(), integral_constant<int, 64>());
 }
 
 size_t scratch_of(long N, int V, int K) {
-    const int parts = parts_of(N, V);
+    const int parts = parts_of(N, V, K);
     return parts == 1 ? 0 : (size_t)N * parts * (3 + 2 * (size_t)K) * sizeof(float);
 }
 // where a shared row's statistics and lists are
@@ -436,14 +831,22 @@ void lay_out(RowArgs &a, void *scratch) {
 }
 
 int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
-    a.parts = parts_of(a.N, a.V);
+    a.parts = parts_of(a.N, a.V, a.K);
     lay_out(a, scratch);
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        constexpr int NV = 32 / kWide<T>;
-        if (a.V <= 64 * kWide<T>) launch_rows<T, 1, 1>(stream, a);
-        else if (a.V <= kSpan) launch_rows<T, NV, 1>(stream, a);
-        else launch_rows<T, NV, 4>(stream, a);
+        if (a.V <= kSpan) {
+            with_lanes(a.V, [&](auto count, auto lanes) {
+                constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
+                const dim3 grid((unsigned)((a.N + 256 / LANES - 1) / (256 / LANES)));
+                auto kernel = a.K > 0 ? logprob_short_kernel<T, COUNT, LANES, true> : logprob_short_kernel<T, COUNT, LANES, false>;
+                hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
+            });
+        } else {
+            auto kernel = a.K > 0 ? logprob_kernel<T, 32 / kWide<T>, true> : logprob_kernel<T, 32 / kWide<T>, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)a.N, (unsigned)a.parts), dim3(256), 0, stream, a);
+            if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, stream, a);
+        }
     });
     CNT_HIP(hipGetLastError());
     return CNT_OK;
@@ -537,17 +940,33 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
     a.logp_err = logp_err; a.entropy_err = entropy_err; a.err = err; a.err_stride = err_stride;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "logprob_error_backward");
-    if (parts_of(N, V) > 1) {  // few long rows: shared out among workgroups
+    if (parts_of(N, V, 0) > 1) {  // few long rows: shared out among workgroups
         CNT_TRY(forward(stream, type, a, scratch));
         return gradient(stream, type, a);
     }
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        constexpr int NV = 32 / kWide<T>;
-        const dim3 few((unsigned)((N + 3) / 4)), many((unsigned)N), block(256);
-        if (V <= 64 * kWide<T>) hipLaunchKernelGGL((logprob_error_kernel<T, 1, 1>), few, block, 0, stream, a);
-        else if (V <= kSpan) hipLaunchKernelGGL((logprob_error_kernel<T, NV, 1>), few, block, 0, stream, a);
-        else hipLaunchKernelGGL((logprob_error_kernel<T, NV, 4>), many, block, 0, stream, a);
+        constexpr int W = kWide<T>;
+        const dim3 rows((unsigned)N);
+        if (V <= kSpan) {
+            with_lanes(V, [&](auto count, auto lanes) {
+                constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
+                const dim3 grid((unsigned)((N + 256 / LANES - 1) / (256 / LANES)));
+                hipLaunchKernelGGL((logprob_short_error_kernel<T, COUNT, LANES>), grid, dim3(256), 0, stream, a);
+            });
+        } else if (V <= 256 * 4 * W) {
+            hipLaunchKernelGGL((logprob_held_error_kernel<T, 4, 256, 4>), rows, dim3(256), 0, stream, a);
+        } else if (V <= 256 * 8 * W) {
+            hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 256, 4>), rows, dim3(256), 0, stream, a);
+        } else if (V <= 512 * 8 * W) {
+            hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 512, 3>), rows, dim3(512), 0, stream, a);
+        } else if (V <= 1024 * 8 * W) {
+            hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 1024, 2>), rows, dim3(1024), 0, stream, a);
+        } else if (V <= 1024 * 16 * W) {
+            hipLaunchKernelGGL((logprob_held_error_kernel<T, 16, 1024, 1>), rows, dim3(1024), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((logprob_long_error_kernel<T, 32 / W>), rows, dim3(1024), 0, stream, a);
+        }
     });
     CNT_HIP(hipGetLastError());
     return CNT_OK;
