@@ -130,7 +130,7 @@ int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const 
  * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
  * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
  * cnt_embed_scratch(V, D, N) bytes, aligned to 16, with any content, which the call has for itself until it has run (two captured
- * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30. */
+ * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^34. */
 long cnt_embed_scratch(int V, int D, long N);
 int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
                        long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,

@@ -24,22 +24,38 @@ struct LookupArgs {
     float scale;
 };
 
+constexpr int kSlotsPerThread = 4;
+
+// A thread has the same columns of several slots, whose tokens and then rows it asks for together.
 template <typename T, typename O>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
-    constexpr int W = 8;
-    const long n = (long)blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
-    if (n >= a.N) return;
-    const int token = a.tokens[n];
-    const bool held = token >= 0 && token < a.V;
-    const T *from = static_cast<const T *>(a.table) + (held ? token : 0) * a.table_stride;
-    O *to = static_cast<O *>(a.out) + n * a.out_stride;
+    constexpr int W = kBoth<T, O>, U = kSlotsPerThread;
+    const int rows = 256 / a.lanes;
+    const long n = (long)blockIdx.x * (rows * U) + threadIdx.x / a.lanes;
+    bool held[U];
+    const T *from[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int token = n + u * rows < a.N ? a.tokens[n + u * rows] : -1;
+        held[u] = token >= 0 && token < a.V;
+        from[u] = static_cast<const T *>(a.table) + (held[u] ? token : 0) * a.table_stride;
+    }
     for (int d = (threadIdx.x % a.lanes) * W; d < a.D; d += a.lanes * W) {
         const int count = min(W, a.D - d);
-        float v[W];
-        if (held) fetch_some<T, W>(from + d, count, v, 0.0f);
+        float v[U][W];
 #pragma unroll
-        for (int q = 0; q < W; ++q) v[q] = held ? v[q] * a.scale : 0.0f;
-        put_some<O, W>(to + d, count, v);
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
+            if (held[u]) fetch_some<T, W>(from[u] + d, count, v[u], 0.0f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (n + u * rows >= a.N) break;
+#pragma unroll
+            for (int q = 0; q < W; ++q) v[u][q] *= held[u] ? a.scale : 0.0f;
+            put_some<O, W, true>(static_cast<O *>(a.out) + (n + u * rows) * a.out_stride + d, count, v[u]);
+        }
     }
 }
 
@@ -66,7 +82,7 @@ SortPlan sort_plan(long V, int D, long N) {
     p.counted = N > kCountedTwice;
     // partial sums of pieces: about as many entries in a piece as pieces in the longest runs
     p.piece = 32;
-    while (16L * p.piece * p.piece < N) p.piece *= 2;
+    while (64L * p.piece * p.piece < N) p.piece *= 2;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -98,10 +114,15 @@ __device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIR
 
 // how often every digit occurs among entries begin .. end, added to bins
 template <bool FIRST>
-__device__ __forceinline__ void count_digits(const SortArgs &a, long begin, long end, int first, int step, int *bins) {
-    for (long i = begin + first; i < end; i += step) {
-        const int key = a.keys[i];
-        if (listed<FIRST>(a, key)) atomicAdd(&bins[(key >> a.shift) & ((1 << a.bits) - 1)], 1);
+__device__ __forceinline__ void count_digits(const SortArgs &a, long begin, long end, int first, long step, int *bins) {
+    constexpr int U = 8;  // loads in flight
+    for (long i = begin + first; i < end; i += U * step) {
+        int key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) key[u] = i + u * step < end ? a.keys[i + u * step] : -1;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (key[u] >= 0 && listed<FIRST>(a, key[u])) atomicAdd(&bins[(key[u] >> a.shift) & ((1 << a.bits) - 1)], 1);
     }
 }
 
@@ -213,6 +234,7 @@ struct SumArgs {
     float *partial;
     long err_stride, grad_stride;
     int V, D, lanes, piece, accumulate;
+    int tiles;         // of `lanes` threads' columns in a row; neighbouring workgroups have neighbouring ones
     int first_blocks;  // workgroups of the first kind of a launch, in front of those of the second
     float scale;
 };
@@ -300,25 +322,25 @@ __device__ __forceinline__ void write_row(const SumArgs &a, int row, bool any, i
     if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
 #pragma unroll
     for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + sum[q] * a.scale : sum[q] * a.scale;
-    put_some<G, W>(to, count, sum);
+    put_some<G, W, true>(to, count, sum);
 }
 
 // First workgroups: rows whose run holds the first entry of a piece, by all groups of the workgroup of the first such piece; whole pieces go
 // by their sums.  The others: the other rows, a group of `lanes` threads for each, which have fewer entries than a piece.
-template <typename E, typename G, int W>
+template <typename E, typename G, int W, int R>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
-    const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    const int block = blockIdx.x / a.tiles, column = ((int)blockIdx.x % a.tiles * a.lanes + x) * W, count = max(0, min(W, a.D - column));
     float sum[W] = {};
-    if ((int)blockIdx.x < a.first_blocks) {
-        const int here = blockIdx.x * a.piece;
+    if (block < a.first_blocks) {
+        const int here = block * a.piece;
         if (here >= *a.total) return;
         const int row = a.keys[here], begin = a.starts[row], end = a.starts[row + 1];
         if (here - begin >= a.piece) return;
         const int whole = end / a.piece * a.piece;  // >= here
         if (count > 0) {
             add_entries<E, W>(a, begin + g, here, groups, column, count, sum);
-            for (int p = blockIdx.x + g; p < whole / a.piece; p += groups) {
+            for (int p = block + g; p < whole / a.piece; p += groups) {
                 float v[W];
                 fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
 #pragma unroll
@@ -330,29 +352,57 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         if (g == 0) write_row<G, W>(a, row, true, column, count, sum);
         return;
     }
-    const long row = (long)(blockIdx.x - a.first_blocks) * groups + g;
-    if (row >= a.V || count <= 0) return;
-    const int begin = a.starts[row], end = a.starts[row + 1];
-    if (end > begin && (end - 1) / a.piece * a.piece >= begin) return;  // holds the first entry of a piece
-    add_entries<E, W>(a, begin, end, 1, column, count, sum);
-    write_row<G, W>(a, (int)row, end > begin, column, count, sum);
+    // A group's rows are far apart: frequent tokens are neighbours in most vocabularies.
+    const long first = (long)(block - a.first_blocks) * groups + g, step = (long)(gridDim.x / a.tiles - a.first_blocks) * groups;
+    if (count <= 0) return;
+    int begin[R], end[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const long row = min(a.V - 1L, first + r * step);
+        begin[r] = a.starts[row];
+        end[r] = a.starts[row + 1];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (first + r * step >= a.V) break;
+        if (end[r] > begin[r] && (end[r] - 1) / a.piece * a.piece >= begin[r]) continue;  // holds the first entry of a piece
+        float row_sum[W] = {};
+        add_entries<E, W>(a, begin[r], end[r], 1, column, count, row_sum);
+        write_row<G, W>(a, (int)(first + r * step), end[r] > begin[r], column, count, row_sum);
+    }
 }
 
-// what a launch has workgroups for
-bool gradient_sizes(int V, int D, long N) { return V > 0 && V <= 1 << 23 && D > 0 && D <= 1 << 21 && N >= 0 && N <= 1L << 30; }
+// what a launch has workgroups for (2^24 of 256 threads)
+bool gradient_sizes(int V, int D, long N) {
+    return V > 0 && V <= 1 << 23 && D > 0 && D <= 1 << 21 && N >= 0 && N <= 1L << 30 && std::max<long>(V, N) * D <= 1L << 34;
+}
+
+// threads that share a row, W columns each
+void share_columns(SumArgs &a, int W) {
+    a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
+    a.tiles = (int)((a.D + (long)a.lanes * W - 1) / (a.lanes * W));
+}
 
 template <typename E, typename G>
 int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
-    constexpr int W = kWide<E>;
     SumArgs a = args;
-    a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
-    const long tiles = (a.D + (long)a.lanes * W - 1) / (a.lanes * W), rows = (a.V + 256L / a.lanes - 1) / (256 / a.lanes);
     const long pieces = N / a.piece, starters = (N + a.piece - 1) / a.piece;
-    a.first_blocks = (int)(N / 256 + 1);
-    hipLaunchKernelGGL((embed_pieces_kernel<E, W>), dim3((unsigned)(a.first_blocks + pieces), (unsigned)tiles), dim3(256), 0, stream, a);
-    CNT_HIP(hipGetLastError());
+    {
+        constexpr int W = kWide<E>;
+        share_columns(a, W);
+        a.first_blocks = (int)(N / 256 + 1);
+        hipLaunchKernelGGL((embed_pieces_kernel<E, W>), dim3((unsigned)(a.first_blocks + pieces), (unsigned)a.tiles), dim3(256), 0, stream, a);
+        CNT_HIP(hipGetLastError());
+    }
+    constexpr int W = kBoth<E, G>;
+    share_columns(a, W);
+    // Four rows for a group of threads where most of the time goes into rows of zeros: fewer workgroups, and bounds of runs that are waited
+    // for once.
+    const bool four = (long)a.V * a.D >= 1L << 22;
+    const long each = 256 / a.lanes * (four ? 4 : 1), rows = (a.V + each - 1) / each;
     a.first_blocks = (int)starters;
-    hipLaunchKernelGGL((embed_rows_kernel<E, G, W>), dim3((unsigned)(starters + rows), (unsigned)tiles), dim3(256), 0, stream, a);
+    auto kernel = four ? embed_rows_kernel<E, G, W, 4> : embed_rows_kernel<E, G, W, 1>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((starters + rows) * a.tiles)), dim3(256), 0, stream, a);
     CNT_HIP(hipGetLastError());
     return CNT_OK;
 }
@@ -370,8 +420,9 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
     CNT_REQUIRE(table_stride >= 0 && out_stride >= D, "embed_forward: rows of the output overlap, or a negative stride");
     CNT_REQUIRE(table && (N == 0 || (tokens && out)), "embed_forward: null argument");
     if (N == 0) return CNT_OK;
-    LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + 7) / 8)), scale};
-    const long blocks = (N + 256 / a.lanes - 1) / (256 / a.lanes);
+    const int wide = table_type == CNT_F32 || out_type == CNT_F32 ? 4 : 8;
+    LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + wide - 1) / wide)), scale};
+    const long slots = 256 / a.lanes * kSlotsPerThread, blocks = (N + slots - 1) / slots;
     CNT_REQUIRE(blocks < 1L << 24, "embed_forward: too many slots");
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "embed_forward");

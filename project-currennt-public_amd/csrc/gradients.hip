@@ -2,7 +2,7 @@
 //
 //   norm = sqrt(sum g^2),   c = norm > max_norm ? max_norm / norm : 1,   out = c * g
 //
-// Two launches whatever the number of tensors.  The list is cut into pieces of at most 8 KB when the set is made, a wave takes a piece at a
+// Two launches whatever the number of tensors.  The list is cut into pieces of at most 4 KB when the set is made, a wave takes a piece at a
 // time, and a workgroup leaves one sum; the second launch adds the workgroups' sums up again in every workgroup (16 KB from the L2) and
 // scales.  Squares are formed and added in 64 bits: an fp32 square overflows from 1.8e19 on, and the 64-bit rate is far from what
 // bounds a pass, which is memory.  Nothing is added in an order that depends on time, so a result is the same every time.
@@ -21,7 +21,7 @@ struct Piece {
     void *out;
     int n, type;
 };
-constexpr int kPieceBytes = 8192, kMostBlocks = 2048;
+constexpr int kPieceBytes = 4096, kMostBlocks = 2048, kLineBytes = 128;
 
 // f(offset, elements) for the vectors of a lane in a piece: all of a whole piece's accesses are asked for together
 template <typename T, bool ONCE, typename F>
@@ -178,8 +178,11 @@ int cnt_gradients_create(int count, const void *const *gradients, void *const *c
             CNT_REQUIRE(reinterpret_cast<uintptr_t>(in) % size == 0 && reinterpret_cast<uintptr_t>(to) % size == 0,
                         "gradients_create: tensor %d is not aligned to its elements", i);
             CNT_REQUIRE(sizes[i] / step + (long)pieces.size() < 0x7fffffffL - 8192, "gradients_create: too many elements");
-            for (long at = 0; at < sizes[i]; at += step)
-                pieces.push_back({in + at * (long)size, to + at * (long)size, (int)std::min(step, sizes[i] - at), types[i]});
+            // a tensor that begins inside a cache line: its first piece ends with the line, so that the others read whole lines
+            long n = step;
+            if (reinterpret_cast<uintptr_t>(in) % kLineBytes) n = (long)((kLineBytes - reinterpret_cast<uintptr_t>(in) % kLineBytes) / size);
+            for (long at = 0; at < sizes[i]; at += n, n = step)
+                pieces.push_back({in + at * (long)size, to + at * (long)size, (int)std::min(n, sizes[i] - at), types[i]});
         }
         cnt_gradients *set = new cnt_gradients;
         set->count = (int)pieces.size();

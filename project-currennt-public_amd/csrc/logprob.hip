@@ -85,6 +85,54 @@ __device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int
     }
 }
 
+// 16 bytes of a row as they stand in memory.  renewed() hides that nothing has changed: the compiler would keep the 32-bit values from one use
+// to the next otherwise, which takes twice the registers of 16-bit logits.
+template <typename T>
+struct Raw {
+    typedef typename Packed<T, kWide<T>>::type vec;
+    typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
+    words x;
+    __device__ __forceinline__ void load(const T *p, bool whole) {
+        vec v;
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) v[i] = (T)kMinusInfinity;
+        x = __builtin_bit_cast(words, v);
+        if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
+    }
+    __device__ __forceinline__ void renewed() {
+        unsigned a = x[0], b = x[1], c = x[2], d = x[3];
+        asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+        x = words{a, b, c, d};
+    }
+    __device__ __forceinline__ void values(float (&v)[kWide<T>]) const {
+        const vec y = __builtin_bit_cast(vec, x);
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) v[i] = (float)y[i];
+    }
+};
+
+// a whole chunk as it stands in memory
+template <typename T, int NV>
+struct RawChunk {
+    Raw<T> part[NV];
+    __device__ __forceinline__ void load(const T *chunk, int lane) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) part[j].load(chunk + (j * 64 + lane) * kWide<T>, true);
+    }
+    __device__ __forceinline__ void values(Chunk<T, NV> &c) const {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float v[kWide<T>];
+            part[j].values(v);
+#pragma unroll
+            for (int i = 0; i < kWide<T>; ++i) c.x[j * kWide<T> + i] = v[i];
+        }
+    }
+};
+
+// up to here r - m * c is below 2^-4
+constexpr float kMostFused = 1 << 20;
+
 // ----- statistics ------------------------------------------------------------------------------------------------------------
 struct Stats {
     float m, s, w;
@@ -117,6 +165,29 @@ __device__ __forceinline__ float fold(Stats &a, const Chunk<T, NV> &x, float c) 
         a.s += e;
         a.w = __builtin_fmaf(e, at_least(t), a.w);
     }
+    return largest;
+}
+// t as one fused operation, x * c - r with r = m * c rounded, for 16-bit logits, where instructions and memory bound a pass about equally.  All
+// of a chunk's terms are off by the same factor 2^(r - m * c) then, which is known exactly and taken out of the chunk's sums.
+template <typename T, int NV>
+__device__ __forceinline__ float fold_fused(Stats &a, const Chunk<T, NV> &x, float c) {
+    float largest = x.x[0];
+#pragma unroll
+    for (int i = 1; i < Chunk<T, NV>::COUNT; ++i) largest = fmaxf(largest, x.x[i]);
+    const float m = fmaxf(a.m, largest), ref = m == kMinusInfinity ? 0.0f : m, r = ref * c;
+    if (__ballot(!(fabsf(r) <= kMostFused))) return fold(a, x, c);
+    shift_stats(a, m, ref, c);
+    const float off = __builtin_fmaf(ref, c, -r);  // m * c - r
+    float s = 0.0f, w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) {
+        const float t = __builtin_fmaf(x.x[i], c, -r), e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        w = __builtin_fmaf(e, at_least(t), w);
+    }
+    const float f = __builtin_amdgcn_exp2f(-off);
+    a.s = __builtin_fmaf(s, f, a.s);
+    a.w = __builtin_fmaf(w - s * off, f, a.w);
     return largest;
 }
 __device__ __forceinline__ Stats join(Stats a, Stats b, float c) {
@@ -325,9 +396,9 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
 // ----- long rows: a workgroup of four waves for a row or a part of one ------------------------------------------------------------
 // The best K without keeping them up to date on the way, which at K = 16 took longer than everything else (2047 rows of 100003: 200 us, of
 // which a list per wave 130): a lane remembers the largest logit of its best two chunks, and of which chunks, and that of its third.  The
-// K-th largest of the lanes' largest is a bound that K logits reach.  Only the remembered chunks' logits of their lanes
-// that reach it are read again, some 16 K of them, unless a lane's third chunk reaches it too, or ties make
-// them too many: then the row is read once more with lists.
+// K-th largest of the lanes' largest is a bound that K logits reach.  Read again are the remembered chunks that reach it, their lane's logits
+// only, some 16 K or 32 K of them, and all of a lane whose third chunk reaches it too.  Where ties or sorted rows make that too
+// many, the row is read once more with lists.
 struct Cells {
     float first, second, third;
     int first_at, second_at;
@@ -360,14 +431,15 @@ __device__ __forceinline__ unsigned kth_largest(const unsigned (&key)[COUNT], in
     return t;
 }
 
-constexpr int kMostCells = 64, kMostCandidates = 256;
+constexpr int kMostCells = 256, kMostWhole = 16, kMostCandidates = 512;
 struct Shared {
     Stats stats[4];
-    float first[256], second[256], third[4];
+    float first[256], second[256], third[256];
     int first_at[256], second_at[256];
     int cell_lane[kMostCells], cell_at[kMostCells];
+    int whole[kMostWhole];  // lanes (with their waves) all of whose chunks are read again
     unsigned least;
-    int cells, candidates;
+    int cells, wholes, candidates;
     float value[kMostCandidates];
     int token[kMostCandidates];
 };
@@ -395,11 +467,30 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
     Stats s;
     begin_stats(s);
     Cells cells = {kMinusInfinity, kMinusInfinity, kMinusInfinity, -1, -1};
-    for (int at = begin + wave * SPAN; at < end; at += 4 * SPAN) {
+    auto take = [&](const X &x, int at) {
+        const float largest = sizeof(T) == 2 ? fold_fused(s, x, c) : fold(s, x, c);
+        if (TOP) remember(cells, largest, at);
+    };
+    // whole chunks, each asked for while the one before is worked on; what is left behind the last of them
+    int at = begin + wave * SPAN;
+    if (at + SPAN <= end) {
+        RawChunk<T, NV> next;
+        next.load(row + at, lane);
+        while (true) {
+            RawChunk<T, NV> now = next;
+            const int here = at;
+            at += 4 * SPAN;
+            if (at + SPAN <= end) next.load(row + at, lane);
+            X x;
+            now.values(x);
+            take(x, here);
+            if (at + SPAN > end) break;
+        }
+    }
+    if (at < end) {
         X x;
         load_chunk<true>(row, at, end, lane, x);
-        const float largest = fold(s, x, c);
-        if (TOP) remember(cells, largest, at);
+        take(x, at);
     }
     s = join_lanes(s, c);
     if (lane == 0) sh.stats[wave] = s;
@@ -408,8 +499,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
         sh.second[threadIdx.x] = cells.second;
         sh.first_at[threadIdx.x] = cells.first_at;
         sh.second_at[threadIdx.x] = cells.second_at;
-        const float third = max_of<64>(cells.third);
-        if (lane == 0) sh.third[wave] = third;
+        sh.third[threadIdx.x] = cells.third;
     }
     __syncthreads();
     s = sh.stats[0];
@@ -441,23 +531,29 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) key[w] = ordered(sh.first[w * 64 + lane]);
         const unsigned least = kth_largest<4>(key, 256, a.K);
-        bool plain = ordered(fmaxf(fmaxf(sh.third[0], sh.third[1]), fmaxf(sh.third[2], sh.third[3]))) < least;
-        int count = 0;
+        int wholes = 0, count = 0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 12; ++q) {  // third, first, second
             const int from = q % 4 * 64 + lane;
-            const bool in = ordered(q < 4 ? sh.first[from] : sh.second[from]) >= least;
+            const bool whole = ordered(sh.third[from]) >= least;
+            const bool in = q < 4 ? whole : !whole && ordered(q < 8 ? sh.first[from] : sh.second[from]) >= least;
             const unsigned long long b = __ballot(in);
-            const int place = count + __popcll(b & ((1ull << lane) - 1));
-            if (plain && in && place < kMostCells) {
-                sh.cell_lane[place] = lane;
-                sh.cell_at[place] = q < 4 ? sh.first_at[from] : sh.second_at[from];
+            const int place = (q < 4 ? wholes : count) + __popcll(b & ((1ull << lane) - 1));
+            if (q < 4) {
+                if (in && place < kMostWhole) sh.whole[place] = from;
+                wholes += __popcll(b);
+            } else {
+                if (in && place < kMostCells) {
+                    sh.cell_lane[place] = lane;
+                    sh.cell_at[place] = q < 8 ? sh.first_at[from] : sh.second_at[from];
+                }
+                count += __popcll(b);
             }
-            count += __popcll(b);
         }
         if (lane == 0) {
             sh.least = least;
-            sh.cells = plain && count <= kMostCells ? count : -1;
+            sh.cells = wholes <= kMostWhole && count <= kMostCells ? count : -1;
+            sh.wholes = wholes;
             sh.candidates = 0;
         }
     }
@@ -466,8 +562,8 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
     bool listed = n_cells < 0;
     if (!listed) {
         const unsigned least = sh.least;
-        for (int i = threadIdx.x; i < n_cells * NV; i += 256) {
-            const int cell = i / NV, first = sh.cell_at[cell] + (i % NV * 64 + sh.cell_lane[cell]) * W;
+        auto look = [&](int chunk, int of, int vec) {
+            const int first = chunk + (vec * 64 + of) * W;
             float v[W];
             fetch_some<T, W>(row + first, max(0, min(W, end - first)), v, __builtin_nanf(""));
 #pragma unroll
@@ -480,10 +576,17 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
                     }
                 }
             }
+        };
+        for (int i = threadIdx.x; i < n_cells * NV; i += 256) look(sh.cell_at[i / NV], sh.cell_lane[i / NV], i % NV);
+        const int rounds = (end - begin + 4 * SPAN - 1) / (4 * SPAN), each = rounds * NV;
+        for (int i = threadIdx.x; i < sh.wholes * each; i += 256) {
+            const int from = sh.whole[i / each], of = from & 63, in = i % each;
+            look(begin + (in / NV * 4 + from / 64) * SPAN, of, in % NV);
         }
         __syncthreads();
         listed = sh.candidates > kMostCandidates;
-        if (!listed && (int)threadIdx.x < sh.candidates) rank_entry(sh.value, sh.token, sh.candidates, threadIdx.x, a.K, put);
+        const int candidates = sh.candidates;
+        for (int i = threadIdx.x; !listed && i < candidates; i += 256) rank_entry(sh.value, sh.token, candidates, i, a.K, put);
     }
     if (!listed) return;
     // the row again, with a list per wave
@@ -646,32 +749,6 @@ __global__ __launch_bounds__(256) void logprob_short_error_kernel(const RowArgs 
     }
 }
 
-// 16 bytes of a row as they stand in memory.  renewed() hides that nothing has changed: the compiler would keep the 32-bit values from one use
-// to the next otherwise, which takes twice the registers of 16-bit logits.
-template <typename T>
-struct Raw {
-    typedef typename Packed<T, kWide<T>>::type vec;
-    typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
-    words x;
-    __device__ __forceinline__ void load(const T *p, bool whole) {
-        vec v;
-#pragma unroll
-        for (int i = 0; i < kWide<T>; ++i) v[i] = (T)kMinusInfinity;
-        x = __builtin_bit_cast(words, v);
-        if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
-    }
-    __device__ __forceinline__ void renewed() {
-        unsigned a = x[0], b = x[1], c = x[2], d = x[3];
-        asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
-        x = words{a, b, c, d};
-    }
-    __device__ __forceinline__ void values(float (&v)[kWide<T>]) const {
-        const vec y = __builtin_bit_cast(vec, x);
-#pragma unroll
-        for (int i = 0; i < kWide<T>; ++i) v[i] = (float)y[i];
-    }
-};
-
 // A long row that a workgroup of THREADS holds in registers, NV vectors per thread: read once, written once.  GROUPS: workgroups that a compute
 // unit has registers for, so that one's loads and stores go on while another computes.
 template <typename T, int NV, int THREADS, int GROUPS>
@@ -711,7 +788,11 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     const int w = lane % 16;  // every 16 lanes add the waves up
     m = max_of<16>(w < WAVES ? maxima[w] : kMinusInfinity);
     m = m == m ? m : kMinusInfinity;  // (all NaN)
-    const float ref = m == kMinusInfinity ? 0.0f : m, t_rest = (rest - ref) * c, e_rest = __builtin_amdgcn_exp2f(t_rest);
+    const float ref = m == kMinusInfinity ? 0.0f : m, r = ref * c;
+    // (see fold_fused; the whole workgroup has one maximum here)
+    const bool fused = sizeof(T) == 2 && fabsf(r) <= kMostFused;
+    const float off = fused ? __builtin_fmaf(ref, c, -r) : 0.0f;
+    const float t_rest = fused ? __builtin_fmaf(rest, c, -r) : (rest - ref) * c, e_rest = __builtin_amdgcn_exp2f(t_rest);
     Stats s = {m, e_rest, e_rest * at_least(t_rest)};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -719,7 +800,7 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         x[j].values(v);
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const float t = (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+            const float t = fused ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
             s.s += e;
             s.w = __builtin_fmaf(e, at_least(t), s.w);
         }
@@ -735,6 +816,11 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     __syncthreads();
     s.s = sum_of<16>(w < WAVES ? sums[w] : 0.0f);
     s.w = sum_of<16>(w < WAVES ? means[w] : 0.0f);
+    if (fused) {
+        const float f = __builtin_amdgcn_exp2f(-off);
+        s.w = (s.w - s.s * off) * f;
+        s.s *= f;
+    }
     const float log_s = logf(s.s), log2_s = log_s * kLog2e, entropy = entropy_of(s, log_s), lse = s.m * a.scale + log_s;
     if (threadIdx.x == 0) {
         if (a.logp) a.logp[n] = token >= 0 && token < a.V ? logp_of(given, s, a.scale, log_s) : 0.0f;
@@ -754,7 +840,7 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         __builtin_amdgcn_sched_barrier(0);
     }
     if (behind < a.V) {
-        float t[1] = {t_rest - log2_s};
+        float t[1] = {(rest - ref) * c - log2_s};
         errors_of<1>(behind, slopes, t);
         to[behind] = (T)t[0];
     }

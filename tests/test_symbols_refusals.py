@@ -26,7 +26,7 @@ def test_embedding():
     _refused(f(None, 4, 4, 2, 0, P, 4, P, 1.0, 0, P, 3), "overlap")
     _refused(f(None, 4, 4, 2, 0, None, 4, P, 1.0, 0, P, 4), "null")
     _refused(f(None, 4, 4, 2, 0, P, 4, None, 1.0, 0, P, 4), "null")
-    _refused(f(None, 4, 4096, 1 << 24, 0, P, 4096, P, 1.0, 0, P, 4096), "too many")
+    _refused(f(None, 4, 4096, 1 << 26, 0, P, 4096, P, 1.0, 0, P, 4096), "too many")
     assert f(None, 4, 4, 0, 0, P, 4, None, 1.0, 0, None, 4) == 0
     assert L.cnt_embed_scratch(0, 4, 2) == -1 and L.cnt_embed_scratch(4, 4, -1) == -1 and L.cnt_embed_scratch(4, 4, 2 ** 31) == -1
     need = L.cnt_embed_scratch(100, 8, 50)
@@ -38,7 +38,7 @@ def test_embedding():
         a.update(changes)
         return g(*a.values())
 
-    for changes, what in (({"V": 0}, "sizes"), ({"N": -1}, "sizes"), ({"N": 2 ** 31}, "sizes"), ({"V": 2 ** 23 + 1}, "sizes"), ({"D": 2 ** 21 + 1}, "sizes"), ({"et": 7}, "element type"),
+    for changes, what in (({"V": 0}, "sizes"), ({"N": -1}, "sizes"), ({"N": 2 ** 31}, "sizes"), ({"V": 2 ** 23 + 1}, "sizes"), ({"D": 2 ** 21 + 1}, "sizes"), ({"V": 2 ** 20, "D": 2 ** 14 + 1}, "sizes"), ({"N": 2 ** 20, "D": 2 ** 14 + 1}, "sizes"), ({"et": 7}, "element type"),
                           ({"gt": 7}, "element type"), ({"es": -1}, "stride"), ({"gs": 7}, "overlap"), ({"err": None}, "null"),
                           ({"grad": None}, "null"), ({"scratch": None}, "null"), ({"bytes": need - 1}, "scratch"),
                           ({"scratch": C.c_void_p(4100)}, "aligned")):
