@@ -116,13 +116,29 @@ __device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIR
 template <bool FIRST>
 __device__ __forceinline__ void count_digits(const SortArgs &a, long begin, long end, int first, long step, int *bins) {
     constexpr int U = 8;  // loads in flight
-    for (long i = begin + first; i < end; i += U * step) {
+    // (whole waves go round, so that all lanes take part in the ballots)
+    for (long i = begin + first; i - (threadIdx.x & 63) < end; i += U * step) {
         int key[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) key[u] = i + u * step < end ? a.keys[i + u * step] : -1;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (key[u] >= 0 && listed<FIRST>(a, key[u])) atomicAdd(&bins[(key[u] >> a.shift) & ((1 << a.bits) - 1)], 1);
+        for (int u = 0; u < U; ++u) {
+            const bool in = key[u] >= 0 && listed<FIRST>(a, key[u]);
+            const int digit = (key[u] >> a.shift) & ((1 << a.bits) - 1);
+            if (FIRST) {
+                if (in) atomicAdd(&bins[digit], 1);
+                continue;
+            }
+            // Upper digits: that of the wave's first entry is counted at once.  Half of all tokens have the same one, and additions to
+            // one address go one by one (second pass of 16384 tokens of 65536: 12.4 us so, 9.4 us with a count; the first one's 7.4 and 9.6).
+            const unsigned long long all = __ballot(in);
+            if (all) {
+                const int common = __builtin_amdgcn_readlane(digit, __builtin_ctzll(all));
+                const unsigned long long same = __ballot(in && digit == common);
+                if ((threadIdx.x & 63) == __builtin_ctzll(same)) atomicAdd(&bins[common], (int)__popcll(same));
+                if (in && digit != common) atomicAdd(&bins[digit], 1);
+            }
+        }
     }
 }
 
@@ -239,25 +255,30 @@ struct SumArgs {
     float scale;
 };
 
-// sum of entries first, first + step, ... < end of the sorted list, W columns from `column` on
+// Sum of entries first, first + step, ... < end of the sorted list, W columns from `column` on, by the `lanes` threads of a group: every thread
+// has one of the next slots, which go round the group, so that a slot is waited for once in `lanes` entries.
 template <typename E, int W>
 __device__ __forceinline__ void add_entries(const SumArgs &a, int first, int end, int step, int column, int count, float (&sum)[W]) {
+    constexpr int U = 8;  // rows in flight
     const E *err = static_cast<const E *>(a.err) + column;
-    int i = first;
-    for (; i + 3 * step < end; i += 4 * step) {
-        float v[4][W];
+    const int x = threadIdx.x % a.lanes;
+    for (int i = first; i < end; i += a.lanes * step) {
+        const int mine = i + x * step < end ? a.slots[i + x * step] : 0;
+        const int rows = min(a.lanes, (end - i + step - 1) / step);
+        for (int k = 0; k < rows; k += U) {
+            float v[U][W];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) fetch_some<E, W>(err + a.slots[i + u * step] * a.err_stride, count, v[u], 0.0f);
+            for (int u = 0; u < U; ++u) {
+                const int slot = __shfl(mine, k + u, a.lanes);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+                for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
+                if (k + u < rows && count > 0) fetch_some<E, W>(err + slot * a.err_stride, count, v[u], 0.0f);
+            }
 #pragma unroll
-            for (int q = 0; q < W; ++q) sum[q] += v[u][q];
-    }
-    for (; i < end; i += step) {
-        float v[W];
-        fetch_some<E, W>(err + a.slots[i] * a.err_stride, count, v, 0.0f);
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int q = 0; q < W; ++q) sum[q] += v[q];
+                for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+        }
     }
 }
 
@@ -309,7 +330,7 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const SumArgs a) {
     const int x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
     const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
     float sum[W] = {};
-    if (count > 0) add_entries<E, W>(a, begin + g, end, 256 / a.lanes, column, count, sum);
+    add_entries<E, W>(a, begin + g, end, 256 / a.lanes, column, count, sum);
     join_groups<W>(a.lanes, sum);
     if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)piece * a.D + column, count, sum);
 }
@@ -338,23 +359,23 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         const int row = a.keys[here], begin = a.starts[row], end = a.starts[row + 1];
         if (here - begin >= a.piece) return;
         const int whole = end / a.piece * a.piece;  // >= here
+        add_entries<E, W>(a, begin + g, here, groups, column, count, sum);
         if (count > 0) {
-            add_entries<E, W>(a, begin + g, here, groups, column, count, sum);
+#pragma unroll 4
             for (int p = block + g; p < whole / a.piece; p += groups) {
                 float v[W];
                 fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
 #pragma unroll
                 for (int q = 0; q < W; ++q) sum[q] += v[q];
             }
-            add_entries<E, W>(a, whole + g, end, groups, column, count, sum);
         }
+        add_entries<E, W>(a, whole + g, end, groups, column, count, sum);
         join_groups<W>(a.lanes, sum);
         if (g == 0) write_row<G, W>(a, row, true, column, count, sum);
         return;
     }
     // A group's rows are far apart: frequent tokens are neighbours in most vocabularies.
     const long first = (long)(block - a.first_blocks) * groups + g, step = (long)(gridDim.x / a.tiles - a.first_blocks) * groups;
-    if (count <= 0) return;
     int begin[R], end[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -379,7 +400,7 @@ bool gradient_sizes(int V, int D, long N) {
 
 // threads that share a row, W columns each
 void share_columns(SumArgs &a, int W) {
-    a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
+    a.lanes = std::max(8, std::min(64, power_of_two_from((a.D + W - 1) / W)));  // (eight: as many rows are in flight)
     a.tiles = (int)((a.D + (long)a.lanes * W - 1) / (a.lanes * W));
 }
 

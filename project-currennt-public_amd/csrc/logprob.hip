@@ -69,45 +69,71 @@ struct Chunk {
     static constexpr int W = kWide<T>, COUNT = NV * W, SPAN = 64 * COUNT;
     float x[COUNT];
 };
-// logits begin .. begin + SPAN of a row, those from `end` on are -inf
+// Logits of a row are dealt to threads in vectors from a cache line's begin on, `lead` logits before the row's first one, if the row begins inside a
+// line: 16-byte accesses that do not begin at 16 bytes took a fifth longer (2047 rows of 100003 16-bit logits: 97 us for 84).
+template <typename T>
+__device__ __forceinline__ int lead_of(const T *row) { return (int)(reinterpret_cast<uintptr_t>(row) % 128 / sizeof(T)); }
+// W logits from `at` on, those before the row and from `end` on are `rest`
+template <bool ONCE, typename T, int W>
+__device__ __forceinline__ void fetch_within(const T *row, int at, int end, float (&v)[W], float rest) {
+    if (at >= 0 && at + W <= end) {
+        fetch_elements<T, W, ONCE>(row + at, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = at + i >= 0 && at + i < end ? (float)row[at + i] : rest;
+}
+template <typename T, int W>
+__device__ __forceinline__ void put_within(T *row, int at, int end, const float (&v)[W]) {
+    if (at >= 0 && at + W <= end) {
+        put_elements<T, W, true>(row + at, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+        if (at + i >= 0 && at + i < end) row[at + i] = (T)v[i];
+}
+// logits begin .. begin + SPAN of a row, those outside of 0 .. end are -inf
 template <bool ONCE, typename T, int NV>
 __device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int lane, Chunk<T, NV> &c) {
     constexpr int W = Chunk<T, NV>::W;
-    const bool whole = begin + Chunk<T, NV>::SPAN <= end;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int at = begin + (j * 64 + lane) * W;
         float v[W];
-        if (whole) fetch_elements<T, W, ONCE>(row + at, v);
-        else fetch_some<T, W, ONCE>(row + at, max(0, min(W, end - at)), v, kMinusInfinity);
+        fetch_within<ONCE>(row, begin + (j * 64 + lane) * W, end, v, kMinusInfinity);
 #pragma unroll
         for (int i = 0; i < W; ++i) c.x[j * W + i] = v[i];
     }
 }
 
-// 16 bytes of a row as they stand in memory.  renewed() hides that nothing has changed: the compiler would keep the 32-bit values from one use
-// to the next otherwise, which takes twice the registers of 16-bit logits.
+// 16 bytes of a row as they stand in memory.  values<USE>(): the logits in 32 bits, converted anew for every USE: from expressions that it knows to be
+// the same the compiler keeps one use's 32-bit values for the next, which takes twice the registers of 16-bit logits.
+template <int USE>
+__device__ __forceinline__ void halves(unsigned x, float &low, float &high, __bf16) {
+    asm("v_lshlrev_b32 %0, 16, %1 ; %2" : "=v"(low) : "v"(x), "i"(USE));
+    asm("v_and_b32 %0, 0xffff0000, %1 ; %2" : "=v"(high) : "v"(x), "i"(USE));
+}
+template <int USE>
+__device__ __forceinline__ void halves(unsigned x, float &low, float &high, _Float16) {
+    asm("v_cvt_f32_f16 %0, %1 ; %2" : "=v"(low) : "v"(x), "i"(USE));
+    asm("v_cvt_f32_f16_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1 ; %2" : "=v"(high) : "v"(x), "i"(USE));
+}
 template <typename T>
 struct Raw {
-    typedef typename Packed<T, kWide<T>>::type vec;
     typedef unsigned words __attribute__((ext_vector_type(4), aligned(2)));
     words x;
+    // (a vector that is not there is never looked at)
     __device__ __forceinline__ void load(const T *p, bool whole) {
-        vec v;
-#pragma unroll
-        for (int i = 0; i < kWide<T>; ++i) v[i] = (T)kMinusInfinity;
-        x = __builtin_bit_cast(words, v);
+        x = words{0u, 0u, 0u, 0u};
         if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
     }
-    __device__ __forceinline__ void renewed() {
-        unsigned a = x[0], b = x[1], c = x[2], d = x[3];
-        asm volatile("" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
-        x = words{a, b, c, d};
-    }
+    template <int USE>
     __device__ __forceinline__ void values(float (&v)[kWide<T>]) const {
-        const vec y = __builtin_bit_cast(vec, x);
 #pragma unroll
-        for (int i = 0; i < kWide<T>; ++i) v[i] = (float)y[i];
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(x[i]);
+            else halves<USE>(x[i], v[2 * i], v[2 * i + 1], T());
+        }
     }
 };
 
@@ -123,7 +149,7 @@ struct RawChunk {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             float v[kWide<T>];
-            part[j].values(v);
+            part[j].template values<0>(v);
 #pragma unroll
             for (int i = 0; i < kWide<T>; ++i) c.x[j * kWide<T> + i] = v[i];
         }
@@ -199,10 +225,10 @@ __device__ __forceinline__ Stats join(Stats a, Stats b, float c) {
     return a;
 }
 __device__ __forceinline__ Stats join_lanes(Stats a, float c) {
-    for (int o = 32; o > 0; o >>= 1) {
-        const Stats b = {__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.w, o)};
-        a = join(a, b, c);
-    }
+    const float m = max_of<64>(a.m);
+    shift_stats(a, m, m == kMinusInfinity ? 0.0f : m, c);
+    a.s = sum_of<64>(a.s);
+    a.w = sum_of<64>(a.w);
     return a;
 }
 
@@ -233,12 +259,12 @@ template <typename T, int NV>
 __device__ __forceinline__ void take_best(Best &b, Chunk<T, NV> &c, int begin, int end, int K, int lane) {
     constexpr int W = Chunk<T, NV>::W;
     float top[NV], best = __builtin_nanf("");
-    if (begin + Chunk<T, NV>::SPAN > end) {
+    if (begin < 0 || begin + Chunk<T, NV>::SPAN > end) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < W; ++i)
-                if (begin + (j * 64 + lane) * W + i >= end) c.x[j * W + i] = __builtin_nanf("");
+                if (begin + (j * 64 + lane) * W + i < 0 || begin + (j * 64 + lane) * W + i >= end) c.x[j * W + i] = __builtin_nanf("");
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -386,10 +412,11 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
         for (int i = COUNT - 1; i >= 0; --i) at = x.x[i] == best ? i : at;
         const float m = max_of<LANES>(best);
         const int token = min_of<LANES>(best == m ? x.index(at, l) : INT_MAX);
+        if (here && l == 0) write_top(a, n, k, m, token == INT_MAX ? -1 : token, s, log_s);
+        if (k + 1 == a.K) break;
         const int taken = best == m && x.index(at, l) == token ? at : -1;
 #pragma unroll
         for (int i = 0; i < COUNT; ++i) x.x[i] = i == taken ? __builtin_nanf("") : x.x[i];
-        if (here && l == 0) write_top(a, n, k, m, token == INT_MAX ? -1 : token, s, log_s);
     }
 }
 
@@ -416,17 +443,30 @@ __device__ __forceinline__ unsigned ordered(float v) {
     const unsigned u = __float_as_uint(v + 0.0f);
     return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
-// the K-th largest of a wave's keys, up to COUNT per lane, `entries` in all; 0: there are fewer, keys of 0 being none
+// A bound that at least K of a wave's keys reach, and exactly K where no two are equal: keys up to COUNT per lane, `entries` in all; 0: there are
+// fewer, keys of 0 being none.  Bit by bit from the first on that not all keys have in common.
 template <int COUNT>
-__device__ __forceinline__ unsigned kth_largest(const unsigned (&key)[COUNT], int entries, int K) {
-    unsigned t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+__device__ __forceinline__ unsigned bound_of(const unsigned (&key)[COUNT], int entries, int K) {
+    unsigned all = ~0u, any = 0;
+#pragma unroll
+    for (int q = 0; q < COUNT; ++q)
+        if (q * 64 < entries) {
+            all &= key[q];
+            any |= key[q];
+        }
+    all = over_lanes<64>((int)all, [](int a, int b) { return a & b; });
+    any = over_lanes<64>((int)any, [](int a, int b) { return a | b; });
+    const unsigned differ = any & ~all;
+    const int top = differ ? 31 - __builtin_clz(differ) : -1;
+    unsigned t = top < 0 ? all : all & ~((2u << top) - 1);
+    for (int bit = top; bit >= 0; --bit) {
         const unsigned more = t | 1u << bit;
         int count = 0;
 #pragma unroll
         for (int q = 0; q < COUNT; ++q)
             if (q * 64 < entries) count += __popcll(__ballot(key[q] >= more));
-        t = count >= K ? more : t;
+        if (count >= K) t = more;
+        if (count == K) break;
     }
     return t;
 }
@@ -454,8 +494,9 @@ __device__ __forceinline__ void rank_entry(const float *value, const int *token,
     if (rank < K) f(rank, v, t);
 }
 
+// (registers for eight workgroups of a compute unit: with seven, 2047 rows with alternatives took two rounds of the card)
 template <typename T, int NV, bool TOP>
-__global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
+__global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
     using X = Chunk<T, NV>;
     constexpr int SPAN = X::SPAN, W = X::W;
     __shared__ Shared sh;
@@ -463,7 +504,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
     const long n = blockIdx.x;
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-    const int begin = (int)blockIdx.y * a.part, end = min(a.V, begin + a.part);
+    const int begin = (int)blockIdx.y * a.part - lead_of(row), end = min(a.V, begin + a.part);
     Stats s;
     begin_stats(s);
     Cells cells = {kMinusInfinity, kMinusInfinity, kMinusInfinity, -1, -1};
@@ -471,8 +512,17 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
         const float largest = sizeof(T) == 2 ? fold_fused(s, x, c) : fold(s, x, c);
         if (TOP) remember(cells, largest, at);
     };
-    // whole chunks, each asked for while the one before is worked on; what is left behind the last of them
+    // the first chunk, if the row begins within it; whole ones, each asked for while the one before is worked on; the rest of the last one
+    auto take_part = [&](int at) {
+        X x;
+        load_chunk<true>(row, at, end, lane, x);
+        take(x, at);
+    };
     int at = begin + wave * SPAN;
+    if (at < 0) {
+        take_part(at);
+        at += 4 * SPAN;
+    }
     if (at + SPAN <= end) {
         RawChunk<T, NV> next;
         next.load(row + at, lane);
@@ -487,11 +537,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
             if (at + SPAN > end) break;
         }
     }
-    if (at < end) {
-        X x;
-        load_chunk<true>(row, at, end, lane, x);
-        take(x, at);
-    }
+    if (at < end) take_part(at);
     s = join_lanes(s, c);
     if (lane == 0) sh.stats[wave] = s;
     if (TOP) {
@@ -530,7 +576,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
         unsigned key[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) key[w] = ordered(sh.first[w * 64 + lane]);
-        const unsigned least = kth_largest<4>(key, 256, a.K);
+        const unsigned least = bound_of<4>(key, 256, a.K);
         int wholes = 0, count = 0;
 #pragma unroll
         for (int q = 0; q < 12; ++q) {  // third, first, second
@@ -565,7 +611,7 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
         auto look = [&](int chunk, int of, int vec) {
             const int first = chunk + (vec * 64 + of) * W;
             float v[W];
-            fetch_some<T, W>(row + first, max(0, min(W, end - first)), v, __builtin_nanf(""));
+            fetch_within<false>(row, first, end, v, __builtin_nanf(""));
 #pragma unroll
             for (int q = 0; q < W; ++q) {
                 if (v[q] == v[q] && ordered(v[q]) >= least) {
@@ -609,11 +655,11 @@ __global__ __launch_bounds__(256) void logprob_kernel(const RowArgs a) {
     if (lane < a.K) put(lane, b.value, lane < b.count ? b.token : -1);
 }
 
-// The parts of a row, by a wave: up to 16 * 64 alternatives of all parts.
-template <typename T>
+// The parts of a row, by a wave: up to Q * 64 alternatives of all parts.
+template <typename T, int Q>
 __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
-    __shared__ float value[kMostJoined];
-    __shared__ int token[kMostJoined];
+    __shared__ float value[Q * 64];
+    __shared__ int token[Q * 64];
     const long n = blockIdx.x;
     const int lane = threadIdx.x;
     const float c = a.scale * kLog2e;
@@ -621,11 +667,11 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
     begin_stats(s);
     const long p = n * a.parts;
     if (lane < a.parts) s = {a.part_stats[(p + lane) * 3], a.part_stats[(p + lane) * 3 + 1], a.part_stats[(p + lane) * 3 + 2]};
-    float v[kMostJoined / 64];
-    int t[kMostJoined / 64];
+    float v[Q];
+    int t[Q];
     const int entries = a.parts * a.K;
 #pragma unroll
-    for (int q = 0; q < kMostJoined / 64; ++q) {
+    for (int q = 0; q < Q; ++q) {
         const int i = q * 64 + lane;
         v[q] = i < entries ? a.part_values[p * a.K + i] : 0.0f;
         t[q] = i < entries ? a.part_tokens[p * a.K + i] : -1;
@@ -634,13 +680,13 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
     const float log_s = logf(s.s);
     if (lane == 0) write_stats<T>(a, n, s, log_s);
     if (a.K == 0) return;
-    unsigned key[kMostJoined / 64];
+    unsigned key[Q];
 #pragma unroll
-    for (int q = 0; q < kMostJoined / 64; ++q) key[q] = t[q] >= 0 ? ordered(v[q]) : 0u;
-    const unsigned least = max(1u, kth_largest<kMostJoined / 64>(key, entries, a.K));
+    for (int q = 0; q < Q; ++q) key[q] = t[q] >= 0 ? ordered(v[q]) : 0u;
+    const unsigned least = max(1u, bound_of<Q>(key, entries, a.K));
     int count = 0;
 #pragma unroll
-    for (int q = 0; q < kMostJoined / 64; ++q) {
+    for (int q = 0; q < Q; ++q) {
         const unsigned long long b = __ballot(key[q] >= least);
         const int place = count + __popcll(b & ((1ull << lane) - 1));
         if (key[q] >= least) {
@@ -664,7 +710,8 @@ struct Slopes {
 __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse, float entropy) {
     int token = a.tokens ? a.tokens[n] : -1;
     if (token >= a.V || token < 0) token = -1;
-    const float g = a.logp_err && token >= 0 ? a.logp_err[n] : 0.0f, h = a.entropy_err ? a.entropy_err[n] : 0.0f;
+    const float error = a.logp_err ? a.logp_err[n] : 0.0f;  // (not waiting for the token)
+    const float g = token >= 0 ? error : 0.0f, h = a.entropy_err ? a.entropy_err[n] : 0.0f;
     Slopes s;
     s.first = -a.scale * (h == 0.0f ? g : g + h * entropy);
     s.second = -a.scale * h * kLn2;
@@ -673,12 +720,12 @@ __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse,
     if (lse != lse) s.first = lse;
     return s;
 }
-// W errors of a row from logit `at` on in the place of log2 of the probabilities
-template <int W>
+// W errors of a row from logit `at` on in the place of log2 of the probabilities; CLAMPED: some of which may be -inf
+template <int W, bool CLAMPED>
 __device__ __forceinline__ void errors_of(int at, const Slopes &s, float (&t)[W]) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float u = at_least(t[i]);
+        const float u = CLAMPED ? at_least(t[i]) : t[i];
         t[i] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(s.second, u, s.first);
     }
     if ((unsigned)(s.token - at) < (unsigned)W) {
@@ -688,8 +735,8 @@ __device__ __forceinline__ void errors_of(int at, const Slopes &s, float (&t)[W]
 }
 template <typename T, int W>
 __device__ __forceinline__ void put_errors(T *row, int at, int end, const Slopes &s, float (&t)[W]) {
-    errors_of<W>(at, s, t);
-    put_some<T, W, true>(row + at, max(0, min(W, end - at)), t);
+    errors_of<W, true>(at, s, t);
+    put_within(row, at, end, t);
 }
 template <typename T, int NV>
 __device__ __forceinline__ void put_gradient(T *row, int begin, int end, int lane, const Slopes &s, const Chunk<T, NV> &t) {
@@ -709,17 +756,20 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) 
     constexpr int SPAN = Chunk<T, NV>::SPAN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long n = blockIdx.x;
-    const float lse = a.lse[n];
-    const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
+    int at = (blockIdx.y * 4 + wave) * SPAN - lead_of(row);
+    Chunk<T, NV> x;
+    load_chunk<true>(row, at, a.V, lane, x);  // (a wave has one chunk but for very long rows: asked for in front of the row's values)
+    const float lse = a.lse[n];
+    const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
     const float ref = lse == kMinusInfinity ? 0.0f : lse;
-    for (int at = (blockIdx.y * 4 + wave) * SPAN; at < a.V; at += gridDim.y * 4 * SPAN) {
-        Chunk<T, NV> x;
-        load_chunk<true>(row, at, a.V, lane, x);
+    while (at < a.V) {
 #pragma unroll
         for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = __builtin_fmaf(x.x[i], a.scale, -ref) * kLog2e;
         put_gradient(to, at, a.V, lane, s, x);
+        at += gridDim.y * 4 * SPAN;
+        load_chunk<true>(row, at, a.V, lane, x);
     }
 }
 
@@ -761,25 +811,39 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
     const int token = a.tokens ? a.tokens[n] : -1;
-    // the row's whole vectors, and what is left behind them, one logit for each of the first threads
+    // the row's whole vectors; what stands in front of and behind them, a logit for each of the first threads of two waves
+    const int lead = lead_of(row);
     Raw<T> x[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int at = (j * THREADS + (int)threadIdx.x) * W;
-        x[j].load(row + at, at + W <= a.V);
+        const int at = (j * THREADS + (int)threadIdx.x) * W - lead;
+        x[j].load(row + at, at >= 0 && at + W <= a.V);
     }
-    const int behind = a.V / W * W + (int)threadIdx.x;
-    const float rest = behind < a.V ? (float)row[behind] : kMinusInfinity;
-    float m = rest;
+    const int front = (W - lead % W) % W;
+    int other = wave == 0 && lane < front ? lane : -1;
+    if (wave == 1 && lane < (a.V - front) % W) other = front + (a.V - front) / W * W + lane;
+    const float rest = other >= 0 ? (float)row[other] : kMinusInfinity;
+    // f(at, v) for the vectors that the row fills, one after another
+    auto for_vectors = [&](auto use, auto f) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float v[W];
-        x[j].values(v);
+        for (int j = 0; j < NV; ++j) {
+            const int at = (j * THREADS + (int)threadIdx.x) * W - lead;
+            if (at >= 0 && at + W <= a.V) {
+                float v[W];
+                x[j].template values<use.value>(v);
+                f(at, v);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    float m = rest, low = 0.0f;
+    for_vectors(std::integral_constant<int, 1>(), [&](int, const float (&v)[W]) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) m = fmaxf(m, v[i]);
-        x[j].renewed();
-        __builtin_amdgcn_sched_barrier(0);  // (one vector's values at a time)
-    }
+        for (int i = 0; i < W; ++i) {
+            m = fmaxf(m, v[i]);
+            low = fminf(low, v[i]);
+        }
+    });
     m = max_of<64>(m);
     if (lane == 0) maxima[wave] = m;
     // the errors may take the logits' place: the given token's logit is kept before any of them is written
@@ -794,19 +858,22 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     const float off = fused ? __builtin_fmaf(ref, c, -r) : 0.0f;
     const float t_rest = fused ? __builtin_fmaf(rest, c, -r) : (rest - ref) * c, e_rest = __builtin_amdgcn_exp2f(t_rest);
     Stats s = {m, e_rest, e_rest * at_least(t_rest)};
+    // Logits whose t is -inf, which have to be kept from 0 * -inf, are looked for once: most waves have none.
+    const bool ruled_out = __ballot((low - ref) * c < -1e38f) != 0;
+    const std::true_type yes;
+    const std::false_type no;
+    for_vectors(std::integral_constant<int, 2>(), [&](int, const float (&v)[W]) {
+        auto add = [&](auto is_fused, auto clamped) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float v[W];
-        x[j].values(v);
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const float t = fused ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
-            s.s += e;
-            s.w = __builtin_fmaf(e, at_least(t), s.w);
-        }
-        x[j].renewed();
-        __builtin_amdgcn_sched_barrier(0);  // (one vector's values at a time)
-    }
+            for (int i = 0; i < W; ++i) {
+                const float t = is_fused.value ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+                s.s += e;
+                s.w = __builtin_fmaf(e, clamped.value ? at_least(t) : t, s.w);
+            }
+        };
+        if (sizeof(T) == 2 && fused) ruled_out ? add(yes, yes) : add(yes, no);
+        else ruled_out ? add(no, yes) : add(no, no);
+    });
     s.s = sum_of<64>(s.s);
     s.w = sum_of<64>(s.w);
     if (lane == 0) {
@@ -828,21 +895,17 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         a.entropy[n] = entropy;
     }
     const Slopes slopes = slopes_of(a, n, lse, entropy);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float t[W];
-        x[j].values(t);
+    for_vectors(std::integral_constant<int, 3>(), [&](int at, float (&t)[W]) {
 #pragma unroll
         for (int i = 0; i < W; ++i) t[i] = (t[i] - ref) * c - log2_s;
-        const int at = (j * THREADS + (int)threadIdx.x) * W;
-        errors_of<W>(at, slopes, t);
-        if (at + W <= a.V) put_elements<T, W, true>(to + at, t);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    if (behind < a.V) {
+        if (ruled_out) errors_of<W, true>(at, slopes, t);
+        else errors_of<W, false>(at, slopes, t);
+        put_elements<T, W, true>(to + at, t);
+    });
+    if (other >= 0) {
         float t[1] = {(rest - ref) * c - log2_s};
-        errors_of<1>(behind, slopes, t);
-        to[behind] = (T)t[0];
+        errors_of<1, true>(other, slopes, t);
+        to[other] = (T)t[0];
     }
 }
 
@@ -859,7 +922,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
     Stats s;
     begin_stats(s);
     Chunk<T, NV> x;
-    for (int at = wave * SPAN; at < a.V; at += WAVES * SPAN) {
+    for (int at = wave * SPAN - lead_of(row); at < a.V; at += WAVES * SPAN) {
         load_chunk<false>(row, at, a.V, lane, x);
         fold(s, x, c);
     }
@@ -874,7 +937,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
     __syncthreads();  // the errors may take the logits' place: the given token's logit has been read
     const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
-    for (int at = wave * SPAN; at < a.V; at += WAVES * SPAN) {
+    for (int at = wave * SPAN - lead_of(row); at < a.V; at += WAVES * SPAN) {
         load_chunk<true>(row, at, a.V, lane, x);
 #pragma unroll
         for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = (x.x[i] - ref) * c - log2_s;
@@ -883,7 +946,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
 }
 
 // ----- launches ------------------------------------------------------------------------------------------------------------------
-// Logits of a wave's chunk: 32 per lane.  A row that fits into one stays in the registers of a wave or of 16 lanes.
+// A row of this many logits stays in the registers of a wave or of 16 lanes.
 constexpr int kSpan = 64 * 32;
 // Parts of a row: enough workgroups for the card where there are few rows, each with a chunk per wave at least, as many as a wave can join.
 int parts_of(long N, int V, int K) {
@@ -913,7 +976,7 @@ void lay_out(RowArgs &a, void *scratch) {
     a.part_values = a.part_stats + p * 3;
     a.part_tokens = reinterpret_cast<int *>(a.part_values + p * a.K);
     // a part is a whole number of its waves' rounds
-    a.part = ((a.V + a.parts - 1) / a.parts + 4 * kSpan - 1) / (4 * kSpan) * (4 * kSpan);
+    a.part = ((a.V + 63 + a.parts - 1) / a.parts + 4 * kSpan - 1) / (4 * kSpan) * (4 * kSpan);
 }
 
 int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
@@ -929,9 +992,11 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
             });
         } else {
-            auto kernel = a.K > 0 ? logprob_kernel<T, 32 / kWide<T>, true> : logprob_kernel<T, 32 / kWide<T>, false>;
+            constexpr int NV = 16 / kWide<T>;
+            auto kernel = a.K > 0 ? logprob_kernel<T, NV, true> : logprob_kernel<T, NV, false>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)a.N, (unsigned)a.parts), dim3(256), 0, stream, a);
-            if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<T>, dim3((unsigned)a.N), dim3(64), 0, stream, a);
+            auto joined = a.parts * a.K <= 128 ? logprob_join_kernel<T, 2> : logprob_join_kernel<T, kMostJoined / 64>;
+            if (a.parts > 1) hipLaunchKernelGGL(joined, dim3((unsigned)a.N), dim3(64), 0, stream, a);
         }
     });
     CNT_HIP(hipGetLastError());
@@ -939,7 +1004,7 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
 }
 
 int gradient(hipStream_t stream, int type, const RowArgs &a) {
-    const dim3 grid((unsigned)a.N, (unsigned)std::min(1024L, (a.V + 4L * kSpan - 1) / (4 * kSpan)));
+    const dim3 grid((unsigned)a.N, (unsigned)std::min(1024L, (a.V + 63L + 4 * kSpan - 1) / (4 * kSpan)));
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
         hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), grid, dim3(256), 0, stream, a);
@@ -1034,21 +1099,24 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
         using T = typename decltype(t)::type;
         constexpr int W = kWide<T>;
         const dim3 rows((unsigned)N);
+        // what rows may begin inside a cache line by (lead_of)
+        const bool lines = reinterpret_cast<uintptr_t>(logits) % 128 == 0 && (stride * (long)sizeof(T) % 128 == 0 || N == 1);
+        const int lead = lines ? 0 : 127 / (int)sizeof(T);
         if (V <= kSpan) {
             with_lanes(V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((N + 256 / LANES - 1) / (256 / LANES)));
                 hipLaunchKernelGGL((logprob_short_error_kernel<T, COUNT, LANES>), grid, dim3(256), 0, stream, a);
             });
-        } else if (V <= 256 * 4 * W) {
+        } else if (V <= 256 * 4 * W - lead) {
             hipLaunchKernelGGL((logprob_held_error_kernel<T, 4, 256, 4>), rows, dim3(256), 0, stream, a);
-        } else if (V <= 256 * 8 * W) {
+        } else if (V <= 256 * 8 * W - lead) {
             hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 256, 4>), rows, dim3(256), 0, stream, a);
-        } else if (V <= 512 * 8 * W) {
+        } else if (V <= 512 * 8 * W - lead) {
             hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 512, 3>), rows, dim3(512), 0, stream, a);
-        } else if (V <= 1024 * 8 * W) {
+        } else if (V <= 1024 * 8 * W - lead) {
             hipLaunchKernelGGL((logprob_held_error_kernel<T, 8, 1024, 2>), rows, dim3(1024), 0, stream, a);
-        } else if (V <= 1024 * 16 * W) {
+        } else if (V <= 1024 * 16 * W - lead) {
             hipLaunchKernelGGL((logprob_held_error_kernel<T, 16, 1024, 1>), rows, dim3(1024), 0, stream, a);
         } else {
             hipLaunchKernelGGL((logprob_long_error_kernel<T, 32 / W>), rows, dim3(1024), 0, stream, a);
