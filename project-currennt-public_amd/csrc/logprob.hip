@@ -720,22 +720,27 @@ __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse,
     if (lse != lse) s.first = lse;
     return s;
 }
-// W errors of a row from logit `at` on in the place of log2 of the probabilities; CLAMPED: some of which may be -inf
-template <int W, bool CLAMPED>
+// the given token's own error, if it is one of W from logit `at` on
+template <int W>
+__device__ __forceinline__ void add_given(int at, const Slopes &s, float (&v)[W]) {
+    if ((unsigned)(s.token - at) < (unsigned)W) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] += s.token - at == i ? s.given : 0.0f;
+    }
+}
+// W errors of a row from logit `at` on in the place of log2 of the probabilities
+template <int W>
 __device__ __forceinline__ void errors_of(int at, const Slopes &s, float (&t)[W]) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float u = CLAMPED ? at_least(t[i]) : t[i];
+        const float u = at_least(t[i]);
         t[i] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(s.second, u, s.first);
     }
-    if ((unsigned)(s.token - at) < (unsigned)W) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) t[i] += s.token - at == i ? s.given : 0.0f;
-    }
+    add_given<W>(at, s, t);
 }
 template <typename T, int W>
 __device__ __forceinline__ void put_errors(T *row, int at, int end, const Slopes &s, float (&t)[W]) {
-    errors_of<W, true>(at, s, t);
+    errors_of<W>(at, s, t);
     put_within(row, at, end, t);
 }
 template <typename T, int NV>
@@ -750,26 +755,41 @@ __device__ __forceinline__ void put_gradient(T *row, int begin, int end, int lan
     }
 }
 
-// from saved statistics: blockIdx.x the row, blockIdx.y a stretch of it
+// From saved statistics, `parts` workgroups for a row, neighbouring ones for neighbouring stretches (rows of 32000 16-bit logits dealt row by
+// row instead: 75 us for 3001).  A wave has one chunk but in very long rows.
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) {
-    constexpr int SPAN = Chunk<T, NV>::SPAN;
+    constexpr int SPAN = Chunk<T, NV>::SPAN, W = kWide<T>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = blockIdx.x;
+    const long n = blockIdx.x / (unsigned)a.parts;
+    const int stretch = blockIdx.x % (unsigned)a.parts;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
-    int at = (blockIdx.y * 4 + wave) * SPAN - lead_of(row);
-    Chunk<T, NV> x;
-    load_chunk<true>(row, at, a.V, lane, x);  // (a wave has one chunk but for very long rows: asked for in front of the row's values)
-    const float lse = a.lse[n];
-    const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
-    const float ref = lse == kMinusInfinity ? 0.0f : lse;
-    while (at < a.V) {
+    auto errors = [&](float (&t)[W], int at, float ref, const Slopes &s) {
 #pragma unroll
-        for (int i = 0; i < Chunk<T, NV>::COUNT; ++i) x.x[i] = __builtin_fmaf(x.x[i], a.scale, -ref) * kLog2e;
-        put_gradient(to, at, a.V, lane, s, x);
-        at += gridDim.y * 4 * SPAN;
-        load_chunk<true>(row, at, a.V, lane, x);
+        for (int i = 0; i < W; ++i) t[i] = __builtin_fmaf(t[i], a.scale, -ref) * kLog2e;
+        errors_of<W>(at, s, t);
+    };
+    for (int at = (stretch * 4 + wave) * SPAN - lead_of(row); at < a.V; at += a.parts * 4 * SPAN) {
+        const bool whole = at >= 0 && at + SPAN <= a.V;
+        RawChunk<T, NV> x;  // (asked for in front of the row's values)
+        if (whole) x.load(row + at, lane);
+        const float lse = a.lse[n], ref = lse == kMinusInfinity ? 0.0f : lse;
+        const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int first = at + (j * 64 + lane) * W;
+            float t[W];
+            if (whole) {
+                x.part[j].template values<0>(t);
+                errors(t, first, ref, s);
+                put_elements<T, W, true>(to + first, t);
+            } else {
+                fetch_within<true>(row, first, a.V, t, kMinusInfinity);
+                errors(t, first, ref, s);
+                put_within(to, first, a.V, t);
+            }
+        }
     }
 }
 
@@ -810,7 +830,7 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
-    const int token = a.tokens ? a.tokens[n] : -1;
+    const int token = a.tokens ? __builtin_amdgcn_readfirstlane(a.tokens[n]) : -1;
     // the row's whole vectors; what stands in front of and behind them, a logit for each of the first threads of two waves
     const int lead = lead_of(row);
     Raw<T> x[NV];
@@ -823,34 +843,39 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     int other = wave == 0 && lane < front ? lane : -1;
     if (wave == 1 && lane < (a.V - front) % W) other = front + (a.V - front) / W * W + lane;
     const float rest = other >= 0 ? (float)row[other] : kMinusInfinity;
-    // f(at, v) for the vectors that the row fills, one after another
-    auto for_vectors = [&](auto use, auto f) {
+    // The vectors one after another: quick(j, at, v) for those that all threads have, if `use_quick`, else slow(j, at, v) for those that the row
+    // fills.  Both questions are the whole wave's: in front of single instructions they took a fifth of the kernel's time.
+    auto for_vectors = [&](auto use, bool use_quick, auto quick, auto slow) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int at = (j * THREADS + (int)threadIdx.x) * W - lead;
-            if (at >= 0 && at + W <= a.V) {
-                float v[W];
+            const int first = j * THREADS * W - lead, at = first + (int)threadIdx.x * W;
+            float v[W];
+            if (use_quick && first >= 0 && first + THREADS * W <= a.V) {
                 x[j].template values<use.value>(v);
-                f(at, v);
+                quick(j, at, v);
+            } else if (at >= 0 && at + W <= a.V) {
+                x[j].template values<use.value>(v);
+                slow(j, at, v);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     float m = rest, low = 0.0f;
-    for_vectors(std::integral_constant<int, 1>(), [&](int, const float (&v)[W]) {
+    auto look = [&](int, int, const float (&v)[W]) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             m = fmaxf(m, v[i]);
             low = fminf(low, v[i]);
         }
-    });
+    };
+    for_vectors(std::integral_constant<int, 1>(), true, look, look);
     m = max_of<64>(m);
     if (lane == 0) maxima[wave] = m;
     // the errors may take the logits' place: the given token's logit is kept before any of them is written
     if (threadIdx.x == 0 && token >= 0 && token < a.V) given = (float)row[token];
     __syncthreads();
     const int w = lane % 16;  // every 16 lanes add the waves up
-    m = max_of<16>(w < WAVES ? maxima[w] : kMinusInfinity);
+    m = of_lane(max_of<16>(w < WAVES ? maxima[w] : kMinusInfinity), 0);
     m = m == m ? m : kMinusInfinity;  // (all NaN)
     const float ref = m == kMinusInfinity ? 0.0f : m, r = ref * c;
     // (see fold_fused; the whole workgroup has one maximum here)
@@ -860,20 +885,23 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     Stats s = {m, e_rest, e_rest * at_least(t_rest)};
     // Logits whose t is -inf, which have to be kept from 0 * -inf, are looked for once: most waves have none.
     const bool ruled_out = __ballot((low - ref) * c < -1e38f) != 0;
-    const std::true_type yes;
-    const std::false_type no;
-    for_vectors(std::integral_constant<int, 2>(), [&](int, const float (&v)[W]) {
-        auto add = [&](auto is_fused, auto clamped) {
+    for_vectors(std::integral_constant<int, 2>(), !ruled_out && (sizeof(T) == 4 || fused),
+        [&](int, int, const float (&v)[W]) {
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const float t = is_fused.value ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+                const float t = sizeof(T) == 2 ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
                 s.s += e;
-                s.w = __builtin_fmaf(e, clamped.value ? at_least(t) : t, s.w);
+                s.w = __builtin_fmaf(e, t, s.w);
             }
-        };
-        if (sizeof(T) == 2 && fused) ruled_out ? add(yes, yes) : add(yes, no);
-        else ruled_out ? add(no, yes) : add(no, no);
-    });
+        },
+        [&](int, int, const float (&v)[W]) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float t = fused ? __builtin_fmaf(v[i], c, -r) : (v[i] - ref) * c, e = __builtin_amdgcn_exp2f(t);
+                s.s += e;
+                s.w = __builtin_fmaf(e, at_least(t), s.w);
+            }
+        });
     s.s = sum_of<64>(s.s);
     s.w = sum_of<64>(s.w);
     if (lane == 0) {
@@ -881,8 +909,8 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         means[wave] = s.w;
     }
     __syncthreads();
-    s.s = sum_of<16>(w < WAVES ? sums[w] : 0.0f);
-    s.w = sum_of<16>(w < WAVES ? means[w] : 0.0f);
+    s.s = of_lane(sum_of<16>(w < WAVES ? sums[w] : 0.0f), 0);
+    s.w = of_lane(sum_of<16>(w < WAVES ? means[w] : 0.0f), 0);
     if (fused) {
         const float f = __builtin_amdgcn_exp2f(-off);
         s.w = (s.w - s.s * off) * f;
@@ -895,16 +923,28 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         a.entropy[n] = entropy;
     }
     const Slopes slopes = slopes_of(a, n, lse, entropy);
-    for_vectors(std::integral_constant<int, 3>(), [&](int at, float (&t)[W]) {
+    // 16-bit errors take log2 p = x * c - z from one operation: below 64 z is rounded by 2^-18, the results by 2^-9 or 2^-12
+    const float z = r + (log2_s + off);
+    const int holder = (slopes.token + lead) / (THREADS * W);
+    for_vectors(std::integral_constant<int, 3>(), !ruled_out && (sizeof(T) == 4 || (fused && fabsf(z) <= 64.0f)),
+        [&](int j, int at, float (&t)[W]) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) t[i] = (t[i] - ref) * c - log2_s;
-        if (ruled_out) errors_of<W, true>(at, slopes, t);
-        else errors_of<W, false>(at, slopes, t);
-        put_elements<T, W, true>(to + at, t);
-    });
+            for (int i = 0; i < W; ++i) {
+                t[i] = sizeof(T) == 2 ? __builtin_fmaf(t[i], c, -z) : (t[i] - ref) * c - log2_s;
+                t[i] = __builtin_amdgcn_exp2f(t[i]) * __builtin_fmaf(slopes.second, t[i], slopes.first);
+            }
+            if (j == holder) add_given<W>(at, slopes, t);
+            put_elements<T, W, true>(to + at, t);
+        },
+        [&](int, int at, float (&t)[W]) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) t[i] = (t[i] - ref) * c - log2_s;
+            errors_of<W>(at, slopes, t);
+            put_elements<T, W, true>(to + at, t);
+        });
     if (other >= 0) {
         float t[1] = {(rest - ref) * c - log2_s};
-        errors_of<1, true>(other, slopes, t);
+        errors_of<1>(other, slopes, t);
         to[other] = (T)t[0];
     }
 }
@@ -1003,11 +1043,11 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
     return CNT_OK;
 }
 
-int gradient(hipStream_t stream, int type, const RowArgs &a) {
-    const dim3 grid((unsigned)a.N, (unsigned)std::min(1024L, (a.V + 63L + 4 * kSpan - 1) / (4 * kSpan)));
+int gradient(hipStream_t stream, int type, RowArgs &a) {
+    a.parts = (int)std::min({1024L, ((1L << 24) - 1) / a.N, (a.V + 63L + 4 * kSpan - 1) / (4 * kSpan)});
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), dim3((unsigned)(a.N * a.parts)), dim3(256), 0, stream, a);
     });
     CNT_HIP(hipGetLastError());
     return CNT_OK;
