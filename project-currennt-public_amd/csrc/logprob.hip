@@ -41,6 +41,8 @@ struct RowArgs {
 template <int ROTATE>
 __device__ __forceinline__ int rotated(int v) { return __builtin_amdgcn_update_dpp(v, v, 0x120 + ROTATE, 0xf, 0xf, false); }
 template <int ROTATE>
+__device__ __forceinline__ unsigned rotated(unsigned v) { return (unsigned)rotated<ROTATE>((int)v); }
+template <int ROTATE>
 __device__ __forceinline__ float rotated(float v) { return __int_as_float(rotated<ROTATE>(__float_as_int(v))); }
 __device__ __forceinline__ float of_lane(float v, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); }
 template <int LANES, typename V, typename F>
@@ -51,8 +53,8 @@ __device__ __forceinline__ V over_lanes(V v, F f) {
     v = f(v, rotated<1>(v));
     if (LANES == 16) return v;
     auto at = [&](int lane) {
-        if constexpr (sizeof(V) == 4 && !std::is_integral<V>::value) return of_lane(v, lane);
-        else return (V)__builtin_amdgcn_readlane(v, lane);
+        if constexpr (std::is_integral<V>::value) return (V)__builtin_amdgcn_readlane((int)v, lane);
+        else return of_lane(v, lane);
     };
     return f(f(at(0), at(16)), f(at(32), at(48)));
 }
@@ -349,6 +351,13 @@ __device__ __forceinline__ void write_top(const RowArgs &a, long n, int rank, fl
     if (a.top_tokens) a.top_tokens[n * a.K + rank] = token;
 }
 
+// whole numbers in the order of floats, -0 the same as 0; no number is 0
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned u = __float_as_uint(v + 0.0f);
+    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_ordered(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
 // ----- short rows: LANES lanes hold a row, COUNT logits each ---------------------------------------------------------------------
 // The row is read once and stays in registers, so the maximum is known before the first exponential.  16 lanes per row and not a wave
 // where they can hold it: a row's steps across lanes and the rounds of its alternatives are then taken for four rows at a time.
@@ -401,22 +410,40 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
     const float log_s = logf(s.s);
     if (here && l == 0) write_stats<T>(a, n, s, log_s);
     if (!TOP) return;
-    // K rounds: the largest of what is left, the lowest token where several hold it; its place is taken by a NaN, which is never the largest
+    // K rounds: the largest of what is left, the lowest token where several hold it.  As whole numbers in the order of the logits: their maxima
+    // take one instruction per step across lanes.  What is taken, NaN and what is behind the row is 0, which no number is.
+    unsigned key[COUNT];
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i)
-        if (x.index(i, l) >= a.V) x.x[i] = __builtin_nanf("");
+    for (int i = 0; i < COUNT; ++i) key[i] = ordered(x.x[i]);
+    if (a.V < COUNT * LANES || __ballot(s.s != s.s)) {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) key[i] = x.index(i, l) < a.V && x.x[i] == x.x[i] ? key[i] : 0u;
+    }
+    unsigned kept = 0;  // result number k stays with lane k % LANES until all lanes have one
+    int kept_token = -1;
     for (int k = 0; k < a.K; ++k) {
-        const float best = x.largest();
+        unsigned best = key[0];
+#pragma unroll
+        for (int i = 1; i < COUNT; ++i) best = max(best, key[i]);
+        const unsigned most = over_lanes<LANES>(best, [](unsigned p, unsigned q) { return max(p, q); });
         int at = 0;
+        bool first[COUNT], seen = false;  // the first of the lane's that hold it
 #pragma unroll
-        for (int i = COUNT - 1; i >= 0; --i) at = x.x[i] == best ? i : at;
-        const float m = max_of<LANES>(best);
-        const int token = min_of<LANES>(best == m ? x.index(at, l) : INT_MAX);
-        if (here && l == 0) write_top(a, n, k, m, token == INT_MAX ? -1 : token, s, log_s);
-        if (k + 1 == a.K) break;
-        const int taken = best == m && x.index(at, l) == token ? at : -1;
+        for (int i = 0; i < COUNT; ++i) {
+            first[i] = key[i] == most && !seen;
+            seen = seen || first[i];
+            at = first[i] ? i : at;
+        }
+        const int own = seen ? x.index(at, l) : INT_MAX, token = min_of<LANES>(own);
+        const bool mine = k % LANES == l, last = k + 1 == a.K;
+        kept = mine ? most : kept;
+        kept_token = mine ? token : kept_token;
+        if (here && (last || k % LANES == LANES - 1) && l <= k % LANES)
+            write_top(a, n, k / LANES * LANES + l, of_ordered(kept), kept ? kept_token : -1, s, log_s);
+        if (last) break;
+        const bool owner = own == token;
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i) x.x[i] = i == taken ? __builtin_nanf("") : x.x[i];
+        for (int i = 0; i < COUNT; ++i) key[i] = owner && first[i] ? 0u : key[i];
     }
 }
 
@@ -437,11 +464,6 @@ __device__ __forceinline__ void remember(Cells &c, float largest, int at) {
     c.second = a ? c.first : b ? largest : c.second;
     c.first_at = a ? at : c.first_at;
     c.first = a ? largest : c.first;
-}
-// whole numbers in the order of floats, -0 the same as 0; no number is 0
-__device__ __forceinline__ unsigned ordered(float v) {
-    const unsigned u = __float_as_uint(v + 0.0f);
-    return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 // A bound that at least K of a wave's keys reach, and exactly K where no two are equal: keys up to COUNT per lane, `entries` in all; 0: there are
 // fewer, keys of 0 being none.  Bit by bit from the first on that not all keys have in common.
@@ -988,10 +1010,12 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
 // ----- launches ------------------------------------------------------------------------------------------------------------------
 // A row of this many logits stays in the registers of a wave or of 16 lanes.
 constexpr int kSpan = 64 * 32;
+// Logits of a long row that a workgroup takes at a time: 16 for every lane.
+constexpr int kChunk = 16, kRound = 256 * kChunk;
 // Parts of a row: enough workgroups for the card where there are few rows, each with a chunk per wave at least, as many as a wave can join.
 int parts_of(long N, int V, int K) {
     if (V <= kSpan || N == 0 || N >= 512) return 1;
-    return (int)std::min({64L, (V + 4L * kSpan - 1) / (4 * kSpan), (1023 + N) / N, K > 0 ? (long)kMostJoined / K : 64L});
+    return (int)std::min({64L, (V + kRound - 1L) / kRound, (1023 + N) / N, K > 0 ? (long)kMostJoined / K : 64L});
 }
 
 // f(COUNT, LANES) for a short row
@@ -1016,7 +1040,7 @@ void lay_out(RowArgs &a, void *scratch) {
     a.part_values = a.part_stats + p * 3;
     a.part_tokens = reinterpret_cast<int *>(a.part_values + p * a.K);
     // a part is a whole number of its waves' rounds
-    a.part = ((a.V + 63 + a.parts - 1) / a.parts + 4 * kSpan - 1) / (4 * kSpan) * (4 * kSpan);
+    a.part = ((a.V + 63 + a.parts - 1) / a.parts + kRound - 1) / kRound * kRound;
 }
 
 int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
@@ -1032,10 +1056,10 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
                 hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
             });
         } else {
-            constexpr int NV = 16 / kWide<T>;
+            constexpr int NV = kChunk / kWide<T>;
             auto kernel = a.K > 0 ? logprob_kernel<T, NV, true> : logprob_kernel<T, NV, false>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)a.N, (unsigned)a.parts), dim3(256), 0, stream, a);
-            auto joined = a.parts * a.K <= 128 ? logprob_join_kernel<T, 2> : logprob_join_kernel<T, kMostJoined / 64>;
+            auto joined = a.parts * a.K <= 256 ? logprob_join_kernel<T, 4> : logprob_join_kernel<T, kMostJoined / 64>;
             if (a.parts > 1) hipLaunchKernelGGL(joined, dim3((unsigned)a.N), dim3(64), 0, stream, a);
         }
     });
