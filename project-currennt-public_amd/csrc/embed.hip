@@ -63,6 +63,8 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
 constexpr int kMostBits = 10, kMostBins = 1 << kMostBits, kMostSortBlocks = 512, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
 // Up to here every workgroup counts the whole list's digits for itself, which takes less than a launch of its own for the counts.
 constexpr long kCountedTwice = 32768;
+constexpr int kFillVectors = 4;
+constexpr size_t kFillFrom = 16 << 20, kFillBytes = 48 << 20;  // tables that are filled on the way, bytes per launch
 
 // Scratch of a gradient: two lists of (token, slot), counts of every block and digit, the number of slots with a token, where the rows' runs
 // begin, partial sums.
@@ -100,10 +102,26 @@ SortPlan sort_plan(long V, int D, long N) {
     return p;
 }
 
+// Zeros for a stretch of the table's gradient, from workgroups behind those of a launch that leaves most of the card idle.
+struct Fill {
+    char *to;
+    long vectors;  // of 16 bytes
+};
+template <int THREADS>
+__device__ __forceinline__ void fill_zeros(const Fill &f, int block) {
+    typedef unsigned four __attribute__((ext_vector_type(4), aligned(2)));
+    const long first = (long)block * (THREADS * kFillVectors) + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < kFillVectors; ++u)
+        if (first + u * THREADS < f.vectors) __builtin_nontemporal_store(four{0u, 0u, 0u, 0u}, reinterpret_cast<four *>(f.to) + first + u * THREADS);
+}
+unsigned fill_blocks(const Fill &f, int threads) { return (unsigned)((f.vectors + threads * kFillVectors - 1) / (threads * kFillVectors)); }
+
 struct SortArgs {
     const int *keys, *slots;  // the list before the pass; first pass: keys are the tokens, slots NULL
     int *keys_out, *slots_out, *counts, *total;
-    int N, V, shift, bits, block;
+    int N, V, shift, bits, block, blocks;
+    Fill fill;
 };
 
 // First pass: a slot without a token has no place in the list.  Later ones: `total` entries are in it.
@@ -162,6 +180,10 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
     __shared__ int next[kSortWaves][kMostBins];  // counts of a wave's entries, then the next place for every wave and digit
     __shared__ int earlier[kMostBins], others[kMostBins];
     __shared__ int wave_totals[kSortWaves];
+    if ((int)blockIdx.x >= a.blocks) {
+        fill_zeros<kSortThreads>(a.fill, blockIdx.x - a.blocks);
+        return;
+    }
     const int n_bins = 1 << a.bits, n = entries<FIRST>(a), d = threadIdx.x, lane = d & 63, wave = d >> 6;
     if (d < n_bins) {
 #pragma unroll
@@ -177,7 +199,7 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
     if (COUNTED) {
         if (d < n_bins) {
 #pragma unroll 8
-            for (int b = 0; b < (int)gridDim.x; ++b) {
+            for (int b = 0; b < a.blocks; ++b) {
                 const int c = a.counts[b * n_bins + d];
                 all += c;
                 before += b < (int)blockIdx.x ? c : 0;
@@ -242,6 +264,8 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
 }
 
 // ----- sums of the runs -------------------------------------------------------------------------------------------------------
+constexpr int kWindow = 16, kZeroRows = 4;
+
 struct SumArgs {
     const int *keys, *slots, *total;
     const void *err;
@@ -251,20 +275,27 @@ struct SumArgs {
     long err_stride, grad_stride;
     int V, D, lanes, piece, accumulate;
     int tiles;         // of `lanes` threads' columns in a row; neighbouring workgroups have neighbouring ones
-    int first_blocks;  // workgroups of the first kind of a launch, in front of those of the second
+    int by_rows;
+    int first_blocks, run_blocks;  // workgroups of a launch's first and second kind, in front of those of the third
+    int pieces;
+    int filled;  // rows, the first ones, that hold zeros already
+    Fill fill;
     float scale;
 };
 
-// Sum of entries first, first + step, ... < end of the sorted list, W columns from `column` on, by the `lanes` threads of a group: every thread
-// has one of the next slots, which go round the group, so that a slot is waited for once in `lanes` entries.
+// Sum of every step-th of the entries begin .. end and begin2 .. end2 of the sorted list, from number `first` on, W columns from `column` on, by the
+// `lanes` threads of a group: every thread has one of the next slots, which go round the group, so that a slot is waited for once in
+// `lanes` entries.
 template <typename E, int W>
-__device__ __forceinline__ void add_entries(const SumArgs &a, int first, int end, int step, int column, int count, float (&sum)[W]) {
+__device__ __forceinline__ void add_entries(const SumArgs &a, int begin, int end, int begin2, int end2, int first, int step, int column, int count,
+                                            float (&sum)[W]) {
     constexpr int U = 8;  // rows in flight
     const E *err = static_cast<const E *>(a.err) + column;
-    const int x = threadIdx.x % a.lanes;
-    for (int i = first; i < end; i += a.lanes * step) {
-        const int mine = i + x * step < end ? a.slots[i + x * step] : 0;
-        const int rows = min(a.lanes, (end - i + step - 1) / step);
+    const int x = threadIdx.x % a.lanes, n1 = end - begin, n = n1 + end2 - begin2;
+    for (int i = first; i < n; i += a.lanes * step) {
+        const int e = i + x * step;
+        const int mine = e < n ? a.slots[e < n1 ? begin + e : begin2 + e - n1] : 0;
+        const int rows = min(a.lanes, (n - i + step - 1) / step);
         for (int k = 0; k < rows; k += U) {
             float v[U][W];
 #pragma unroll
@@ -317,7 +348,7 @@ __device__ __forceinline__ void find_starts(const SumArgs &a) {
     }
 }
 
-// First workgroups: where the runs begin.  The others: sums of the pieces of the sorted list that lie within one run.
+// First workgroups: where the runs begin.  Then sums of the pieces of the sorted list that lie within one run.  Then zeros.
 // blockIdx.y: the columns.
 template <typename E, int W>
 __global__ __launch_bounds__(256) void embed_pieces_kernel(const SumArgs a) {
@@ -325,30 +356,82 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const SumArgs a) {
         if (blockIdx.y == 0) find_starts(a);
         return;
     }
+    if ((int)blockIdx.x >= a.first_blocks + a.pieces) {
+        if (blockIdx.y == 0) fill_zeros<256>(a.fill, blockIdx.x - a.first_blocks - a.pieces);
+        return;
+    }
     const int piece = blockIdx.x - a.first_blocks, begin = piece * a.piece, end = begin + a.piece;
     if (end > *a.total || a.keys[begin] != a.keys[end - 1]) return;
     const int x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
     const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
     float sum[W] = {};
-    add_entries<E, W>(a, begin + g, end, 256 / a.lanes, column, count, sum);
+    add_entries<E, W>(a, begin, end, 0, 0, g, 256 / a.lanes, column, count, sum);
     join_groups<W>(a.lanes, sum);
     if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)piece * a.D + column, count, sum);
 }
 
 template <typename G, int W>
-__device__ __forceinline__ void write_row(const SumArgs &a, int row, bool any, int column, int count, float (&sum)[W]) {
-    if (count <= 0 || (a.accumulate && !any)) return;
+__device__ __forceinline__ void write_row(const SumArgs &a, int row, int column, int count, const float (&total)[W]) {
+    if (count <= 0) return;
     G *to = static_cast<G *>(a.grad) + row * a.grad_stride + column;
-    float old[W];
+    float old[W], sum[W];
     if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
 #pragma unroll
-    for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + sum[q] * a.scale : sum[q] * a.scale;
+    for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + total[q] * a.scale : total[q] * a.scale;
     put_some<G, W, true>(to, count, sum);
 }
 
+// The rows of the runs that begin at entries from .. from + kWindow of the sorted list and hold no first entry of a piece, by a group of threads:
+// it goes through the list, eight rows of errors in flight, and writes a row where its run ends.
+template <typename E, typename G, int W>
+__device__ __forceinline__ void sum_short_runs(const SumArgs &a, int from, int column, int count) {
+    constexpr int U = 8;
+    const int n = *a.total, x = threadIdx.x % a.lanes;
+    if (from >= n) return;
+    // from `stop` on, runs are others'; so is the run that holds the entry in front, or the first one of a piece
+    const int stop = min(n, (from / a.piece + 1) * a.piece), behind = min(from + kWindow, stop);
+    const int skipped = a.keys[from % a.piece == 0 ? from : from - 1], last = a.keys[behind - 1];
+    if (last == skipped) return;
+    const E *err = static_cast<const E *>(a.err) + column;
+    int current = skipped;
+    float sum[W] = {};
+    for (int i0 = from; i0 < stop; i0 += a.lanes) {
+        const int mine = i0 + x < stop ? a.keys[i0 + x] : skipped, my_slot = i0 + x < stop ? a.slots[i0 + x] : 0;
+        const int here = min(a.lanes, stop - i0);
+        for (int k = 0; k < here; k += U) {
+            float v[U][W];
+            int key[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                key[u] = __shfl(mine, k + u, a.lanes);
+                const int slot = __shfl(my_slot, k + u, a.lanes);
+                const bool needed = k + u < here && key[u] != skipped && (i0 + k + u < behind || key[u] == last);
+#pragma unroll
+                for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
+                if (needed && count > 0) fetch_some<E, W>(err + slot * a.err_stride, count, v[u], 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (k + u >= here) break;
+                if (key[u] != current) {
+                    if (current != skipped) write_row<G, W>(a, current, column, count, sum);
+                    if (i0 + k + u >= behind) return;
+                    current = key[u];
+#pragma unroll
+                    for (int q = 0; q < W; ++q) sum[q] = 0.0f;
+                }
+#pragma unroll
+                for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+            }
+        }
+    }
+    if (stop == n || a.keys[stop] != current) write_row<G, W>(a, current, column, count, sum);
+}
+
 // First workgroups: rows whose run holds the first entry of a piece, by all groups of the workgroup of the first such piece; whole pieces go
-// by their sums.  The others: the other rows, a group of `lanes` threads for each, which have fewer entries than a piece.
-template <typename E, typename G, int W, int R>
+// by their sums.  Then the other runs, a group of `lanes` threads for those that begin in kWindow entries, and zeros for the rows
+// without entries, kZeroRows for a group; or, by_rows, a row for each group in place of both.
+template <typename E, typename G, int W>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
     const int block = blockIdx.x / a.tiles, column = ((int)blockIdx.x % a.tiles * a.lanes + x) * W, count = max(0, min(W, a.D - column));
@@ -359,9 +442,8 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         const int row = a.keys[here], begin = a.starts[row], end = a.starts[row + 1];
         if (here - begin >= a.piece) return;
         const int whole = end / a.piece * a.piece;  // >= here
-        add_entries<E, W>(a, begin + g, here, groups, column, count, sum);
         if (count > 0) {
-#pragma unroll 4
+#pragma unroll 8
             for (int p = block + g; p < whole / a.piece; p += groups) {
                 float v[W];
                 fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
@@ -369,28 +451,31 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
                 for (int q = 0; q < W; ++q) sum[q] += v[q];
             }
         }
-        add_entries<E, W>(a, whole + g, end, groups, column, count, sum);
+        add_entries<E, W>(a, begin, here, whole, end, g, groups, column, count, sum);
         join_groups<W>(a.lanes, sum);
-        if (g == 0) write_row<G, W>(a, row, true, column, count, sum);
+        if (g == 0) write_row<G, W>(a, row, column, count, sum);
         return;
     }
-    // A group's rows are far apart: frequent tokens are neighbours in most vocabularies.
-    const long first = (long)(block - a.first_blocks) * groups + g, step = (long)(gridDim.x / a.tiles - a.first_blocks) * groups;
-    int begin[R], end[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const long row = min(a.V - 1L, first + r * step);
-        begin[r] = a.starts[row];
-        end[r] = a.starts[row + 1];
+    if (block < a.first_blocks + a.run_blocks) {
+        sum_short_runs<E, G, W>(a, ((block - a.first_blocks) * groups + g) * kWindow, column, count);
+        return;
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (first + r * step >= a.V) break;
-        if (end[r] > begin[r] && (end[r] - 1) / a.piece * a.piece >= begin[r]) continue;  // holds the first entry of a piece
-        float row_sum[W] = {};
-        add_entries<E, W>(a, begin[r], end[r], 1, column, count, row_sum);
-        write_row<G, W>(a, (int)(first + r * step), end[r] > begin[r], column, count, row_sum);
+    if (a.by_rows) {
+        const long row = (long)(block - a.first_blocks) * groups + g;
+        if (row >= a.V) return;
+        const int begin = a.starts[row], end = a.starts[row + 1];
+        if (end > begin ? (end - 1) / a.piece * a.piece >= begin : a.accumulate) return;  // the first workgroups', or nothing to add
+        add_entries<E, W>(a, begin, end, 0, 0, 0, 1, column, count, sum);
+        write_row<G, W>(a, (int)row, column, count, sum);
+        return;
     }
+    const long first = a.filled + ((long)(block - a.first_blocks - a.run_blocks) * groups + g) * kZeroRows;
+    int bounds[kZeroRows + 1];
+#pragma unroll
+    for (int r = 0; r <= kZeroRows; ++r) bounds[r] = a.starts[min((long)a.V, first + r)];
+#pragma unroll
+    for (int r = 0; r < kZeroRows; ++r)
+        if (first + r < a.V && bounds[r] == bounds[r + 1]) write_row<G, W>(a, (int)(first + r), column, count, sum);
 }
 
 // what a launch has workgroups for (2^24 of 256 threads)
@@ -412,18 +497,23 @@ int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
         constexpr int W = kWide<E>;
         share_columns(a, W);
         a.first_blocks = (int)(N / 256 + 1);
-        hipLaunchKernelGGL((embed_pieces_kernel<E, W>), dim3((unsigned)(a.first_blocks + pieces), (unsigned)a.tiles), dim3(256), 0, stream, a);
+        a.pieces = (int)pieces;
+        hipLaunchKernelGGL((embed_pieces_kernel<E, W>), dim3((unsigned)(a.first_blocks + pieces) + fill_blocks(a.fill, 256), (unsigned)a.tiles), dim3(256), 0,
+                           stream, a);
         CNT_HIP(hipGetLastError());
     }
     constexpr int W = kBoth<E, G>;
     share_columns(a, W);
-    // Four rows for a group of threads where most of the time goes into rows of zeros: fewer workgroups, and bounds of runs that are waited
-    // for once.
-    const bool four = (long)a.V * a.D >= 1L << 22;
-    const long each = 256 / a.lanes * (four ? 4 : 1), rows = (a.V + each - 1) / each;
+    // Few rows: a group's time is that of one run, and no rows are left to go through for their zeros (256 rows of 64, 32000 slots: 6.5 us
+    // for this launch, 10.6 by windows of the list).  Many rows: most are without entries, and the runs' groups are those of the list (65536 rows of
+    // 1024, 16384 slots: 32 us, 36 by rows).
+    a.by_rows = a.V <= N;
+    const long groups = 256 / a.lanes, windows = a.by_rows ? 0 : (N + kWindow - 1) / kWindow;
+    const long others = a.by_rows ? a.V : a.accumulate ? 0 : (a.V - a.filled + kZeroRows - 1) / kZeroRows;
     a.first_blocks = (int)starters;
-    auto kernel = four ? embed_rows_kernel<E, G, W, 4> : embed_rows_kernel<E, G, W, 1>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((starters + rows) * a.tiles)), dim3(256), 0, stream, a);
+    a.run_blocks = (int)((windows + groups - 1) / groups);
+    const long blocks = (a.first_blocks + a.run_blocks + (others + groups - 1) / groups) * a.tiles;
+    if (blocks > 0) hipLaunchKernelGGL((embed_rows_kernel<E, G, W>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
     CNT_HIP(hipGetLastError());
     return CNT_OK;
 }
@@ -479,13 +569,28 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     auto ints = [&](size_t at) { return reinterpret_cast<int *>(mem + at); };
     SortArgs s = {};
     s.counts = ints(plan.counts); s.total = ints(plan.total);
-    s.N = (int)N; s.V = V; s.bits = plan.bits; s.block = plan.block;
+    s.N = (int)N; s.V = V; s.bits = plan.bits; s.block = plan.block; s.blocks = plan.blocks;
+    // The sort and the search for runs leave most of the card idle: they bring zeros for the first rows with them, what the card writes in their
+    // time (gradient of 65536 x 1024 in fp32: 73 us without).  Sixteen rows at a time are whole vectors in every type.
+    const size_t row_bytes = (size_t)D * element_size(grad_type);
+    const bool fills = !accumulate && grad_stride == D && (size_t)V * row_bytes >= kFillFrom;
+    long filled = 0;
+    auto next_fill = [&]() {
+        Fill f = {};
+        if (!fills) return f;
+        const long rows = std::min<long>(V - filled, (long)(kFillBytes / row_bytes)) / 16 * 16;
+        f.to = static_cast<char *>(grad) + (size_t)filled * row_bytes;
+        f.vectors = rows * (long)row_bytes / 16;
+        filled += rows;
+        return f;
+    };
     for (int pass = 0; pass < plan.passes; ++pass) {
         const int to = pass & 1;
         s.keys = pass ? ints(plan.keys[1 - to]) : tokens;
         s.slots = pass ? ints(plan.slots[1 - to]) : nullptr;
         s.keys_out = ints(plan.keys[to]); s.slots_out = ints(plan.slots[to]);
         s.shift = pass * plan.bits;
+        s.fill = next_fill();
         const dim3 grid((unsigned)plan.blocks), block(kSortThreads);
         auto count = pass == 0 ? token_count_kernel<true> : token_count_kernel<false>;
         auto place = plan.counted ? (pass == 0 ? token_place_kernel<true, true> : token_place_kernel<false, true>)
@@ -494,7 +599,7 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
             hipLaunchKernelGGL(count, grid, block, 0, stream, s);
             CNT_HIP(hipGetLastError());
         }
-        hipLaunchKernelGGL(place, grid, block, 0, stream, s);
+        hipLaunchKernelGGL(place, dim3(plan.blocks + fill_blocks(s.fill, kSortThreads)), block, 0, stream, s);
         CNT_HIP(hipGetLastError());
     }
     const int last = (plan.passes - 1) & 1;
@@ -504,6 +609,8 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     a.err = err; a.grad = grad; a.partial = reinterpret_cast<float *>(mem + plan.partial);
     a.err_stride = err_stride; a.grad_stride = grad_stride;
     a.V = V; a.D = D; a.piece = plan.piece; a.accumulate = accumulate; a.scale = scale;
+    a.fill = next_fill();
+    a.filled = (int)filled;
     int status = CNT_OK;
     with_type(err_type, [&](auto e) {
         with_type(grad_type, [&](auto g) { status = sum_runs<typename decltype(e)::type, typename decltype(g)::type>(stream, a, N); });
