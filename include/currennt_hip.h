@@ -23,7 +23,8 @@ extern "C" {
 
 enum { CNT_OK = 0, CNT_ERR_ARG = 1, CNT_ERR_HIP = 2, CNT_ERR_STATE = 3, CNT_ERR_DEVICE = 4 };
 
-/* Element types of the operators over symbols (embedding, log probabilities, gradient norm); everything else is fp32. */
+/* Element types of the operators over symbols (embedding, log probabilities, gradient norm); everything else is fp32.  What these
+ * operators write overlaps no other argument, where nothing else is said. */
 enum { CNT_F32 = 0, CNT_BF16 = 1, CNT_F16 = 2 };
 
 enum { CNT_ACT_IDENTITY = 0, CNT_ACT_TANH = 1, CNT_ACT_LOGISTIC = 2, CNT_ACT_RELU = 3 };
@@ -139,7 +140,7 @@ int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, fl
 /* ---- log probabilities of symbols ----------------------------------------------------------------
  * What the softmax unit of the MDN layer (layers/MDNUnit.cu) does for classes, for vocabularies of any size and with what
  * scoring, sampling and losses ask for.  Row n of `logits` (V values of `type`, rows `stride` >= 0 elements apart) with
- * z = scale * logits, scale > 0:
+ * z = scale * logits, 1e-30 <= scale <= 1e30:
  *   lse[n]     = log sum_v exp z_v
  *   logp[n]    = z_t - lse[n], t = tokens[n]; 0 where tokens[n] is outside 0 .. V-1 (a slot without a symbol)
  *   entropy[n] = - sum_v p_v log p_v, p = exp(z - lse)
@@ -156,7 +157,7 @@ int cnt_logprob_forward(void *stream, long N, int V, int type, const void *logit
 /* Errors of the logits from the errors of logp and entropy (either may be NULL: zeros):
  *   err[v] = scale * (logp_err[n] * ([v = t] - p_v) - entropy_err[n] * p_v * (log p_v + entropy[n]))
  * with the lse and entropy of the forward call, in the logits' type (rows err_stride apart).  err may be the logits themselves, with the
- * same stride.  Rows where everything is ruled out get zeros, slots without a symbol the entropy's part alone. */
+ * same stride, and overlaps them in no other way (CNT_ERR_ARG).  Rows where everything is ruled out get zeros, slots without a symbol the entropy's part alone. */
 int cnt_logprob_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
                          const float *lse, const float *entropy, const float *logp_err, const float *entropy_err, void *err,
                          long err_stride);

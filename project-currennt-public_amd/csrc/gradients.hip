@@ -184,6 +184,27 @@ int cnt_gradients_create(int count, const void *const *gradients, void *const *c
             for (long at = 0; at < sizes[i]; at += n, n = step)
                 pieces.push_back({in + at * (long)size, to + at * (long)size, (int)std::min(n, sizes[i] - at), types[i]});
         }
+        // What is written may be its own tensor's gradient and nothing else of the list: another order of the waves would give other results.
+        struct Span {
+            uintptr_t begin, end;
+            int tensor, writes;
+        };
+        std::vector<Span> spans;
+        for (int i = 0; i < count; ++i) {
+            const uintptr_t bytes = (uintptr_t)sizes[i] * element_size(types[i]), in = reinterpret_cast<uintptr_t>(gradients[i]);
+            const uintptr_t to = clipped ? reinterpret_cast<uintptr_t>(clipped[i]) : in;
+            if (bytes == 0) continue;
+            spans.push_back({to, to + bytes, i, 1});
+            if (to != in) spans.push_back({in, in + bytes, i, 0});
+        }
+        std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+        const Span *written = nullptr, *any = nullptr;  // those that reach furthest so far
+        for (const Span &s : spans) {
+            const Span *other = s.writes ? any : written;
+            CNT_REQUIRE(!other || other->end <= s.begin, "gradients_create: tensors %d and %d overlap where one is written", other->tensor, s.tensor);
+            if (s.writes && (!written || written->end < s.end)) written = &s;
+            if (!any || any->end < s.end) any = &s;
+        }
         cnt_gradients *set = new cnt_gradients;
         set->count = (int)pieces.size();
         set->blocks = std::max(1, std::min((set->count + 3) / 4, kMostBlocks));

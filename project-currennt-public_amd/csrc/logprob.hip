@@ -1083,7 +1083,17 @@ int check_rows(const char *who, long N, int V, int type, const void *logits, lon
     CNT_REQUIRE(known_type(type), "%s: unknown element type %d", who, type);
     CNT_REQUIRE(stride >= 0, "%s: negative stride", who);
     CNT_REQUIRE(N == 0 || logits, "%s: null argument", who);
-    CNT_REQUIRE(scale > 0 && std::isfinite(scale), "%s: the scale has to be positive and finite", who);
+    CNT_REQUIRE(scale >= 1e-30f && scale <= 1e30f, "%s: the scale has to be within 1e-30 .. 1e30", who);
+    return CNT_OK;
+}
+// the errors' rows, which may be the logits' own places and overlap them in no other way
+int check_errors(const char *who, long N, int V, int type, const void *logits, long stride, const void *err, long err_stride) {
+    CNT_REQUIRE(err_stride >= V, "%s: rows of the errors overlap", who);
+    if (N == 0) return CNT_OK;
+    const uintptr_t size = element_size(type), from = reinterpret_cast<uintptr_t>(logits), to = reinterpret_cast<uintptr_t>(err);
+    const uintptr_t from_end = from + ((N - 1) * stride + V) * size, to_end = to + ((N - 1) * err_stride + V) * size;
+    CNT_REQUIRE(from_end <= to || to_end <= from || (from == to && (stride == err_stride || N == 1)),
+                "%s: the errors overlap the logits without being in their places", who);
     return CNT_OK;
 }
 int check_scratch(const char *who, long N, int V, int K, const void *scratch, size_t bytes) {
@@ -1126,8 +1136,8 @@ int cnt_logprob_backward(void *stream_, long N, int V, int type, const void *log
                          long err_stride) {
     using namespace cnt;
     CNT_TRY(check_rows("logprob_backward", N, V, type, logits, stride, scale));
-    CNT_REQUIRE(err_stride >= V, "logprob_backward: rows of the errors overlap");
     CNT_REQUIRE(N == 0 || (lse && err), "logprob_backward: null argument");
+    CNT_TRY(check_errors("logprob_backward", N, V, type, logits, stride, err, err_stride));
     CNT_REQUIRE(!entropy_err || entropy || N == 0, "logprob_backward: errors of entropies without the entropies");
     CNT_REQUIRE(!logp_err || tokens || N == 0, "logprob_backward: errors of log probabilities of which tokens?");
     if (N == 0) return CNT_OK;
@@ -1144,8 +1154,8 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
                                long err_stride, void *scratch, size_t scratch_bytes) {
     using namespace cnt;
     CNT_TRY(check_rows("logprob_error_backward", N, V, type, logits, stride, scale));
-    CNT_REQUIRE(err_stride >= V, "logprob_error_backward: rows of the errors overlap");
     CNT_REQUIRE(N == 0 || (err && lse && entropy), "logprob_error_backward: null argument");
+    CNT_TRY(check_errors("logprob_error_backward", N, V, type, logits, stride, err, err_stride));
     CNT_REQUIRE((!logp_err && !logp) || tokens || N == 0, "logprob_error_backward: log probabilities of which tokens?");
     CNT_TRY(check_scratch("logprob_error_backward", N, V, 0, scratch, scratch_bytes));
     if (N == 0) return CNT_OK;

@@ -87,6 +87,14 @@ def test_gradient_sizes(V, D, N):
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.float32, torch.float32, rng)
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("grad", S.TYPES)
+@pytest.mark.parametrize("V,D,N", [(70001, 64, 5000), (90007, 257, 3000), (131072, 301, 40000)])
+def test_gradient_of_tables_that_are_filled_on_the_way(V, D, N, grad, accumulate):
+    rng = np.random.default_rng(V)
+    _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.bfloat16, grad, rng, accumulate)
+
+
 @pytest.mark.parametrize("kind", ["none", "one", "last", "ascending", "descending", "outside"])
 def test_gradient_orders_of_tokens(kind):
     rng = np.random.default_rng(3)
@@ -111,6 +119,26 @@ def test_gradient_rows_anywhere_and_broadcast_errors():
             want, size, count = S.embed_grad(t, S.f64(e), V, 1.0)
             S.assert_close(S.f64(place[:, 1:66]), want, S.U * (count[:, None] + 1.0) * size)
             assert torch.all(place[:, :1] == 3.0) and torch.all(place[:, 66:] == 3.0) and torch.all(scratch[-512:] == 0xAB)
+
+
+def test_more_than_two_to_the_31_values():
+    # rows whose addresses are beyond 32 bits
+    capi = PC.pkg().capi
+    V, D = 66000, 32800
+    w = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    t = torch.tensor([V - 1, 0, -1, V - 2, V - 1], dtype=torch.int32, device="cuda")
+    rows = torch.randn(5, D, device="cuda").bfloat16()
+    w[V - 1], w[0] = rows[0], rows[1]
+    out = torch.empty(5, D, device="cuda")
+    capi.embed_forward(w, t, out, scale=2.0)
+    zero = torch.zeros_like(rows[0])
+    assert torch.equal(out, 2 * torch.stack([rows[0], rows[1], zero, zero, rows[0]]).float())
+    w.fill_(7.0)
+    capi.embed_backward(t, rows, w)
+    assert torch.equal(w[V - 1], (rows[0].float() + rows[4].float()).bfloat16()) and torch.equal(w[V - 2], rows[3]) and torch.equal(w[0], rows[1])
+    w[V - 2:] = 0
+    w[0] = 0
+    assert not w.any()
 
 
 def test_gradient_against_differences():

@@ -77,6 +77,30 @@ def test_no_tensors_zeros_and_the_limits_of_values():
     S.assert_close(S.f64(result), [2.0 ** -120 * np.sqrt(1000.0), 1.0], 0.0)
 
 
+def test_read_twice_and_side_by_side():
+    # the same tensor may be read twice, and tensors may touch
+    capi = PC.pkg().capi
+    g, result = torch.randn(300, device="cuda"), torch.zeros(2, device="cuda")
+    capi.opt_grad_norm(capi.GradientSet([g, g], [torch.empty_like(g), torch.empty_like(g)]), 1.0, result)
+    assert result[0].item() == pytest.approx(_norm([g, g]), rel=1e-6)
+    before = g.clone()
+    capi.opt_clip(capi.GradientSet([g[:100], g[100:137], g[137:]]), 0.5, result)
+    assert torch.equal(g, before * result[1])
+
+
+def test_more_than_two_to_the_31_elements():
+    capi = PC.pkg().capi
+    n = 2 ** 31 + 4099
+    g, result = torch.full((n,), 2.0 ** -10, device="cuda", dtype=torch.bfloat16), torch.zeros(2, device="cuda")
+    g[-1] = 3.0
+    capi.opt_clip(capi.GradientSet([g]), 1.0, result)
+    norm = np.sqrt((n - 1) * 2.0 ** -20 + 9.0)
+    S.assert_close(S.f64(result), [norm, 1 / norm], 1e-9 * norm)
+    f = result[1].item()
+    S.assert_close(S.f64(g[-3:]), [2.0 ** -10 * f, 2.0 ** -10 * f, 3 * f], S.U * 3, torch.bfloat16)
+    assert g[0] == g[n - 2] == g[2 ** 31] == g[2 ** 31 - 1]
+
+
 @pytest.mark.parametrize("bad", [float("inf"), float("nan"), -float("inf")])
 def test_a_norm_that_is_no_number_leaves_zeros(bad):
     capi = PC.pkg().capi

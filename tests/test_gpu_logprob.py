@@ -68,7 +68,8 @@ def test_forward(N, V, K, dtype):
 
 @pytest.mark.parametrize("dtype", S.TYPES)
 @pytest.mark.parametrize("V", [70, 900, 5000, 40000])
-def test_rows_that_masks_leave_little_of(V, dtype):
+@pytest.mark.parametrize("times", [1, 50])
+def test_rows_that_masks_leave_little_of(times, V, dtype):
     rng = np.random.default_rng(V)
     x = _logits(rng, 12, V, dtype)
     low, inf = torch.finfo(dtype).min, float("inf")
@@ -88,9 +89,18 @@ def test_rows_that_masks_leave_little_of(V, dtype):
     x[10] = torch.finfo(dtype).max
     x[11, :] = float("nan")
     t = np.array([3, 3, V - 1, 5, 0, 0, 3, 3, 5, 7, 9, 1], np.int32)
-    _check_forward(PC.pkg().capi, x, t, 6)
+    capi = PC.pkg().capi
+    got, _ = _check_forward(capi, x, t, 6)
+    if times > 1:  # among so many that a row is one workgroup's: sums in another order, so values against 64 bits again, tokens the same
+        many = _forward(capi, x.repeat(times, 1), _dev(np.tile(t, times)), 6)
+        R = S.Rows(S.f64(x), 1.0)
+        for k in (0, 1, times - 1):
+            part = {n: v[12 * k:12 * k + 12] for n, v in many.items()}
+            assert torch.equal(part["top_tokens"], got["top_tokens"])
+            S.assert_close(S.f64(part["lse"]), R.lse, R.tol_lse)
+            S.assert_close(S.f64(part["entropy"]), R.entropy, R.tol_entropy)
     t[:] = 2
-    _check_forward(PC.pkg().capi, x, t, 1)
+    _check_forward(capi, x, t, 1)
 
 
 @pytest.mark.parametrize("V", [200, 3000, 30000, 70001])
@@ -163,8 +173,34 @@ def test_gradient(N, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", S.TYPES)
+@pytest.mark.parametrize("V", [4090, 8150, 16350, 30001, 60001, 65540, 100003, 131072, 140001])
+def test_gradient_of_many_long_rows(V, dtype):
+    # every form that a row of its own workgroup takes; some of the rows are checked
+    capi = PC.pkg().capi
+    N, rng, some = 513, np.random.default_rng(V), [0, 1, 2, 255, 511, 512]
+    x = torch.randn(N, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V)).mul_(2.5).to(dtype)
+    g, h = rng.standard_normal(N).astype(np.float32), (0.3 * rng.standard_normal(N)).astype(np.float32)
+    t = _tokens(rng, N, V)
+    t[some] = [0, V - 1, -1, 5, V // 2, V - 3]
+    f, err = [torch.empty(N, device="cuda") for _ in range(3)], torch.empty_like(x)
+    capi.logprob_error_backward(x, _dev(t), _dev(g), _dev(h), *f, err, scale=0.75)
+    R = S.Rows(S.f64(x[some]), 0.75)
+    want, tol = R.gradient(t[some], g[some].astype(np.float64), h[some].astype(np.float64), False)
+    S.assert_close(S.f64(err[some]), want, tol, dtype)
+    S.assert_close(S.f64(f[1][some]), R.lse, R.tol_lse)
+    S.assert_close(S.f64(f[2][some]), R.entropy, R.tol_entropy)
+    held = t[some] >= 0
+    at, rows = np.maximum(t[some], 0), np.arange(len(some))
+    S.assert_close(S.f64(f[0][some]), np.where(held, R.logp[rows, at], 0.0), np.where(held, R.tol_logp[rows, at], 0.0))
+    again, logp = x, torch.empty(N, device="cuda")
+    capi.logprob_error_backward(again, _dev(t), _dev(g), _dev(h), logp, f[1], f[2], again, scale=0.75)
+    assert torch.equal(again, err) and torch.equal(logp, f[0])
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
 @pytest.mark.parametrize("V", [70, 900, 5000, 40000])
-def test_gradient_of_masked_rows(V, dtype):
+@pytest.mark.parametrize("times", [1, 80])
+def test_gradient_of_masked_rows(times, V, dtype):
     rng = np.random.default_rng(V)
     x = _logits(rng, 7, V, dtype)
     x[0] = -float("inf")
@@ -175,7 +211,20 @@ def test_gradient_of_masked_rows(V, dtype):
     x[4, 5] = float("nan")
     x[5, 6] = float("inf")
     t = np.array([2, 2, 1, 0, 3, 3, -1], np.int32)
-    _check_gradients(PC.pkg().capi, x, t, 1.0, np.ones(7, np.float32), np.full(7, 0.5, np.float32))
+    if times == 1:
+        _check_gradients(PC.pkg().capi, x, t, 1.0, np.ones(7, np.float32), np.full(7, 0.5, np.float32))
+        return
+    # the same rows among so many that a row is one workgroup's
+    N, capi = 7 * times, PC.pkg().capi
+    many, g, h = x.repeat(times, 1), np.ones(7), np.full(7, 0.5)
+    f, err = [torch.empty(N, device="cuda") for _ in range(3)], torch.empty_like(many)
+    capi.logprob_error_backward(many, _dev(np.tile(t, times)), torch.ones(N, device="cuda"), torch.full((N,), 0.5, device="cuda"), *f, err)
+    R = S.Rows(S.f64(x), 1.0)
+    want, tol = R.gradient(t, g, h, False)
+    for k in (0, 1, times - 1):
+        S.assert_close(S.f64(err[7 * k:7 * k + 7]), want, tol, dtype)
+        S.assert_close(S.f64(f[1][7 * k:7 * k + 7]), R.lse, R.tol_lse)
+        S.assert_close(S.f64(f[2][7 * k:7 * k + 7]), R.entropy, R.tol_entropy)
 
 
 def test_gradient_of_a_row_of_the_types_lowest_value():

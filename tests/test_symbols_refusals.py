@@ -6,7 +6,7 @@ import torch
 
 from __graft_entry__ import load_package
 
-P = C.c_void_p(4096)  # some address: no refused call may touch it
+P, Q = C.c_void_p(4096), C.c_void_p(1 << 40)  # some addresses: no refused call may touch them
 
 
 def _refused(status, what):
@@ -57,6 +57,7 @@ def test_log_probabilities():
     for changes, what in (({"N": -1}, "sizes"), ({"V": 0}, "sizes"), ({"V": 2 ** 31 - 1}, "sizes"), ({"N": 1 << 24}, "sizes"),
                           ({"type": 3}, "element type"), ({"stride": -1}, "stride"), ({"logits": None}, "null"), ({"scale": 0.0}, "scale"),
                           ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"),
+                          ({"scale": 2e30}, "scale"), ({"scale": 0.5e-30}, "scale"),
                           ({"K": -1}, "alternatives"), ({"K": 65, "V": 100}, "alternatives"), ({"K": 11}, "alternatives"),
                           ({"top": None, "ids": None}, "alternatives"), ({"tokens": None}, "which tokens"),
                           ({"V": 100000, "stride": 100000}, "scratch")):
@@ -64,22 +65,25 @@ def test_log_probabilities():
     assert forward(N=0) == 0 and forward(N=0, V=100000, stride=100000) == 0
 
     def backward(**changes):
-        a = dict(stream=None, N=4, V=10, type=0, logits=P, stride=10, scale=1.0, tokens=P, lse=P, entropy=P, g=P, h=P, err=P, es=10)
+        a = dict(stream=None, N=4, V=10, type=0, logits=P, stride=10, scale=1.0, tokens=P, lse=P, entropy=P, g=P, h=P, err=Q, es=10)
         a.update(changes)
         return L.cnt_logprob_backward(*a.values())
 
     for changes, what in (({"V": 0}, "sizes"), ({"type": 9}, "element type"), ({"es": 9}, "overlap"), ({"lse": None}, "null"),
-                          ({"err": None}, "null"), ({"entropy": None}, "entropies"), ({"tokens": None}, "which tokens"), ({"scale": 0.0}, "scale")):
+                          ({"err": None}, "null"), ({"entropy": None}, "entropies"), ({"tokens": None}, "which tokens"), ({"scale": 0.0}, "scale"),
+                          ({"err": P, "es": 11}, "in their places"), ({"err": C.c_void_p(4096 + 159)}, "in their places"),
+                          ({"err": C.c_void_p(4096 - 156)}, "in their places"), ({"err": P, "stride": 0}, "in their places")):
         _refused(backward(**changes), what)
     assert backward(N=0) == 0
 
     def both(**changes):
-        a = dict(stream=None, N=4, V=10, type=0, logits=P, stride=10, scale=1.0, tokens=P, g=P, h=P, logp=P, lse=P, entropy=P, err=P, es=10,
+        a = dict(stream=None, N=4, V=10, type=0, logits=P, stride=10, scale=1.0, tokens=P, g=P, h=P, logp=P, lse=P, entropy=P, err=Q, es=10,
                  scratch=None, bytes=0)
         a.update(changes)
         return L.cnt_logprob_error_backward(*a.values())
 
     for changes, what in (({"V": 0}, "sizes"), ({"es": 9}, "overlap"), ({"lse": None}, "null"), ({"entropy": None}, "null"),
+                          ({"err": P, "es": 12}, "in their places"), ({"err": C.c_void_p(4100)}, "in their places"),
                           ({"tokens": None}, "which tokens"), ({"V": 100000, "stride": 100000, "es": 100000}, "scratch")):
         _refused(both(**changes), what)
     assert both(N=0, V=100000, stride=100000, es=100000) == 0 and L.cnt_logprob_scratch(0, 100000, 3) == 0
@@ -99,6 +103,11 @@ def test_gradients():
     _refused(L.cnt_gradients_create(1, ptrs, (C.c_void_p * 1)(None), sizes, types, C.byref(h)), "null pointer")
     _refused(L.cnt_gradients_create(1, (C.c_void_p * 1)(4098), None, sizes, types, C.byref(h)), "aligned")
     _refused(L.cnt_gradients_create(1, ptrs, None, (C.c_long * 1)(2 ** 62), types, C.byref(h)), "too many")
+    # a tensor twice, or a stretch of another, where it is written
+    two, sizes2, types2 = (C.c_void_p * 2), (C.c_long * 2)(5, 5), (C.c_int * 2)(0, 0)
+    for grads, clipped in (((4096, 4096), None), ((4096, 4112), None), ((4096, 8192), (16384, 16384)), ((4096, 8192), (16384, 4096)),
+                           ((4096, 8192), (4100, 16384)), ((4096, 8192), (16384, 8188))):
+        _refused(L.cnt_gradients_create(2, two(*grads), two(*clipped) if clipped else None, sizes2, types2, C.byref(h)), "overlap")
     assert not h
     assert L.cnt_gradients_destroy(None) == 0
     _refused(L.cnt_opt_grad_norm(None, None, 1.0, P), "null")
