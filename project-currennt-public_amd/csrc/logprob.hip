@@ -447,7 +447,7 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
     }
 }
 
-// ----- long rows: a workgroup of four waves for a row or a part of one ------------------------------------------------------------
+// ----- long rows: a workgroup of one or four waves for a row or a part of one ------------------------------------------------------------
 // The best K without keeping them up to date on the way, which at K = 16 took longer than everything else (2047 rows of 100003: 200 us, of
 // which a list per wave 130): a lane remembers the largest logit of its best two chunks, and of which chunks, and that of its third.  The
 // K-th largest of the lanes' largest is a bound that K logits reach.  Read again are the remembered chunks that reach it, their lane's logits
@@ -493,17 +493,19 @@ __device__ __forceinline__ unsigned bound_of(const unsigned (&key)[COUNT], int e
     return t;
 }
 
-constexpr int kMostCells = 256, kMostWhole = 16, kMostCandidates = 512;
+constexpr int kMostWhole = 16;
+template <int WAVES>
 struct Shared {
-    Stats stats[4];
-    float first[256], second[256], third[256];
-    int first_at[256], second_at[256];
-    int cell_lane[kMostCells], cell_at[kMostCells];
+    static constexpr int THREADS = 64 * WAVES, CELLS = WAVES == 1 ? 128 : THREADS, CANDIDATES = WAVES == 1 ? 256 : 512;
+    Stats stats[WAVES];
+    float first[THREADS], second[THREADS], third[THREADS];
+    int first_at[THREADS], second_at[THREADS];
+    int cell_lane[CELLS], cell_at[CELLS];
     int whole[kMostWhole];  // lanes (with their waves) all of whose chunks are read again
     unsigned least;
     int cells, wholes, candidates;
-    float value[kMostCandidates];
-    int token[kMostCandidates];
+    float value[CANDIDATES];
+    int token[CANDIDATES];
 };
 
 // entry i of a list, at its rank if that is among the first K: f(rank)
@@ -517,11 +519,12 @@ __device__ __forceinline__ void rank_entry(const float *value, const int *token,
 }
 
 // (registers for eight workgroups of a compute unit: with seven, 2047 rows with alternatives took two rounds of the card)
-template <typename T, int NV, bool TOP>
-__global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
+template <typename T, int NV, int WAVES, bool TOP>
+__global__ __launch_bounds__(64 * WAVES, 8) void logprob_kernel(const RowArgs a) {
     using X = Chunk<T, NV>;
-    constexpr int SPAN = X::SPAN, W = X::W;
-    __shared__ Shared sh;
+    using Sh = Shared<WAVES>;
+    constexpr int SPAN = X::SPAN, W = X::W, THREADS = 64 * WAVES;
+    __shared__ Sh sh;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long n = blockIdx.x;
     const float c = a.scale * kLog2e;
@@ -543,7 +546,7 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
     int at = begin + wave * SPAN;
     if (at < 0) {
         take_part(at);
-        at += 4 * SPAN;
+        at += WAVES * SPAN;
     }
     if (at + SPAN <= end) {
         RawChunk<T, NV> next;
@@ -551,7 +554,7 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
         while (true) {
             RawChunk<T, NV> now = next;
             const int here = at;
-            at += 4 * SPAN;
+            at += WAVES * SPAN;
             if (at + SPAN <= end) next.load(row + at, lane);
             X x;
             now.values(x);
@@ -572,7 +575,7 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
     __syncthreads();
     s = sh.stats[0];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) s = join(s, sh.stats[w], c);
+    for (int w = 1; w < WAVES; ++w) s = join(s, sh.stats[w], c);
     const float log_s = logf(s.s);
     const bool shared_row = a.parts > 1;
     const long p = n * a.parts + blockIdx.y;
@@ -595,32 +598,32 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
         }
     };
     if (wave == 0) {
-        unsigned key[4];
+        unsigned key[WAVES];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) key[w] = ordered(sh.first[w * 64 + lane]);
-        const unsigned least = bound_of<4>(key, 256, a.K);
+        for (int w = 0; w < WAVES; ++w) key[w] = ordered(sh.first[w * 64 + lane]);
+        const unsigned least = bound_of<WAVES>(key, THREADS, a.K);
         int wholes = 0, count = 0;
 #pragma unroll
-        for (int q = 0; q < 12; ++q) {  // third, first, second
-            const int from = q % 4 * 64 + lane;
+        for (int q = 0; q < 3 * WAVES; ++q) {  // third, first, second
+            const int from = q % WAVES * 64 + lane;
             const bool whole = ordered(sh.third[from]) >= least;
-            const bool in = q < 4 ? whole : !whole && ordered(q < 8 ? sh.first[from] : sh.second[from]) >= least;
+            const bool in = q < WAVES ? whole : !whole && ordered(q < 2 * WAVES ? sh.first[from] : sh.second[from]) >= least;
             const unsigned long long b = __ballot(in);
-            const int place = (q < 4 ? wholes : count) + __popcll(b & ((1ull << lane) - 1));
-            if (q < 4) {
+            const int place = (q < WAVES ? wholes : count) + __popcll(b & ((1ull << lane) - 1));
+            if (q < WAVES) {
                 if (in && place < kMostWhole) sh.whole[place] = from;
                 wholes += __popcll(b);
             } else {
-                if (in && place < kMostCells) {
+                if (in && place < Sh::CELLS) {
                     sh.cell_lane[place] = lane;
-                    sh.cell_at[place] = q < 8 ? sh.first_at[from] : sh.second_at[from];
+                    sh.cell_at[place] = q < 2 * WAVES ? sh.first_at[from] : sh.second_at[from];
                 }
                 count += __popcll(b);
             }
         }
         if (lane == 0) {
             sh.least = least;
-            sh.cells = wholes <= kMostWhole && count <= kMostCells ? count : -1;
+            sh.cells = wholes <= kMostWhole && count <= Sh::CELLS ? count : -1;
             sh.wholes = wholes;
             sh.candidates = 0;
         }
@@ -638,29 +641,29 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
             for (int q = 0; q < W; ++q) {
                 if (v[q] == v[q] && ordered(v[q]) >= least) {
                     const int place = atomicAdd(&sh.candidates, 1);
-                    if (place < kMostCandidates) {
+                    if (place < Sh::CANDIDATES) {
                         sh.value[place] = v[q];
                         sh.token[place] = first + q;
                     }
                 }
             }
         };
-        for (int i = threadIdx.x; i < n_cells * NV; i += 256) look(sh.cell_at[i / NV], sh.cell_lane[i / NV], i % NV);
-        const int rounds = (end - begin + 4 * SPAN - 1) / (4 * SPAN), each = rounds * NV;
-        for (int i = threadIdx.x; i < sh.wholes * each; i += 256) {
+        for (int i = threadIdx.x; i < n_cells * NV; i += THREADS) look(sh.cell_at[i / NV], sh.cell_lane[i / NV], i % NV);
+        const int rounds = (end - begin + WAVES * SPAN - 1) / (WAVES * SPAN), each = rounds * NV;
+        for (int i = threadIdx.x; i < sh.wholes * each; i += THREADS) {
             const int from = sh.whole[i / each], of = from & 63, in = i % each;
-            look(begin + (in / NV * 4 + from / 64) * SPAN, of, in % NV);
+            look(begin + (in / NV * WAVES + from / 64) * SPAN, of, in % NV);
         }
         __syncthreads();
-        listed = sh.candidates > kMostCandidates;
+        listed = sh.candidates > Sh::CANDIDATES;
         const int candidates = sh.candidates;
-        for (int i = threadIdx.x; !listed && i < candidates; i += 256) rank_entry(sh.value, sh.token, candidates, i, a.K, put);
+        for (int i = threadIdx.x; !listed && i < candidates; i += THREADS) rank_entry(sh.value, sh.token, candidates, i, a.K, put);
     }
     if (!listed) return;
     // the row again, with a list per wave
     Best b;
     begin_best(b);
-    for (int at = begin + wave * SPAN; at < end; at += 4 * SPAN) {
+    for (int at = begin + wave * SPAN; at < end; at += WAVES * SPAN) {
         X x;
         load_chunk<false>(row, at, end, lane, x);
         take_best(b, x, at, end, a.K, lane);
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(256, 8) void logprob_kernel(const RowArgs a) {
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) merge_best(b, values[w * 64 + lane], tokens[w * 64 + lane], a.K, lane);
+    for (int w = 1; w < WAVES; ++w) merge_best(b, values[w * 64 + lane], tokens[w * 64 + lane], a.K, lane);
     if (lane < a.K) put(lane, b.value, lane < b.count ? b.token : -1);
 }
 
@@ -1008,10 +1011,27 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
 }
 
 // ----- launches ------------------------------------------------------------------------------------------------------------------
-// A row of this many logits stays in the registers of a wave or of 16 lanes.
+// A row of this many logits has room in the registers of a wave.
 constexpr int kSpan = 64 * 32;
 // Logits of a long row that a workgroup takes at a time: 16 for every lane.
 constexpr int kChunk = 16, kRound = 256 * kChunk;
+
+// Which kernel takes the rows; measured on 32000 rows of up to 1000 logits, 20000 of 1975, 16384 of 3000 and 8192 of 10000, us:
+//   a row in registers, K rounds (HELD) against a wave that streams a row (WAVE): 500 logits, K = 8 34 / 47, 16 55 / 52, 32 96 / 66;
+//   1000, K = 2 31 / 43, 8 58 / 48, 32 183 / 70; 1975, K = 1 37 / 35, 4 50 / 38, 32 217 / 57; 256, K = 16 31 / 41, 64 100 / 359
+//   four waves for a row (GROUP) against WAVE: 1975, K = 64 161 / 326 (HELD 415); 3000, K = 0 29 / 23, 16 80 / 38, 64 123 / 278; 10000,
+//   K = 16 56 / 41, 64 78 / 266; 4096 rows of 30000, K = 16 55 / 53
+// A wave bounds its alternatives by 64 lanes, four by 256: beyond 32 alternatives too many logits reach a wave's bound.
+enum Form { HELD, WAVE, GROUP };
+constexpr int kWaveTop = 32;
+Form form_of(long N, int V, int K) {
+    const bool wave = K <= kWaveTop;
+    if (V <= 256) return HELD;
+    if (V <= 512) return K > 16 && wave ? WAVE : HELD;
+    if (V <= 1024) return K >= 8 && wave ? WAVE : HELD;
+    if (V <= kSpan) return K <= 1 ? HELD : wave ? WAVE : GROUP;
+    return N >= 2048 && V <= 16384 && wave ? WAVE : GROUP;
+}
 // Parts of a row: enough workgroups for the card where there are few rows, each with a chunk per wave at least, as many as a wave can join.
 int parts_of(long N, int V, int K) {
     if (V <= kSpan || N == 0 || N >= 512) return 1;
@@ -1048,7 +1068,8 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
     lay_out(a, scratch);
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        if (a.V <= kSpan) {
+        const Form form = form_of(a.N, a.V, a.K);
+        if (form == HELD) {
             with_lanes(a.V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((a.N + 256 / LANES - 1) / (256 / LANES)));
@@ -1057,8 +1078,11 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
             });
         } else {
             constexpr int NV = kChunk / kWide<T>;
-            auto kernel = a.K > 0 ? logprob_kernel<T, NV, true> : logprob_kernel<T, NV, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)a.N, (unsigned)a.parts), dim3(256), 0, stream, a);
+            auto four = a.K > 0 ? logprob_kernel<T, NV, 4, true> : logprob_kernel<T, NV, 4, false>;
+            auto one = a.K > 0 ? logprob_kernel<T, NV, 1, true> : logprob_kernel<T, NV, 1, false>;
+            const dim3 grid((unsigned)a.N, (unsigned)a.parts);
+            if (form == WAVE) hipLaunchKernelGGL(one, grid, dim3(64), 0, stream, a);
+            else hipLaunchKernelGGL(four, grid, dim3(256), 0, stream, a);
             auto joined = a.parts * a.K <= 256 ? logprob_join_kernel<T, 4> : logprob_join_kernel<T, kMostJoined / 64>;
             if (a.parts > 1) hipLaunchKernelGGL(joined, dim3((unsigned)a.N), dim3(64), 0, stream, a);
         }

@@ -60,7 +60,9 @@ def _tokens(rng, N, V):
 @pytest.mark.parametrize("N,V,K", [
     (1, 1, 1), (1, 2, 2), (3, 63, 5), (5, 64, 64), (9, 255, 4), (6, 256, 1), (4, 257, 8), (7, 512, 3), (3, 513, 20), (2, 1024, 2),
     (3, 2047, 64), (2, 2048, 7), (2, 2049, 7), (3, 8192, 16), (1, 8193, 16), (2, 50001, 33), (1, 131072, 8), (600, 2500, 6), (513, 300, 0),
-    (511, 16400, 2), (1, 600000, 50)])
+    (511, 16400, 2), (1, 600000, 50),
+    (5, 300, 20), (9, 511, 32), (7, 512, 33), (6, 700, 9), (6, 1024, 32), (5, 1500, 3), (5, 1500, 40), (4, 2048, 32), (2100, 2600, 5), (2049, 2100, 32),
+    (2060, 2500, 33), (2048, 2049, 0)])
 def test_forward(N, V, K, dtype):
     rng = np.random.default_rng(N * 31 + V)
     _check_forward(PC.pkg().capi, _logits(rng, N, V, dtype), _tokens(rng, N, V), K, scale=0.8)
@@ -68,7 +70,7 @@ def test_forward(N, V, K, dtype):
 
 @pytest.mark.parametrize("dtype", S.TYPES)
 @pytest.mark.parametrize("V", [70, 900, 5000, 40000])
-@pytest.mark.parametrize("times", [1, 50])
+@pytest.mark.parametrize("times", [1, 50, 200])
 def test_rows_that_masks_leave_little_of(times, V, dtype):
     rng = np.random.default_rng(V)
     x = _logits(rng, 12, V, dtype)
@@ -103,15 +105,18 @@ def test_rows_that_masks_leave_little_of(times, V, dtype):
     _check_forward(capi, x, t, 1)
 
 
-@pytest.mark.parametrize("V", [200, 3000, 30000, 70001])
+@pytest.mark.parametrize("V", [200, 400, 900, 1500, 3000, 30000, 70001])
 def test_alternatives_of_sorted_and_repeated_logits(V):
     capi = PC.pkg().capi
     up = np.linspace(-5, 5, V).astype(np.float32)
     rng = np.random.default_rng(V)
     few = rng.integers(0, 4, V).astype(np.float32)
     x = _dev(np.stack([up, up[::-1], few, np.zeros(V, np.float32), np.where(np.arange(V) % 97 == 96, 3.0, -np.inf).astype(np.float32)]))
-    for K in (1, 5, 64):
-        _check_forward(capi, x, np.zeros(5, np.int32), K)
+    for K in (1, 5, 20, 64):
+        got, _ = _check_forward(capi, x, np.zeros(5, np.int32), K)
+        if V in (3000, 30000):  # and where a row is a wave's, or a workgroup's
+            many = _forward(capi, x.repeat(420, 1), _dev(np.zeros(2100, np.int32)), K)
+            assert torch.equal(many["top_tokens"], got["top_tokens"].repeat(420, 1))
 
 
 def test_rows_anywhere_and_results_that_nobody_asks_for():
