@@ -128,20 +128,20 @@ struct SortArgs {
 template <bool FIRST>
 __device__ __forceinline__ int entries(const SortArgs &a) { return FIRST ? a.N : *a.total; }
 template <bool FIRST>
-__device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIRST || (key >= 0 && key < a.V); }
+__device__ __forceinline__ bool listed(const SortArgs &a, int key) { return !FIRST || (unsigned)key < (unsigned)a.V; }
 
 // how often every digit occurs among entries begin .. end, added to bins
 template <bool FIRST>
-__device__ __forceinline__ void count_digits(const SortArgs &a, long begin, long end, int first, long step, int *bins) {
+__device__ __forceinline__ void count_digits(const SortArgs &a, int begin, int end, int first, int step, int *bins) {
     constexpr int U = 8;  // loads in flight
     // (whole waves go round, so that all lanes take part in the ballots)
-    for (long i = begin + first; i - (threadIdx.x & 63) < end; i += U * step) {
+    for (int i = begin + first; i - (int)(threadIdx.x & 63) < end; i += U * step) {
         int key[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) key[u] = i + u * step < end ? a.keys[i + u * step] : -1;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool in = key[u] >= 0 && listed<FIRST>(a, key[u]);
+            const bool in = FIRST ? (unsigned)key[u] < (unsigned)a.V : key[u] >= 0;
             const int digit = (key[u] >> a.shift) & ((1 << a.bits) - 1);
             if (FIRST) {
                 if (in) atomicAdd(&bins[digit], 1);
@@ -166,8 +166,8 @@ __global__ __launch_bounds__(kSortThreads) void token_count_kernel(const SortArg
     const int n_bins = 1 << a.bits, n = entries<FIRST>(a), d = threadIdx.x;
     bins[d] = 0;
     __syncthreads();
-    const long begin = (long)blockIdx.x * a.block;
-    count_digits<FIRST>(a, begin, min((long)n, begin + a.block), d, kSortThreads, bins);
+    const int begin = min(n, (int)blockIdx.x * a.block);
+    count_digits<FIRST>(a, begin, min(n, begin + a.block), d, kSortThreads, bins);
     __syncthreads();
     if (d < n_bins) a.counts[blockIdx.x * n_bins + d] = bins[d];
 }
@@ -191,9 +191,8 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
         earlier[d] = others[d] = 0;
     }
     __syncthreads();
-    const long block_begin = min((long)n, (long)blockIdx.x * a.block), block_end = min((long)n, block_begin + a.block);
-    const int share = a.block / kSortWaves;
-    const long begin = min((long)n, (long)blockIdx.x * a.block + (long)wave * share), end = min((long)n, begin + share);
+    const int block_begin = min(n, (int)blockIdx.x * a.block), block_end = min(n, block_begin + a.block);
+    const int share = a.block / kSortWaves, begin = min(n, block_begin + wave * share), end = min(n, begin + share);
     count_digits<FIRST>(a, begin, end, lane, 64, next[wave]);
     int before = 0, all = 0;
     if (COUNTED) {
@@ -240,8 +239,8 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
     // In steps of 64 entries, in order: lanes of one digit find each other by one ballot per bit.  Every lane reads its digit's
     // next place before the first lane of the digit moves it on (the accesses of one wave to LDS are performed in order).
     volatile int *mine = next[wave];
-    for (long i0 = begin; i0 < end; i0 += 64) {
-        const long i = i0 + lane;
+    for (int i0 = begin; i0 < end; i0 += 64) {
+        const int i = i0 + lane;
         const int key = i < end ? a.keys[i] : -1;
         const bool in = i < end && listed<FIRST>(a, key);
         const int digit = in ? (key >> a.shift) & (n_bins - 1) : 0;
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
         __builtin_amdgcn_wave_barrier();
         if (in) {
             a.keys_out[place] = key;
-            a.slots_out[place] = FIRST ? (int)i : a.slots[i];
+            a.slots_out[place] = FIRST ? i : a.slots[i];
         }
     }
 }
