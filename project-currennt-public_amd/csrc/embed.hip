@@ -262,6 +262,19 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
     }
 }
 
+// Whether rows of the gradient are written past the caches: rows of whole lines (53665 of 512 fp32 zeros 21 us, 22.5 through the caches), and
+// tables that the last-level cache has no room for (65536 rows of 1000 from 16384 slots 75 us and 97).  Other rows share lines, which are written twice
+// past the caches (53665 of 458: 27 us, 20 through them).
+inline bool past_caches(const void *grad, int V, int D, long stride, int type) {
+    const long row = stride * (long)element_size(type);
+    return (reinterpret_cast<uintptr_t>(grad) % 128 == 0 && row % 128 == 0) || V * (long)D * (long)element_size(type) > 128L << 20;
+}
+template <typename T, int W>
+__device__ __forceinline__ void put_row(T *to, int count, const float (&v)[W], bool once) {
+    if (once) put_some<T, W, true>(to, count, v);
+    else put_some<T, W, false>(to, count, v);
+}
+
 // ----- sums of the runs -------------------------------------------------------------------------------------------------------
 constexpr int kWindow = 16, kZeroRows = 4;
 
@@ -274,7 +287,7 @@ struct SumArgs {
     long err_stride, grad_stride;
     int V, D, lanes, piece, accumulate;
     int tiles;         // of `lanes` threads' columns in a row; neighbouring workgroups have neighbouring ones
-    int by_rows, searched;
+    int by_rows, searched, once;
     int first_blocks, run_blocks;  // workgroups of a launch's first and second kind, in front of those of the third
     int pieces;
     int filled;  // rows, the first ones, that hold zeros already
@@ -391,7 +404,7 @@ __device__ __forceinline__ void write_row(const SumArgs &a, int row, int column,
     if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
 #pragma unroll
     for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + total[q] * a.scale : total[q] * a.scale;
-    put_some<G, W, true>(to, count, sum);
+    put_row(to, count, sum, a.once);
 }
 
 // The rows of the runs that begin at entries from .. from + kWindow of the sorted list and hold no first entry of a piece, by a group of threads:
@@ -501,19 +514,20 @@ struct FewArgs {
     const void *err;
     void *grad;
     long err_stride, grad_stride;
-    int N, V, D, lanes, tiles, accumulate;
+    int N, V, D, lanes, tiles, accumulate, once;
     float scale;
 };
 
 template <typename E, typename G, int W, int R>
 __global__ __launch_bounds__(256) void embed_few_kernel(const FewArgs a) {
     constexpr int U = 8;
-    __shared__ int rows[kFewSlots + U], slots[kFewSlots + U], counts[2];
+    __shared__ int rows[kFewSlots], slots[kFewSlots], counts[2];
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int block = blockIdx.x / a.tiles, column = ((int)blockIdx.x % a.tiles * a.lanes + x) * W, count = max(0, min(W, a.D - column));
-    const long first = (long)block * groups * R, behind = min((long)a.V, first + groups * R);
+    // the workgroup's rows, `step` apart: frequent tokens are neighbours in most vocabularies
+    const int first = block * groups, step = (int)(gridDim.x / a.tiles) * groups;
     const int token = (int)threadIdx.x < a.N ? a.tokens[threadIdx.x] : -1;
-    const bool mine = token >= first && token < behind;
+    const bool mine = token >= first && token < a.V && (token - first) % step < groups;
     const unsigned long long in = __ballot(mine);
     if (wave < 2 && lane == 0) counts[wave] = __popcll(in);
     __syncthreads();
@@ -523,37 +537,40 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const FewArgs a) {
         rows[place] = token;
         slots[place] = threadIdx.x;
     }
-    if (threadIdx.x >= 128 && threadIdx.x < 128 + U) rows[found + threadIdx.x - 128] = -1;
     __syncthreads();
     const E *err = static_cast<const E *>(a.err) + column;
+    const unsigned long long group = a.lanes == 64 ? ~0ull : (1ull << a.lanes) - 1;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const long row = first + (long)r * groups + g;
-        if (row >= a.V || count <= 0) continue;
+        const long row = first + (long)r * step + g;
         float sum[W] = {};
         bool any = false;
-        for (int i = 0; i < found; i += U) {
-            float v[U][W];
+        for (int i = 0; i < found; i += a.lanes) {
+            // those of the group's row among the next entries, a bit for each, eight rows of errors in flight
+            unsigned long long own = __ballot(i + x < found && rows[i + x] == row) >> (lane - lane % a.lanes) & group;
+            any = any || own;
+            while (own) {
+                float v[U][W];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool own = rows[i + u] == row;
-                any = any || own;
+                for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
-                if (own) fetch_some<E, W>(err + slots[i + u] * a.err_stride, count, v[u], 0.0f);
+                    for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
+                    if (own && count > 0) fetch_some<E, W>(err + slots[i + __builtin_ctzll(own)] * a.err_stride, count, v[u], 0.0f);
+                    own &= own - 1;
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int q = 0; q < W; ++q) sum[q] += v[u][q];
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int q = 0; q < W; ++q) sum[q] += v[u][q];
         }
-        if (a.accumulate && !any) continue;
+        if (row >= a.V || count <= 0 || (a.accumulate && !any)) continue;
         G *to = static_cast<G *>(a.grad) + row * a.grad_stride + column;
         float old[W];
         if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
 #pragma unroll
         for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + sum[q] * a.scale : sum[q] * a.scale;
-        put_some<G, W, true>(to, count, sum);
+        put_row(to, count, sum, a.once);
     }
 }
 
@@ -561,7 +578,7 @@ template <typename E, typename G>
 int sum_few(hipStream_t stream, const FewArgs &args) {
     constexpr int W = kBoth<E, G>;
     FewArgs a = args;
-    a.lanes = std::min(64, power_of_two_from((a.D + W - 1) / W));
+    a.lanes = std::max(8, std::min(64, power_of_two_from((a.D + W - 1) / W)));
     a.tiles = (int)((a.D + (long)a.lanes * W - 1) / (a.lanes * W));
     // eight rows for a group where there are enough of them for the card
     const long groups = 256 / a.lanes, blocks = (a.V + groups - 1) / groups * a.tiles;
@@ -663,8 +680,9 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "embed_backward");
     int status = CNT_OK;
+    const bool once = past_caches(grad, V, D, grad_stride, grad_type);
     if (N <= kFewSlots) {
-        FewArgs few = {tokens, err, grad, err_stride, grad_stride, (int)N, V, D, 0, 0, accumulate, scale};
+        FewArgs few = {tokens, err, grad, err_stride, grad_stride, (int)N, V, D, 0, 0, accumulate, once, scale};
         with_type(err_type, [&](auto e) {
             with_type(grad_type, [&](auto g) { status = sum_few<typename decltype(e)::type, typename decltype(g)::type>(stream, few); });
         });
@@ -714,6 +732,7 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     a.err = err; a.grad = grad; a.partial = reinterpret_cast<float *>(mem + plan.partial);
     a.err_stride = err_stride; a.grad_stride = grad_stride;
     a.V = V; a.D = D; a.piece = plan.piece; a.accumulate = accumulate; a.scale = scale;
+    a.once = once;
     a.fill = next_fill();
     a.filled = (int)filled;
     with_type(err_type, [&](auto e) {
