@@ -94,7 +94,8 @@ int cnt_dense_backward(void *stream, int P, int D, int N, int act, float bias, c
  * split; calling both in this order on one stream is cnt_dense_backward.
  * Device memory: a weight half whose sum over the slots is cut into parts adds the parts up through a scratch buffer of 36 MB per
  * stream, which the library allocates the first time such a product runs on a stream and keeps; the same holds for
- * cnt_cnn_backward_weights, cnt_wavnetc_backward_weights and cnt_lstm_backward_weights.  Apart from that, only the *_create calls allocate. */
+ * cnt_cnn_backward_weights, cnt_wavnetc_backward_weights and cnt_lstm_backward_weights.  Apart from that, only the *_create calls
+ * allocate, and the first cnt_network_update and cnt_network_update_clipped of a network. */
 int cnt_dense_backward_errors(void *stream, int P, int D, int N, int act, const float *weights, const float *y,
                               float *err, float *prev_err);
 int cnt_dense_backward_weights(void *stream, int P, int D, int N, float bias, const float *x, const float *err,
@@ -105,9 +106,9 @@ int cnt_dense_backward_weights(void *stream, int P, int D, int N, float bias, co
  * memory, a stream under capture) adds its splits atomically instead. */
 int cnt_gemm_reserve(void *stream);
 int cnt_gemm_release(void *stream);
-/* How many such buffers the library holds at the moment.  That allocation is the only one any entry point other
- * than a *_create call makes, so a caller (or a test) that sees the same number before and after a pass knows that
- * the pass allocated nothing.  No counterpart in the reference. */
+/* How many such buffers the library holds at the moment.  No entry point allocates anything else but
+ * the *_create calls and a network's first cnt_network_update and cnt_network_update_clipped, so a caller (or a test)
+ * that sees the same number before and after a pass knows that the pass allocated nothing.  No counterpart in the reference. */
 int cnt_gemm_scratch_buffers(void);
 /* cnt_dense_backward_weights for callers that cannot allocate device memory (code under HIP graph capture, tight
  * serving loops, harnesses that forbid hipMalloc): same arguments, same result, but the split partial products go
@@ -124,14 +125,15 @@ int cnt_dense_backward_weights_static(void *stream, int P, int D, int N, float b
  *   out[n] = scale * table[tokens[n]], a row of zeros where tokens[n] is outside 0 .. V-1 (a slot without a symbol).
  * Row r of a matrix begins at r * stride elements; rows that are read may overlap (stride 0: one row for all), rows that are written
  * may not (stride >= D).  Bases need the alignment of an element only.  table_type, out_type: CNT_F32, CNT_BF16 or CNT_F16, any two of
- * them; products are formed in 32 bits and rounded once.  N and D up to a launch of 2^24 workgroups (CNT_ERR_ARG beyond). */
+ * them; products are formed in 32 bits and rounded once.  D <= 2^30, N up to a launch of 2^24 workgroups of
+ * 4 to 1024 slots (CNT_ERR_ARG beyond). */
 int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const void *table, long table_stride, const int *tokens,
                       float scale, int out_type, void *out, long out_stride);
 /* The table's gradient: grad[v] = scale * sum of err[n] over the slots n with tokens[n] = v, for all V rows (rows of zeros where
  * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
  * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
  * cnt_embed_scratch(V, D, N) bytes, aligned to 16, with any content, which the call has for itself until it has run (two captured
- * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^34. */
+ * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^33. */
 long cnt_embed_scratch(int V, int D, long N);
 int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
                        long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,

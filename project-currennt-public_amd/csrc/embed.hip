@@ -490,7 +490,8 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         const long row = (long)(block - a.first_blocks) * groups + g;
         if (row >= a.V) return;
         const int begin = a.starts[row], end = a.starts[row + 1];
-        if (end > begin ? (end - 1) / a.piece * a.piece >= begin : a.accumulate) return;  // the first workgroups', or nothing to add
+        // the first workgroups', or nothing to write
+        if (end > begin ? (end - 1) / a.piece * a.piece >= begin : a.accumulate || row < a.filled) return;
         add_entries<E, W>(a, begin, end, 0, 0, 0, 1, column, count, sum);
         write_row<G, W>(a, (int)row, column, count, sum);
         return;
@@ -590,9 +591,9 @@ int sum_few(hipStream_t stream, const FewArgs &args) {
     return CNT_OK;
 }
 
-// what a launch has workgroups for (2^24 of 256 threads)
+// What a launch has workgroups for, 2^24 of 256 threads: rows of 256 columns take the most, a fourth of one for each.
 bool gradient_sizes(int V, int D, long N) {
-    return V > 0 && V <= 1 << 23 && D > 0 && D <= 1 << 21 && N >= 0 && N <= 1L << 30 && std::max<long>(V, N) * D <= 1L << 34;
+    return V > 0 && V <= 1 << 23 && D > 0 && D <= 1 << 21 && N >= 0 && N <= 1L << 30 && std::max<long>(V, N) * D <= 1L << 33;
 }
 
 // threads that share a row, W columns each
@@ -640,7 +641,7 @@ extern "C" {
 int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const void *table, long table_stride, const int *tokens,
                       float scale, int out_type, void *out, long out_stride) {
     using namespace cnt;
-    CNT_REQUIRE(V > 0 && D > 0 && N >= 0, "embed_forward: bad sizes");
+    CNT_REQUIRE(V > 0 && D > 0 && D <= 1 << 30 && N >= 0, "embed_forward: bad sizes");
     CNT_REQUIRE(known_type(table_type) && known_type(out_type), "embed_forward: unknown element type");
     CNT_REQUIRE(table_stride >= 0 && out_stride >= D, "embed_forward: rows of the output overlap, or a negative stride");
     CNT_REQUIRE(table && (N == 0 || (tokens && out)), "embed_forward: null argument");

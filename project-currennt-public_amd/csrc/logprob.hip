@@ -4,7 +4,7 @@
 //   err_v = scale * (g * ([v = token] - p_v) - h * p_v * (logp_v + H))       g, h: errors of the token's logp and of the entropy
 //
 // One pass over the logits: a lane keeps the running maximum m of its logits, s = sum 2^t and w = sum t 2^t with t = (x - m) * scale *
-// log2(e), and brings them to a new maximum once in up to 32 logits; then lse = scale * m + log s and H = log s - ln 2 * w / s.  The
+// log2(e), and brings them to a new maximum once in 16 logits (32 in the longest rows' errors); then lse = scale * m + log s and H = log s - ln 2 * w / s.  The
 // difference to the maximum is formed before it is scaled, so the rows of a mask of the type's lowest value stay exact.  All sums are fp32.
 #include "elements.hpp"
 

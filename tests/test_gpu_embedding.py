@@ -90,7 +90,7 @@ def test_gradient_sizes(V, D, N):
 
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("grad", S.TYPES)
-@pytest.mark.parametrize("V,D,N", [(70001, 64, 5000), (90007, 257, 3000), (131072, 301, 40000)])
+@pytest.mark.parametrize("V,D,N", [(70001, 64, 5000), (90007, 257, 3000), (131072, 301, 40000), (8200, 520, 9000)])
 def test_gradient_of_tables_that_are_filled_on_the_way(V, D, N, grad, accumulate):
     rng = np.random.default_rng(V)
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.bfloat16, grad, rng, accumulate)

@@ -45,6 +45,15 @@ def test_embedding():
         _refused(call(**changes), what)
 
 
+def test_sizes_that_no_launch_takes():
+    L = load_package().capi.lib()
+    _refused(L.cnt_embed_forward(None, 4, 2 ** 30 + 1, 2, 0, P, 2 ** 31, P, 1.0, 0, P, 2 ** 31), "sizes")
+    assert L.cnt_embed_scratch(2 ** 23, 2 ** 10, 2 ** 23) > 0
+    for V, D, N in ((2 ** 23, 2 ** 10 + 1, 5), (5, 2 ** 10 + 1, 2 ** 23), (2 ** 12 + 1, 2 ** 21, 5)):
+        assert L.cnt_embed_scratch(V, D, N) == -1
+        _refused(L.cnt_embed_backward(None, V, D, N, P, 1.0, 0, P, D, 0, P, D, 0, P, 2 ** 40), "sizes")
+
+
 def test_log_probabilities():
     L = load_package().capi.lib()
 
