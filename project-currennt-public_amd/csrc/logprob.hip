@@ -334,14 +334,21 @@ __device__ __forceinline__ float logp_of(float x, const Stats &a, float scale, f
 __device__ __forceinline__ float entropy_of(const Stats &a, float log_s) {
     return a.m == kMinusInfinity && a.s == 0.0f ? 0.0f : log_s - kLn2 * (a.w / a.s);
 }
-// by one lane
+// The given token's logit, read in two steps that a kernel has in front of its work (behind it, values and gradient of 32000 rows of 1024 in fp32
+// took 48.0 us, 46.4 so).
+struct Given {
+    int token;  // -1: none, or nobody asks
+    float logit;
+};
+__device__ __forceinline__ int given_token(const RowArgs &a, long n) {
+    const int token = a.logp && a.tokens ? a.tokens[n] : -1;
+    return token < a.V ? token : -1;
+}
 template <typename T>
-__device__ __forceinline__ void write_stats(const RowArgs &a, long n, const Stats &s, float log_s) {
-    if (a.logp) {
-        const int token = a.tokens ? a.tokens[n] : -1;
-        const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-        a.logp[n] = token >= 0 && token < a.V ? logp_of((float)row[token], s, a.scale, log_s) : 0.0f;
-    }
+__device__ __forceinline__ Given given_logit(const T *row, int token) { return {token, token >= 0 ? (float)row[token] : 0.0f}; }
+// by one lane
+__device__ __forceinline__ void write_stats(const RowArgs &a, long n, const Given &g, const Stats &s, float log_s) {
+    if (a.logp) a.logp[n] = g.token >= 0 ? logp_of(g.logit, s, a.scale, log_s) : 0.0f;
     if (a.lse) a.lse[n] = s.m * a.scale + log_s;
     if (a.entropy) a.entropy[n] = entropy_of(s, log_s);
 }
@@ -404,11 +411,13 @@ __global__ __launch_bounds__(256) void logprob_short_kernel(const RowArgs a) {
     const long n = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const bool here = n < a.N;  // (whole groups of lanes)
     const T *row = static_cast<const T *>(a.logits) + (here ? n : 0) * a.stride;
+    const int token = here && l == 0 ? given_token(a, n) : -1;
     ShortRow<T, COUNT, LANES> x;
     x.load(row, here ? a.V : 0, l);
+    const Given given = given_logit(row, token);
     const Stats s = x.stats(a.scale * kLog2e);
     const float log_s = logf(s.s);
-    if (here && l == 0) write_stats<T>(a, n, s, log_s);
+    if (here && l == 0) write_stats(a, n, given, s, log_s);
     if (!TOP) return;
     // K rounds: the largest of what is left, the lowest token where several hold it.  As whole numbers in the order of the logits: their maxima
     // take one instruction per step across lanes.  What is taken, NaN and what is behind the row is 0, which no number is.
@@ -465,8 +474,9 @@ __device__ __forceinline__ void remember(Cells &c, float largest, int at) {
     c.first_at = a ? at : c.first_at;
     c.first = a ? largest : c.first;
 }
-// A bound that at least K of a wave's keys reach, and exactly K where no two are equal: keys up to COUNT per lane, `entries` in all; 0: there are
-// fewer, keys of 0 being none.  Bit by bit from the first on that not all keys have in common.
+// A bound that at least K of a wave's keys reach, and no more than K + kSlack but for equal ones: keys up to COUNT per lane, `entries` in all; 0: there
+// are fewer, keys of 0 being none.  Bit by bit between the first and the last that not all keys have in common.
+constexpr int kSlack = 8;
 template <int COUNT>
 __device__ __forceinline__ unsigned bound_of(const unsigned (&key)[COUNT], int entries, int K) {
     unsigned all = ~0u, any = 0;
@@ -479,16 +489,16 @@ __device__ __forceinline__ unsigned bound_of(const unsigned (&key)[COUNT], int e
     all = over_lanes<64>((int)all, [](int a, int b) { return a & b; });
     any = over_lanes<64>((int)any, [](int a, int b) { return a | b; });
     const unsigned differ = any & ~all;
-    const int top = differ ? 31 - __builtin_clz(differ) : -1;
+    const int top = differ ? 31 - __builtin_clz(differ) : -1, last = differ ? __builtin_ctz(differ) : 0;
     unsigned t = top < 0 ? all : all & ~((2u << top) - 1);
-    for (int bit = top; bit >= 0; --bit) {
+    for (int bit = top; bit >= last; --bit) {
         const unsigned more = t | 1u << bit;
         int count = 0;
 #pragma unroll
         for (int q = 0; q < COUNT; ++q)
             if (q * 64 < entries) count += __popcll(__ballot(key[q] >= more));
         if (count >= K) t = more;
-        if (count == K) break;
+        if (count >= K && count <= K + kSlack) break;
     }
     return t;
 }
@@ -530,6 +540,8 @@ __global__ __launch_bounds__(64 * WAVES, 8) void logprob_kernel(const RowArgs a)
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     const int begin = (int)blockIdx.y * a.part - lead_of(row), end = min(a.V, begin + a.part);
+    const bool shared_row = a.parts > 1;
+    const Given given = given_logit(row, shared_row || threadIdx.x > 0 ? -1 : given_token(a, n));
     Stats s;
     begin_stats(s);
     Cells cells = {kMinusInfinity, kMinusInfinity, kMinusInfinity, -1, -1};
@@ -577,7 +589,6 @@ __global__ __launch_bounds__(64 * WAVES, 8) void logprob_kernel(const RowArgs a)
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s = join(s, sh.stats[w], c);
     const float log_s = logf(s.s);
-    const bool shared_row = a.parts > 1;
     const long p = n * a.parts + blockIdx.y;
     if (threadIdx.x == 0) {
         if (shared_row) {
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(64 * WAVES, 8) void logprob_kernel(const RowArgs a)
             a.part_stats[p * 3 + 1] = s.s;
             a.part_stats[p * 3 + 2] = s.w;
         } else {
-            write_stats<T>(a, n, s, log_s);
+            write_stats(a, n, given, s, log_s);
         }
     }
     if (!TOP) return;
@@ -691,6 +702,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
     Stats s;
     begin_stats(s);
     const long p = n * a.parts;
+    const int given_one = given_token(a, n);
     if (lane < a.parts) s = {a.part_stats[(p + lane) * 3], a.part_stats[(p + lane) * 3 + 1], a.part_stats[(p + lane) * 3 + 2]};
     float v[Q];
     int t[Q];
@@ -701,9 +713,10 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
         v[q] = i < entries ? a.part_values[p * a.K + i] : 0.0f;
         t[q] = i < entries ? a.part_tokens[p * a.K + i] : -1;
     }
+    const Given given = given_logit(static_cast<const T *>(a.logits) + n * a.stride, given_one);
     s = join_lanes(s, c);
     const float log_s = logf(s.s);
-    if (lane == 0) write_stats<T>(a, n, s, log_s);
+    if (lane == 0) write_stats(a, n, given, s, log_s);
     if (a.K == 0) return;
     unsigned key[Q];
 #pragma unroll
@@ -826,12 +839,15 @@ __global__ __launch_bounds__(256) void logprob_short_error_kernel(const RowArgs 
     const long n = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const bool here = n < a.N;
     const float c = a.scale * kLog2e;
+    const T *row = static_cast<const T *>(a.logits) + (here ? n : 0) * a.stride;
+    const int token = here && l == 0 ? given_token(a, n) : -1;
     X x;
-    x.load(static_cast<const T *>(a.logits) + (here ? n : 0) * a.stride, here ? a.V : 0, l);
+    x.load(row, here ? a.V : 0, l);
+    const Given given = given_logit(row, token);
     const Stats s = x.stats(c);
     if (!here) return;
     const float log_s = logf(s.s), log2_s = log_s * kLog2e;
-    if (l == 0) write_stats<T>(a, n, s, log_s);
+    if (l == 0) write_stats(a, n, given, s, log_s);
     const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
@@ -984,6 +1000,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
     const float c = a.scale * kLog2e;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
+    const Given given = given_logit(row, threadIdx.x == 0 ? given_token(a, n) : -1);
     Stats s;
     begin_stats(s);
     Chunk<T, NV> x;
@@ -998,7 +1015,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s = join(s, stats[w], c);
     const float log_s = logf(s.s), log2_s = log_s * kLog2e;
-    if (threadIdx.x == 0) write_stats<T>(a, n, s, log_s);
+    if (threadIdx.x == 0) write_stats(a, n, given, s, log_s);
     __syncthreads();  // the errors may take the logits' place: the given token's logit has been read
     const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
