@@ -125,14 +125,14 @@ int cnt_dense_backward_weights_static(void *stream, int P, int D, int N, float b
  *   out[n] = scale * table[tokens[n]], a row of zeros where tokens[n] is outside 0 .. V-1 (a slot without a symbol).
  * Row r of a matrix begins at r * stride elements; rows that are read may overlap (stride 0: one row for all), rows that are written
  * may not (stride >= D).  Bases need the alignment of an element only.  table_type, out_type: CNT_F32, CNT_BF16 or CNT_F16, any two of
- * them; products are formed in 32 bits and rounded once.  D <= 2^30, N up to a launch of 2^24 workgroups of
+ * them; products are formed in 32 bits and rounded once; the scale is finite.  D <= 2^30, N up to a launch of 2^24 workgroups of
  * 4 to 1024 slots (CNT_ERR_ARG beyond). */
 int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const void *table, long table_stride, const int *tokens,
                       float scale, int out_type, void *out, long out_stride);
 /* The table's gradient: grad[v] = scale * sum of err[n] over the slots n with tokens[n] = v, for all V rows (rows of zeros where
  * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
  * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
- * cnt_embed_scratch(V, D, N) bytes, aligned to 16, with any content, which the call has for itself until it has run (two captured
+ * cnt_embed_scratch(V, D, N) bytes (0 for some sizes: NULL then), aligned to 16, with any content, which the call has for itself until it has run (two captured
  * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^33. */
 long cnt_embed_scratch(int V, int D, long N);
 int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,

@@ -3,13 +3,15 @@
 //   out[n] = scale * table[token[n]]                       (zero where slot n has no token)
 //   grad[v] = scale * sum over the slots n of token v of err[n]    (+ what grad held, if asked)
 //
-// Both move rows and are bounded by memory.  The gradient is formed by sorted tokens: a stable counting sort of the slots' tokens (one or
+// Both move rows and are bounded by memory.  Up to 128 slots, and tables that a workgroup's few hundred slots fill well, have kernels of their own
+// (see there).  Else the gradient is formed by sorted tokens: a stable counting sort of the slots' tokens (one or
 // two passes of at most ten bits) makes a token's slots neighbours in ascending order, so a row's sum has one order, is formed in 32 bits
 // and written once, without atomics and without clearing the table first.  Tokens are as skewed as in any text: a run that covers
 // whole pieces of the sorted list is added up piece by piece by workgroups of their own first.
 #include "elements.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 namespace cnt {
 namespace {
@@ -41,20 +43,20 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
         from[u] = static_cast<const T *>(a.table) + (held[u] ? token : 0) * a.table_stride;
     }
     for (int d = (threadIdx.x % a.lanes) * W; d < a.D; d += a.lanes * W) {
-        const int count = min(W, a.D - d);
-        float v[U][W];
+        const Columns c = columns_of<W>(d, a.D);
+        Vector<T, W> x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
-            if (held[u]) fetch_some<T, W>(from[u] + d, count, v[u], 0.0f);
+            x[u].clear();
+            if (held[u]) x[u].load(from[u], c);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (n + u * rows >= a.N) break;
+            float v[W];
 #pragma unroll
-            for (int q = 0; q < W; ++q) v[u][q] *= held[u] ? a.scale : 0.0f;
-            put_some<O, W, true>(static_cast<O *>(a.out) + (n + u * rows) * a.out_stride + d, count, v[u]);
+            for (int q = 0; q < W; ++q) v[q] = x[u].value(q) * (held[u] ? a.scale : 0.0f);
+            put_columns<O, W, true>(static_cast<O *>(a.out) + (n + u * rows) * a.out_stride, c, v);
         }
     }
 }
@@ -269,10 +271,22 @@ inline bool past_caches(const void *grad, int V, int D, long stride, int type) {
     const long row = stride * (long)element_size(type);
     return (reinterpret_cast<uintptr_t>(grad) % 128 == 0 && row % 128 == 0) || V * (long)D * (long)element_size(type) > 128L << 20;
 }
-template <typename T, int W>
-__device__ __forceinline__ void put_row(T *to, int count, const float (&v)[W], bool once) {
-    if (once) put_some<T, W, true>(to, count, v);
-    else put_some<T, W, false>(to, count, v);
+// columns c of a row of the gradient
+template <typename G, int W>
+__device__ __forceinline__ void put_sums(G *row, const Columns &c, const float (&sum)[W], float scale, int accumulate, int once) {
+    if (c.count <= 0) return;
+    float v[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = sum[q] * scale;
+    if (accumulate) {
+        Vector<G, W> old;
+        old.clear();
+        old.load(row, c);
+#pragma unroll
+        for (int q = 0; q < W; ++q) v[q] = old.value(q) + sum[q] * scale;
+    }
+    if (once) put_columns<G, W, true>(row, c, v);
+    else put_columns<G, W, false>(row, c, v);
 }
 
 // ----- sums of the runs -------------------------------------------------------------------------------------------------------
@@ -295,32 +309,31 @@ struct SumArgs {
     float scale;
 };
 
-// Sum of every step-th of the entries begin .. end and begin2 .. end2 of the sorted list, from number `first` on, W columns from `column` on, by the
+// Sum of every step-th of the entries begin .. end and begin2 .. end2 of the sorted list, from number `first` on, by the
 // `lanes` threads of a group: every thread has one of the next slots, which go round the group, so that a slot is waited for once in
 // `lanes` entries.
 template <typename E, int W>
-__device__ __forceinline__ void add_entries(const SumArgs &a, int begin, int end, int begin2, int end2, int first, int step, int column, int count,
+__device__ __forceinline__ void add_entries(const SumArgs &a, int begin, int end, int begin2, int end2, int first, int step, const Columns &c,
                                             float (&sum)[W]) {
     constexpr int U = 8;  // rows in flight
-    const E *err = static_cast<const E *>(a.err) + column;
+    const E *err = static_cast<const E *>(a.err);
     const int x = threadIdx.x % a.lanes, n1 = end - begin, n = n1 + end2 - begin2;
     for (int i = first; i < n; i += a.lanes * step) {
         const int e = i + x * step;
         const int mine = e < n ? a.slots[e < n1 ? begin + e : begin2 + e - n1] : 0;
         const int rows = min(a.lanes, (n - i + step - 1) / step);
         for (int k = 0; k < rows; k += U) {
-            float v[U][W];
+            Vector<E, W> v[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int slot = __shfl(mine, k + u, a.lanes);
-#pragma unroll
-                for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
-                if (k + u < rows && count > 0) fetch_some<E, W>(err + slot * a.err_stride, count, v[u], 0.0f);
+                v[u].clear();
+                if (k + u < rows && c.count > 0) v[u].load(err + slot * a.err_stride, c);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+                for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
         }
     }
 }
@@ -389,28 +402,22 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(const SumArgs a) {
     const int piece = blockIdx.x - a.first_blocks, begin = piece * a.piece, end = begin + a.piece;
     if (end > *a.total || a.keys[begin] != a.keys[end - 1]) return;
     const int x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
-    const int column = (blockIdx.y * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    const Columns c = columns_of<W>((blockIdx.y * a.lanes + x) * W, a.D);
     float sum[W] = {};
-    add_entries<E, W>(a, begin, end, 0, 0, g, 256 / a.lanes, column, count, sum);
+    add_entries<E, W>(a, begin, end, 0, 0, g, 256 / a.lanes, c, sum);
     join_groups<W>(a.lanes, sum);
-    if (g == 0 && count > 0) put_some<float, W>(a.partial + (size_t)piece * a.D + column, count, sum);
+    if (g == 0) put_sums(a.partial + (size_t)piece * a.D, c, sum, 1.0f, 0, 0);
 }
 
 template <typename G, int W>
-__device__ __forceinline__ void write_row(const SumArgs &a, int row, int column, int count, const float (&total)[W]) {
-    if (count <= 0) return;
-    G *to = static_cast<G *>(a.grad) + row * a.grad_stride + column;
-    float old[W], sum[W];
-    if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
-#pragma unroll
-    for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + total[q] * a.scale : total[q] * a.scale;
-    put_row(to, count, sum, a.once);
+__device__ __forceinline__ void write_row(const SumArgs &a, int row, const Columns &c, const float (&sum)[W]) {
+    put_sums(static_cast<G *>(a.grad) + row * a.grad_stride, c, sum, a.scale, a.accumulate, a.once);
 }
 
 // The rows of the runs that begin at entries from .. from + kWindow of the sorted list and hold no first entry of a piece, by a group of threads:
 // it goes through the list, eight rows of errors in flight, and writes a row where its run ends.
 template <typename E, typename G, int W>
-__device__ __forceinline__ void sum_short_runs(const SumArgs &a, int from, int column, int count) {
+__device__ __forceinline__ void sum_short_runs(const SumArgs &a, int from, const Columns &c) {
     constexpr int U = 8;
     const int n = *a.total, x = threadIdx.x % a.lanes;
     if (from >= n) return;
@@ -418,40 +425,39 @@ __device__ __forceinline__ void sum_short_runs(const SumArgs &a, int from, int c
     const int stop = min(n, (from / a.piece + 1) * a.piece), behind = min(from + kWindow, stop);
     const int skipped = a.keys[from % a.piece == 0 ? from : from - 1], last = a.keys[behind - 1];
     if (last == skipped) return;
-    const E *err = static_cast<const E *>(a.err) + column;
+    const E *err = static_cast<const E *>(a.err);
     int current = skipped;
     float sum[W] = {};
     for (int i0 = from; i0 < stop; i0 += a.lanes) {
         const int mine = i0 + x < stop ? a.keys[i0 + x] : skipped, my_slot = i0 + x < stop ? a.slots[i0 + x] : 0;
         const int here = min(a.lanes, stop - i0);
         for (int k = 0; k < here; k += U) {
-            float v[U][W];
+            Vector<E, W> v[U];
             int key[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 key[u] = __shfl(mine, k + u, a.lanes);
                 const int slot = __shfl(my_slot, k + u, a.lanes);
                 const bool needed = k + u < here && key[u] != skipped && (i0 + k + u < behind || key[u] == last);
-#pragma unroll
-                for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
-                if (needed && count > 0) fetch_some<E, W>(err + slot * a.err_stride, count, v[u], 0.0f);
+                v[u].clear();
+                if (needed && c.count > 0) v[u].load(err + slot * a.err_stride, c);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (k + u >= here) break;
                 if (key[u] != current) {
-                    if (current != skipped) write_row<G, W>(a, current, column, count, sum);
+                    if (current != skipped) write_row<G, W>(a, current, c, sum);
                     if (i0 + k + u >= behind) return;
                     current = key[u];
 #pragma unroll
                     for (int q = 0; q < W; ++q) sum[q] = 0.0f;
                 }
 #pragma unroll
-                for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+                for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
             }
         }
     }
-    if (stop == n || a.keys[stop] != current) write_row<G, W>(a, current, column, count, sum);
+    if (stop == n || a.keys[stop] != current) write_row<G, W>(a, current, c, sum);
 }
 
 // First workgroups: rows whose run holds the first entry of a piece, by all groups of the workgroup of the first such piece; whole pieces go
@@ -460,7 +466,8 @@ __device__ __forceinline__ void sum_short_runs(const SumArgs &a, int from, int c
 template <typename E, typename G, int W>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
-    const int block = blockIdx.x / a.tiles, column = ((int)blockIdx.x % a.tiles * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    const int block = blockIdx.x / a.tiles;
+    const Columns c = columns_of<W>(((int)blockIdx.x % a.tiles * a.lanes + x) * W, a.D);
     float sum[W] = {};
     if (block < a.first_blocks) {
         const int here = block * a.piece;
@@ -468,22 +475,23 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         const int row = a.keys[here], begin = a.starts[row], end = a.starts[row + 1];
         if (here - begin >= a.piece) return;
         const int whole = end / a.piece * a.piece;  // >= here
-        if (count > 0) {
+        if (c.count > 0) {
 #pragma unroll 8
             for (int p = block + g; p < whole / a.piece; p += groups) {
-                float v[W];
-                fetch_some<float, W>(a.partial + (size_t)p * a.D + column, count, v, 0.0f);
+                Vector<float, W> v;
+                v.clear();
+                v.load(a.partial + (size_t)p * a.D, c);
 #pragma unroll
-                for (int q = 0; q < W; ++q) sum[q] += v[q];
+                for (int q = 0; q < W; ++q) sum[q] += v.value(q);
             }
         }
-        add_entries<E, W>(a, begin, here, whole, end, g, groups, column, count, sum);
+        add_entries<E, W>(a, begin, here, whole, end, g, groups, c, sum);
         join_groups<W>(a.lanes, sum);
-        if (g == 0) write_row<G, W>(a, row, column, count, sum);
+        if (g == 0) write_row<G, W>(a, row, c, sum);
         return;
     }
     if (block < a.first_blocks + a.run_blocks) {
-        sum_short_runs<E, G, W>(a, ((block - a.first_blocks) * groups + g) * kWindow, column, count);
+        sum_short_runs<E, G, W>(a, ((block - a.first_blocks) * groups + g) * kWindow, c);
         return;
     }
     if (a.by_rows) {
@@ -492,8 +500,8 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         const int begin = a.starts[row], end = a.starts[row + 1];
         // the first workgroups', or nothing to write
         if (end > begin ? (end - 1) / a.piece * a.piece >= begin : a.accumulate || row < a.filled) return;
-        add_entries<E, W>(a, begin, end, 0, 0, 0, 1, column, count, sum);
-        write_row<G, W>(a, (int)row, column, count, sum);
+        add_entries<E, W>(a, begin, end, 0, 0, 0, 1, c, sum);
+        write_row<G, W>(a, (int)row, c, sum);
         return;
     }
     const long first = a.filled + ((long)(block - a.first_blocks - a.run_blocks) * groups + g) * kZeroRows;
@@ -502,7 +510,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
     for (int r = 0; r <= kZeroRows; ++r) bounds[r] = a.starts[min((long)a.V, first + r)];
 #pragma unroll
     for (int r = 0; r < kZeroRows; ++r)
-        if (first + r < a.V && bounds[r] == bounds[r + 1]) write_row<G, W>(a, (int)(first + r), column, count, sum);
+        if (first + r < a.V && bounds[r] == bounds[r + 1]) write_row<G, W>(a, (int)(first + r), c, sum);
 }
 
 // ----- few slots: no sort ---------------------------------------------------------------------------------------------------------
@@ -524,7 +532,8 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const FewArgs a) {
     constexpr int U = 8;
     __shared__ int rows[kFewSlots], slots[kFewSlots], counts[2];
     const int groups = 256 / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int block = blockIdx.x / a.tiles, column = ((int)blockIdx.x % a.tiles * a.lanes + x) * W, count = max(0, min(W, a.D - column));
+    const int block = blockIdx.x / a.tiles;
+    const Columns c = columns_of<W>(((int)blockIdx.x % a.tiles * a.lanes + x) * W, a.D);
     // the workgroup's rows, `step` apart: frequent tokens are neighbours in most vocabularies
     const int first = block * groups, step = (int)(gridDim.x / a.tiles) * groups;
     const int token = (int)threadIdx.x < a.N ? a.tokens[threadIdx.x] : -1;
@@ -539,7 +548,7 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const FewArgs a) {
         slots[place] = threadIdx.x;
     }
     __syncthreads();
-    const E *err = static_cast<const E *>(a.err) + column;
+    const E *err = static_cast<const E *>(a.err);
     const unsigned long long group = a.lanes == 64 ? ~0ull : (1ull << a.lanes) - 1;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -551,27 +560,21 @@ __global__ __launch_bounds__(256) void embed_few_kernel(const FewArgs a) {
             unsigned long long own = __ballot(i + x < found && rows[i + x] == row) >> (lane - lane % a.lanes) & group;
             any = any || own;
             while (own) {
-                float v[U][W];
+                Vector<E, W> v[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-#pragma unroll
-                    for (int q = 0; q < W; ++q) v[u][q] = 0.0f;
-                    if (own && count > 0) fetch_some<E, W>(err + slots[i + __builtin_ctzll(own)] * a.err_stride, count, v[u], 0.0f);
+                    v[u].clear();
+                    if (own && c.count > 0) v[u].load(err + slots[i + __builtin_ctzll(own)] * a.err_stride, c);
                     own &= own - 1;
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int q = 0; q < W; ++q) sum[q] += v[u][q];
+                    for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
             }
         }
-        if (row >= a.V || count <= 0 || (a.accumulate && !any)) continue;
-        G *to = static_cast<G *>(a.grad) + row * a.grad_stride + column;
-        float old[W];
-        if (a.accumulate) fetch_some<G, W>(to, count, old, 0.0f);
-#pragma unroll
-        for (int q = 0; q < W; ++q) sum[q] = a.accumulate ? old[q] + sum[q] * a.scale : sum[q] * a.scale;
-        put_row(to, count, sum, a.once);
+        if (row >= a.V || (a.accumulate && !any)) continue;
+        put_sums(static_cast<G *>(a.grad) + row * a.grad_stride, c, sum, a.scale, a.accumulate, a.once);
     }
 }
 
@@ -587,6 +590,222 @@ int sum_few(hipStream_t stream, const FewArgs &args) {
     auto kernel = many ? embed_few_kernel<E, G, W, 8> : embed_few_kernel<E, G, W, 1>;
     const long each = groups * (many ? 8 : 1);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((a.V + each - 1) / each * a.tiles)), dim3(256), 0, stream, a);
+    CNT_HIP(hipGetLastError());
+    return CNT_OK;
+}
+
+// ----- slabs of the list, each with a table of its own -----------------------------------------------------------------------------------
+// A workgroup sorts the slots of a slab that are its rows' in LDS, adds their errors up and writes its rows of the slab's table.  One slab's
+// table is the gradient itself; those of several are added up in order by a second launch.
+constexpr int kSlab = 512, kSlabRows = 1024, kSlabWaves = kSlab / 64, kSlabLanes = 16;
+// Against the sorted list, us.  One slab: 1000 x 64 from 300 slots 6.6 / 17.0, 100000 x 64 from 500 10 / 21, 50000 x 458 from 300 22 / 28; beyond
+// 65536 x 1024 from 500 54 / 47 (the zeros, in rows of 256 bytes here).
+constexpr long kOneSlabValues = 1 << 25;
+// Several: 256 x 64 from 32000 13.8 / 21.5, 5000 x 64 from 4000 13.6 / 24.5, 1100 x 256 from 4000 15.0 / 20.2, 2000 x 64 from 16000 16.6 / 26.2; beyond 1000
+// x 512 from 2000 15.8 / 14.5, 5000 x 512 from 1000 26 / 21, 20000 x 64 from 2000 21.0 / 23.7, 100 x 2048 from 16000 41 / 37.
+constexpr long kSlabValues = 3 << 17;    // of one table
+constexpr size_t kSlabBytes = 16 << 20;  // of all
+
+struct SlabArgs {
+    const int *tokens;
+    const void *err;
+    void *out;    // tables side by side, or the gradient
+    int *counts;  // entries of the slabs' rows, may be NULL
+    long err_stride, out_stride;
+    int N, V, D, bits, lanes, tiles, parts, accumulate, once;  // parts: workgroups that share a slab's rows
+    float scale;
+};
+
+template <typename E, typename G, int W>
+__global__ __launch_bounds__(kSlab) void embed_slab_kernel(const SlabArgs a) {
+    constexpr int U = kSlabLanes;  // entries of a group of threads at most: all of its errors are in flight together
+    static_assert(kSlabRows == 2 * kSlab, "two rows per thread in the scan");
+    union Words {
+        unsigned short one[kSlabWaves][kSlabRows];
+        unsigned two[kSlabWaves][kSlab];
+        uint4 all[kSlabWaves * kSlabRows / 8];
+    };
+    __shared__ Words before;  // entries of a row in 64 slots, then in all 64 slots in front of them
+    __shared__ int starts[kSlabRows + 1];
+    __shared__ unsigned list[kSlab];  // row and slot
+    __shared__ int totals[kSlabWaves];
+    __shared__ float heads[kSlab * W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tile = blockIdx.x % a.tiles, part = blockIdx.x / a.tiles % a.parts, slab = blockIdx.x / (a.tiles * a.parts);
+    const int base = slab * kSlab, slot = base + (int)threadIdx.x;
+    // the workgroup's rows
+    const int low = (int)((long)a.V * part / a.parts), rows = (int)((long)a.V * (part + 1) / a.parts) - low;
+    const int token = slot < a.N ? a.tokens[slot] : -1, row_of = token >= low && token < low + rows ? token - low : -1;
+    for (int k = threadIdx.x; k < kSlabWaves * kSlabRows / 8; k += kSlab) before.all[k] = uint4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    // lanes of one row find each other by one ballot per bit
+    const bool in = row_of >= 0;
+    unsigned long long same = __ballot(in);
+    for (int bit = 0; bit < a.bits; ++bit) {
+        const bool set = (row_of >> bit) & 1;
+        const unsigned long long b = __ballot(set);
+        same &= set ? b : ~b;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    if (in && rank == 0) before.one[wave][row_of] = (unsigned short)__popcll(same);
+    __syncthreads();
+    unsigned both = 0;  // of rows 2 * thread and 2 * thread + 1, side by side
+#pragma unroll
+    for (int h = 0; h < kSlabWaves; ++h) {
+        const unsigned c = before.two[h][threadIdx.x];
+        before.two[h][threadIdx.x] = both;
+        both += c;
+    }
+    const int all = (int)((both & 0xffff) + (both >> 16));
+    int upto = all;
+    for (int o = 1; o < 64; o *= 2) {
+        const int other = __shfl_up(upto, o);
+        if (lane >= o) upto += other;
+    }
+    if (lane == 63) totals[wave] = upto;
+    __syncthreads();
+    int at = upto - all;
+#pragma unroll
+    for (int w = 0; w < kSlabWaves; ++w) at += w < wave ? totals[w] : 0;
+    starts[2 * threadIdx.x] = at;
+    starts[2 * threadIdx.x + 1] = at + (int)(both & 0xffff);
+    if (threadIdx.x == kSlab - 1) starts[kSlabRows] = at + all;
+    __syncthreads();
+    if (in) list[starts[row_of] + before.one[wave][row_of] + rank] = (unsigned)row_of << 16 | threadIdx.x;
+    __syncthreads();
+    // Groups of threads have equal shares of the list.  A run that began in another's share is left to the group where it began.
+    const int n = starts[kSlabRows];
+    const int groups = kSlab / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
+    const Columns c = columns_of<W>((tile * a.lanes + x) * W, a.D);
+    const E *err = static_cast<const E *>(a.err) + base * a.err_stride;
+    G *out = static_cast<G *>(a.out) + ((long)slab * a.V + low) * a.out_stride;
+    auto write = [&](int row, const float (&total)[W]) { put_sums(out + row * a.out_stride, c, total, a.scale, a.accumulate, a.once); };
+    const int share = (n + groups - 1) / groups, begin = min(n, g * share), end = min(n, begin + share);
+    const int others = begin > 0 && begin < end && list[begin] >> 16 == list[begin - 1] >> 16 ? (int)(list[begin] >> 16) : -1;
+    Vector<E, W> v[U];
+    int key[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned entry = begin + u < end ? list[begin + u] : ~0u;
+        key[u] = begin + u < end ? (int)(entry >> 16) : -1;
+        v[u].clear();
+        if (begin + u < end && c.count > 0) v[u].load(err + (int)(entry & 0xffff) * a.err_stride, c);
+    }
+    int current = -1;
+    float sum[W] = {};
+    auto keep = [&]() {
+#pragma unroll
+        for (int q = 0; q < W; ++q) heads[(g * W + q) * a.lanes + x] = sum[q];
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (key[u] < 0) break;
+        if (key[u] != current) {
+            if (current >= 0 && current == others) keep();
+            else if (current >= 0) write(current, sum);
+            current = key[u];
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] = 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
+    }
+    if (current >= 0 && current == others) keep();
+    __syncthreads();
+    if (current >= 0 && current != others) {
+        for (int o = g + 1; o * share < n && (int)(list[o * share] >> 16) == current; ++o) {
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] += heads[(o * W + q) * a.lanes + x];
+        }
+        write(current, sum);
+    }
+    if (!a.accumulate) {
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum[q] = 0.0f;
+#pragma unroll 8
+        for (int row = g; row < rows; row += groups)
+            if (starts[row] == starts[row + 1]) write(row, sum);
+    }
+    if (a.counts && tile == 0)
+        for (int row = threadIdx.x; row < rows; row += kSlab) a.counts[slab * a.V + low + row] = starts[row + 1] - starts[row];
+}
+
+// The slabs' tables, a wave for each fourth of them.
+template <typename G>
+__global__ __launch_bounds__(256) void embed_slab_join_kernel(const float *tables, const int *counts, int slabs, int V, int D, int vectors, void *grad,
+                                                              long grad_stride, int accumulate, int once, float scale) {
+    constexpr int W = kBoth<float, G>, U = 8;
+    __shared__ float sums[3][W][64];
+    __shared__ int found[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = (slabs + 3) / 4;
+    const long i = (long)blockIdx.x * 64 + lane;
+    const int row = (int)(i / vectors);
+    Columns c = columns_of<W>((int)(i % vectors) * W, D);
+    if (row >= V) c.count = 0;
+    const int begin = min(slabs, wave * each), end = min(slabs, begin + each);
+    float sum[W] = {};
+    int entries = 0;
+    for (int s = begin; s < end; s += U) {
+        Vector<float, W> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u].clear();
+            if (s + u < end && c.count > 0) v[u].load(tables + ((long)(s + u) * V + row) * D, c);
+            if (accumulate && s + u < end && c.count > 0) entries += counts[(s + u) * V + row];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int q = 0; q < W; ++q) sums[wave - 1][q][lane] = sum[q];
+        found[wave - 1][lane] = entries;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; ++o) {
+        entries += found[o][lane];
+#pragma unroll
+        for (int q = 0; q < W; ++q) sum[q] += sums[o][q][lane];
+    }
+    if (accumulate && entries == 0) return;
+    put_sums(static_cast<G *>(grad) + row * grad_stride, c, sum, scale, accumulate, once);
+}
+
+// Scratch of a gradient by slabs: their tables and counts.
+struct SlabPlan {
+    int slabs;  // 0: by the sorted list
+    size_t counts, bytes;
+};
+SlabPlan slab_plan(int V, int D, long N) {
+    SlabPlan p = {};
+    const long slabs = (N + kSlab - 1) / kSlab;
+    const long values = (long)V * D;
+    if (N <= kFewSlots || values > (slabs > 1 ? kSlabValues : kOneSlabValues)) return p;
+    if (slabs > 1 && (size_t)(slabs * values) * sizeof(float) > kSlabBytes) return p;
+    p.slabs = (int)slabs;
+    if (slabs > 1) {
+        p.counts = (size_t)slabs * V * D * sizeof(float);
+        p.bytes = p.counts + (size_t)slabs * V * sizeof(int);
+    }
+    return p;
+}
+
+template <typename E, typename G>
+int sum_slab(hipStream_t stream, const SlabArgs &args, int slabs) {
+    constexpr int W = kBoth<E, G>;
+    SlabArgs a = args;
+    a.lanes = std::max(8, std::min(kSlabLanes, power_of_two_from((a.D + W - 1) / W)));  // (4: 31 rows of 8, 30000 slots 13.3 us, 11.9 with 8)
+    a.tiles = (int)((a.D + (long)a.lanes * W - 1) / (a.lanes * W));
+    // A workgroup for every compute unit, if its part has 32 rows (256 x 64 from 32000 slots, 512 workgroups 15.5 us; 1000 x 64 from 300, one 11.2;
+    // 131072 x 8 from 500, 1024 11.3).
+    const long most = std::max<long>((a.V + kSlabRows - 1) / kSlabRows, 256 / ((long)slabs * a.tiles));
+    a.parts = (int)std::max(1L, std::min<long>((a.V + 31) / 32, most));
+    while ((long)a.parts << a.bits < a.V) ++a.bits;
+    hipLaunchKernelGGL((embed_slab_kernel<E, G, W>), dim3((unsigned)((long)slabs * a.tiles * a.parts)), dim3(kSlab), 0, stream, a);
     CNT_HIP(hipGetLastError());
     return CNT_OK;
 }
@@ -645,6 +864,7 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
     CNT_REQUIRE(known_type(table_type) && known_type(out_type), "embed_forward: unknown element type");
     CNT_REQUIRE(table_stride >= 0 && out_stride >= D, "embed_forward: rows of the output overlap, or a negative stride");
     CNT_REQUIRE(table && (N == 0 || (tokens && out)), "embed_forward: null argument");
+    CNT_REQUIRE(std::isfinite(scale), "embed_forward: the scale has to be finite");
     if (N == 0) return CNT_OK;
     const int wide = table_type == CNT_F32 || out_type == CNT_F32 ? 4 : 8;
     LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + wide - 1) / wide)), scale};
@@ -664,7 +884,8 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
 
 long cnt_embed_scratch(int V, int D, long N) {
     if (!cnt::gradient_sizes(V, D, N)) return -1;
-    return (long)cnt::sort_plan(V, D, N).bytes;
+    const cnt::SlabPlan slabs = cnt::slab_plan(V, D, N);
+    return (long)(slabs.slabs ? slabs.bytes : cnt::sort_plan(V, D, N).bytes);
 }
 
 int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
@@ -674,9 +895,12 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     CNT_REQUIRE(gradient_sizes(V, D, N), "embed_backward: bad sizes");
     CNT_REQUIRE(known_type(err_type) && known_type(grad_type), "embed_backward: unknown element type");
     CNT_REQUIRE(err_stride >= 0 && grad_stride >= D, "embed_backward: rows of the gradient overlap, or a negative stride");
-    CNT_REQUIRE(grad && scratch && (N == 0 || (tokens && err)), "embed_backward: null argument");
+    CNT_REQUIRE(std::isfinite(scale), "embed_backward: the scale has to be finite");
+    const SlabPlan slabs = slab_plan(V, D, N);
     const SortPlan plan = sort_plan(V, D, N);
-    CNT_REQUIRE(scratch_bytes >= plan.bytes, "embed_backward: %zu bytes of scratch memory, %zu are needed", scratch_bytes, plan.bytes);
+    const size_t need = slabs.slabs ? slabs.bytes : plan.bytes;
+    CNT_REQUIRE(grad && (scratch || need == 0) && (N == 0 || (tokens && err)), "embed_backward: null argument");
+    CNT_REQUIRE(scratch_bytes >= need, "embed_backward: %zu bytes of scratch memory, %zu are needed", scratch_bytes, need);
     CNT_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embed_backward: the scratch memory is not aligned to 16 bytes");
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "embed_backward");
@@ -690,6 +914,28 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
         return status;
     }
     char *mem = static_cast<char *>(scratch);
+    if (slabs.slabs == 1) {
+        SlabArgs s = {tokens, err, grad, nullptr, err_stride, grad_stride, (int)N, V, D, 0, 0, 0, 0, accumulate, once, scale};
+        with_type(err_type, [&](auto e) {
+            with_type(grad_type, [&](auto g) { status = sum_slab<typename decltype(e)::type, typename decltype(g)::type>(stream, s, 1); });
+        });
+        return status;
+    }
+    if (slabs.slabs) {
+        int *counts = reinterpret_cast<int *>(mem + slabs.counts);
+        SlabArgs s = {tokens, err, mem, accumulate ? counts : nullptr, err_stride, D, (int)N, V, D, 0, 0, 0, 0, 0, 0, 1.0f};
+        with_type(err_type, [&](auto e) { status = sum_slab<typename decltype(e)::type, float>(stream, s, slabs.slabs); });
+        CNT_TRY(status);
+        with_type(grad_type, [&](auto g) {
+            using G = typename decltype(g)::type;
+            constexpr int W = kBoth<float, G>;
+            const int vectors = (D + W - 1) / W;
+            hipLaunchKernelGGL((embed_slab_join_kernel<G>), dim3((unsigned)(((long)V * vectors + 63) / 64)), dim3(256), 0, stream,
+                               reinterpret_cast<const float *>(mem), counts, slabs.slabs, V, D, vectors, grad, grad_stride, accumulate, (int)once, scale);
+        });
+        CNT_HIP(hipGetLastError());
+        return CNT_OK;
+    }
     auto ints = [&](size_t at) { return reinterpret_cast<int *>(mem + at); };
     SortArgs s = {};
     s.counts = ints(plan.counts); s.total = ints(plan.total);

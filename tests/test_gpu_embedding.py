@@ -82,10 +82,24 @@ def test_gradient(V, D, N, err, grad, accumulate):
 @pytest.mark.parametrize("V,D,N", [
     (1, 3, 1024), (1, 1, 1000), (2, 300, 1023), (9, 64, 1025), (50, 7, 513), (3000, 100, 1024), (100003, 33, 1000), (20000, 1030, 300), (5, 70, 49),
     (1, 3, 5000), (2, 4, 70001), (256, 8, 66000), (1024, 5, 9001), (1025, 5, 9001), (65536, 3, 5000), (65537, 3, 5000),
-    (1 << 20, 1, 3000), ((1 << 20) + 1, 1, 3000), (700, 1, 600000), (5, 2, 0), (100003, 17, 1), (64, 513, 4097)])
+    (1 << 20, 1, 3000), ((1 << 20) + 1, 1, 3000), (700, 1, 600000), (5, 2, 0), (100003, 17, 1), (64, 513, 4097),
+    (600, 300, 9000), (1024, 1030, 1500), (64, 515, 33000), (1024, 400, 2000), (1025, 400, 2000), (65536, 7, 5000), (65537, 7, 5000), (3, 140000, 1000),
+    (16400, 2051, 512)])
 def test_gradient_sizes(V, D, N):
     rng = np.random.default_rng(N + D)
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.float32, torch.float32, rng)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("grad", S.TYPES)
+@pytest.mark.parametrize("err", [torch.float32, torch.float16])
+@pytest.mark.parametrize("V,D,N", [
+    (1, 1, 129), (1, 70, 512), (2, 3, 513), (7, 130, 511), (1000, 9, 1025), (1023, 5, 500), (1024, 33, 512), (1024, 1, 3001), (1025, 5, 512), (256, 64, 16001),
+    (300, 1030, 200), (512, 8, 140000), (16, 4, 65537), (65, 300, 5000), (1025, 9, 400), (100003, 17, 512), (2047, 65, 3000), (40007, 6, 1500),
+    (3001, 1, 60000)])
+def test_gradient_by_slabs(V, D, N, err, grad, accumulate):
+    rng = np.random.default_rng(V + N)
+    _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), err, grad, rng, accumulate)
 
 
 @pytest.mark.parametrize("accumulate", [False, True])
@@ -96,11 +110,11 @@ def test_gradient_of_tables_that_are_filled_on_the_way(V, D, N, grad, accumulate
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.bfloat16, grad, rng, accumulate)
 
 
-@pytest.mark.parametrize("N", [100, 1000, 2500])
+@pytest.mark.parametrize("N,D", [(100, 33), (500, 33), (1000, 33), (2500, 33), (1000, 1400), (2500, 1400)])
 @pytest.mark.parametrize("kind", ["none", "one", "last", "ascending", "descending", "outside"])
-def test_gradient_orders_of_tokens(kind, N):
+def test_gradient_orders_of_tokens(kind, N, D):
     rng = np.random.default_rng(3)
-    V, D = 300, 33
+    V = 300
     t = {"none": np.full(N, -1), "one": np.full(N, 17), "last": np.full(N, V - 1), "ascending": np.sort(rng.integers(0, V, N)),
          "descending": -np.sort(-rng.integers(0, V, N)), "outside": rng.integers(-V, 3 * V, N)}[kind].astype(np.int32)
     t[:1] = -2 ** 31 if kind == "outside" else t[:1]
@@ -108,10 +122,11 @@ def test_gradient_orders_of_tokens(kind, N):
     _check_gradient(PC.pkg().capi, V, D, t, torch.float32, torch.bfloat16, rng, True)
 
 
-def test_gradient_rows_anywhere_and_broadcast_errors():
+@pytest.mark.parametrize("V,N", [(50, 70), (50, 300), (50, 700), (7000, 700)])
+def test_gradient_rows_anywhere_and_broadcast_errors(V, N):
     capi = PC.pkg().capi
     rng = np.random.default_rng(8)
-    V, D, N = 50, 65, 700
+    D = 65
     t = _tokens(rng, N, V)
     for dtype in S.TYPES:
         wide, place = _dev(rng.standard_normal((N, 80)), dtype), torch.full((V, 71), 3.0, device="cuda")
@@ -162,10 +177,11 @@ def test_gradient_against_differences():
     S.assert_close(S.f64(grad), want, S.U * (count[:, None] + 1.0) * size + 1e-12)
 
 
-def test_on_another_stream_and_replayed_from_a_graph():
+@pytest.mark.parametrize("V,N", [(500, 100), (500, 400), (500, 4000), (9000, 4000)])
+def test_on_another_stream_and_replayed_from_a_graph(V, N):
     capi = PC.pkg().capi
     rng = np.random.default_rng(5)
-    V, D, N = 500, 48, 4000
+    D = 48
     w, t, e = _dev(rng.standard_normal((V, D)).astype(np.float32)), _dev(_tokens(rng, N, V)), _dev(rng.standard_normal((N, D)).astype(np.float32))
     out, grad = torch.zeros(N, D, device="cuda"), torch.zeros(V, D, device="cuda")
     scratch = torch.empty(capi.embed_scratch(V, D, N), dtype=torch.uint8, device="cuda")

@@ -45,6 +45,13 @@ def test_embedding():
         _refused(call(**changes), what)
 
 
+def test_embedding_scales():
+    L = load_package().capi.lib()
+    for scale in (float("inf"), float("nan")):
+        _refused(L.cnt_embed_forward(None, 4, 4, 2, 0, P, 4, P, scale, 0, P, 4), "finite")
+        _refused(L.cnt_embed_backward(None, 4, 4, 2, P, scale, 0, P, 4, 0, P, 4, 0, P, 2 ** 20), "finite")
+
+
 def test_sizes_that_no_launch_takes():
     L = load_package().capi.lib()
     _refused(L.cnt_embed_forward(None, 4, 2 ** 30 + 1, 2, 0, P, 2 ** 31, P, 1.0, 0, P, 2 ** 31), "sizes")
