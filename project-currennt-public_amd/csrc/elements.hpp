@@ -43,17 +43,6 @@ __device__ __forceinline__ void put_elements(T *p, const float (&v)[N]) {
     if (ONCE) __builtin_nontemporal_store(x, to);
     else *to = x;
 }
-// the first `count` of N, 0 <= count <= N
-template <typename T, int N, bool ONCE = false>
-__device__ __forceinline__ void fetch_some(const T *p, int count, float (&v)[N], float rest) {
-    if (count == N) {
-        fetch_elements<T, N, ONCE>(p, v);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < count ? (float)p[i] : rest;
-}
-
 // A thread's columns of a row of D values: `count` from `column` on.  The last ones of a row are read `back` values earlier, so that a row of at least
 // W values is read in whole vectors; a vector's first `back` values are another thread's then.
 struct Columns {

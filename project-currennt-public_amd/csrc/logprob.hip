@@ -95,19 +95,6 @@ __device__ __forceinline__ void put_within(T *row, int at, int end, const float 
     for (int i = 0; i < W; ++i)
         if (at + i >= 0 && at + i < end) row[at + i] = (T)v[i];
 }
-// logits begin .. begin + SPAN of a row, those outside of 0 .. end are -inf
-template <bool ONCE, typename T, int NV>
-__device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int lane, Chunk<T, NV> &c) {
-    constexpr int W = Chunk<T, NV>::W;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float v[W];
-        fetch_within<ONCE>(row, begin + (j * 64 + lane) * W, end, v, kMinusInfinity);
-#pragma unroll
-        for (int i = 0; i < W; ++i) c.x[j * W + i] = v[i];
-    }
-}
-
 // 16 bytes of a row as they stand in memory.  values<USE>(): the logits in 32 bits, converted anew for every USE: from expressions that it knows to be
 // the same the compiler keeps one use's 32-bit values for the next, which takes twice the registers of 16-bit logits.
 template <int USE>
@@ -129,6 +116,28 @@ struct Raw {
         x = words{0u, 0u, 0u, 0u};
         if (whole) x = __builtin_nontemporal_load(reinterpret_cast<const words *>(p));
     }
+    // The logits from `at` on that are within 0 .. end, the others are -inf: whole vectors by the first of these, the rest by the second, which a lane
+    // calls for all of its vectors behind the first, so that one's loads do not wait for another's.
+    template <bool ONCE>
+    __device__ __forceinline__ void load_within(const T *row, int at, int end) {
+        constexpr unsigned nothing = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __bf16>::value ? 0xff80ff80u : 0xfc00fc00u;
+        x = words{nothing, nothing, nothing, nothing};
+        const auto *from = reinterpret_cast<const words *>(row + at);
+        if (at >= 0 && at + kWide<T> <= end) x = ONCE ? __builtin_nontemporal_load(from) : *from;
+    }
+    __device__ __forceinline__ void load_edge(const T *row, int at, int end) {
+        if (at >= end || at + kWide<T> <= 0 || (at >= 0 && at + kWide<T> <= end)) return;
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) {
+            if (at + i < 0 || at + i >= end) continue;
+            if constexpr (sizeof(T) == 4) {
+                x[i] = reinterpret_cast<const unsigned *>(row)[at + i];
+            } else {
+                const unsigned one = reinterpret_cast<const unsigned short *>(row)[at + i];
+                x[i / 2] = i % 2 ? (x[i / 2] & 0xffffu) | one << 16 : (x[i / 2] & 0xffff0000u) | one;
+            }
+        }
+    }
     template <int USE>
     __device__ __forceinline__ void values(float (&v)[kWide<T>]) const {
 #pragma unroll
@@ -147,6 +156,13 @@ struct RawChunk {
 #pragma unroll
         for (int j = 0; j < NV; ++j) part[j].load(chunk + (j * 64 + lane) * kWide<T>, true);
     }
+    template <bool ONCE>
+    __device__ __forceinline__ void load_within(const T *row, int begin, int end, int lane) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) part[j].template load_within<ONCE>(row, begin + (j * 64 + lane) * kWide<T>, end);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) part[j].load_edge(row, begin + (j * 64 + lane) * kWide<T>, end);
+    }
     __device__ __forceinline__ void values(Chunk<T, NV> &c) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -157,6 +173,14 @@ struct RawChunk {
         }
     }
 };
+
+// logits begin .. begin + SPAN of a row, those outside of 0 .. end are -inf
+template <bool ONCE, typename T, int NV>
+__device__ __forceinline__ void load_chunk(const T *row, int begin, int end, int lane, Chunk<T, NV> &c) {
+    RawChunk<T, NV> x;
+    x.template load_within<ONCE>(row, begin, end, lane);
+    x.values(c);
+}
 
 // up to here r - m * c is below 2^-4
 constexpr float kMostFused = 1 << 20;
@@ -370,15 +394,21 @@ __device__ __forceinline__ float of_ordered(unsigned k) { return __uint_as_float
 // where they can hold it: a row's steps across lanes and the rounds of its alternatives are then taken for four rows at a time.
 template <typename T, int COUNT, int LANES>
 struct ShortRow {
-    static constexpr int W = kWide<T> < COUNT ? kWide<T> : COUNT, NV = COUNT / W;
+    static constexpr int W = kWide<T>, NV = COUNT / W;
     float x[COUNT];
     static __device__ __forceinline__ int index(int i, int l) { return (i / W * LANES + l) * W + i % W; }
     __device__ __forceinline__ void load(const T *row, int V, int l) {
+        Raw<T> part[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) part[j].template load_within<true>(row, index(j * W, l), V);
+        if (V % W) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) part[j].load_edge(row, index(j * W, l), V);
+        }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int at = (j * LANES + l) * W;
             float v[W];
-            fetch_some<T, W, true>(row + at, max(0, min(W, V - at)), v, kMinusInfinity);
+            part[j].template values<0>(v);
 #pragma unroll
             for (int i = 0; i < W; ++i) x[j * W + i] = v[i];
         }
@@ -793,14 +823,17 @@ __device__ __forceinline__ void put_gradient(T *row, int begin, int end, int lan
     }
 }
 
-// From saved statistics, `parts` workgroups for a row, neighbouring ones for neighbouring stretches (rows of 32000 16-bit logits dealt row by
-// row instead: 75 us for 3001).  A wave has one chunk but in very long rows.
+// From saved statistics, `parts` waves for a row, neighbouring ones for neighbouring stretches (rows of 32000 16-bit logits dealt row by row
+// instead: 75 us for 3001; workgroups that have one row each: 55 us for
+// 6517 of 9819, 47 so).  A wave has one chunk but in very long rows.
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) {
     constexpr int SPAN = Chunk<T, NV>::SPAN, W = kWide<T>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long n = blockIdx.x / (unsigned)a.parts;
-    const int stretch = blockIdx.x % (unsigned)a.parts;
+    const unsigned id = blockIdx.x * 4 + wave;
+    const long n = id / (unsigned)a.parts;
+    const int stretch = id % (unsigned)a.parts;
+    if (n >= a.N) return;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
     auto errors = [&](float (&t)[W], int at, float ref, const Slopes &s) {
@@ -808,26 +841,44 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) 
         for (int i = 0; i < W; ++i) t[i] = __builtin_fmaf(t[i], a.scale, -ref) * kLog2e;
         errors_of<W>(at, s, t);
     };
-    for (int at = (stretch * 4 + wave) * SPAN - lead_of(row); at < a.V; at += a.parts * 4 * SPAN) {
+    for (int at = stretch * SPAN - lead_of(row); at < a.V; at += a.parts * SPAN) {
         const bool whole = at >= 0 && at + SPAN <= a.V;
         RawChunk<T, NV> x;  // (asked for in front of the row's values)
         if (whole) x.load(row + at, lane);
+        else x.template load_within<true>(row, at, a.V, lane);
         const float lse = a.lse[n], ref = lse == kMinusInfinity ? 0.0f : lse;
         const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int first = at + (j * 64 + lane) * W;
             float t[W];
-            if (whole) {
-                x.part[j].template values<0>(t);
-                errors(t, first, ref, s);
-                put_elements<T, W, true>(to + first, t);
-            } else {
-                fetch_within<true>(row, first, a.V, t, kMinusInfinity);
-                errors(t, first, ref, s);
-                put_within(to, first, a.V, t);
-            }
+            x.part[j].template values<0>(t);
+            errors(t, first, ref, s);
+            if (whole) put_elements<T, W, true>(to + first, t);
+            else put_within(to, first, a.V, t);
         }
+    }
+}
+
+// The same for rows that a wave or 16 lanes hold (a workgroup for each of 38270 rows of 41 16-bit logits: 57 us).
+template <typename T, int COUNT, int LANES>
+__global__ __launch_bounds__(256) void logprob_short_gradient_kernel(const RowArgs a) {
+    using X = ShortRow<T, COUNT, LANES>;
+    constexpr int W = X::W;
+    const int l = threadIdx.x % LANES;
+    const long n = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (n >= a.N) return;
+    X x;
+    x.load(static_cast<const T *>(a.logits) + n * a.stride, a.V, l);
+    const float lse = a.lse[n], ref = lse == kMinusInfinity ? 0.0f : lse;
+    const Slopes slopes = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
+    T *to = static_cast<T *>(a.err) + n * a.err_stride;
+#pragma unroll
+    for (int j = 0; j < X::NV; ++j) {
+        float t[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = __builtin_fmaf(x.x[j * W + i], a.scale, -ref) * kLog2e;
+        put_errors<T, W>(to, (j * LANES + l) * W, a.V, slopes, t);
     }
 }
 
@@ -1066,6 +1117,22 @@ void with_lanes(int V, F f) {
     else f(integral_constant<int, 32>(), integral_constant<int, 64>());
 }
 
+// The same for a row and its errors, which have no alternatives to look for: up to twice as long in 16 bits (values and gradient of 20000 rows of 4000
+// fp16 logits 62 us, 77 by a workgroup for each; of 4001 fp32 logits 118 and 108).
+template <typename T>
+constexpr int kErrorSpan = sizeof(T) == 2 ? 2 * kSpan : kSpan;
+template <typename T, typename F>
+void with_error_lanes(int V, F f) {
+    using std::integral_constant;
+    if constexpr (sizeof(T) == 2) {
+        if (V > kSpan) {
+            f(integral_constant<int, 64>(), integral_constant<int, 64>());
+            return;
+        }
+    }
+    with_lanes(V, f);
+}
+
 size_t scratch_of(long N, int V, int K) {
     const int parts = parts_of(N, V, K);
     return parts == 1 ? 0 : (size_t)N * parts * (3 + 2 * (size_t)K) * sizeof(float);
@@ -1109,10 +1176,18 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
 }
 
 int gradient(hipStream_t stream, int type, RowArgs &a) {
-    a.parts = (int)std::min({1024L, ((1L << 24) - 1) / a.N, (a.V + 63L + 4 * kSpan - 1) / (4 * kSpan)});
+    a.parts = (int)std::min({4096L, ((1L << 26) - 4) / a.N, (a.V + 63L + kSpan - 1) / kSpan});
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), dim3((unsigned)(a.N * a.parts)), dim3(256), 0, stream, a);
+        if (a.V <= kErrorSpan<T>) {
+            with_error_lanes<T>(a.V, [&](auto count, auto lanes) {
+                constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
+                const dim3 grid((unsigned)((a.N + 256 / LANES - 1) / (256 / LANES)));
+                hipLaunchKernelGGL((logprob_short_gradient_kernel<T, COUNT, LANES>), grid, dim3(256), 0, stream, a);
+            });
+            return;
+        }
+        hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), dim3((unsigned)((a.N * a.parts + 3) / 4)), dim3(256), 0, stream, a);
     });
     CNT_HIP(hipGetLastError());
     return CNT_OK;
@@ -1217,8 +1292,8 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
         // what rows may begin inside a cache line by (lead_of)
         const bool lines = reinterpret_cast<uintptr_t>(logits) % 128 == 0 && (stride * (long)sizeof(T) % 128 == 0 || N == 1);
         const int lead = lines ? 0 : 127 / (int)sizeof(T);
-        if (V <= kSpan) {
-            with_lanes(V, [&](auto count, auto lanes) {
+        if (V <= kErrorSpan<T>) {
+            with_error_lanes<T>(V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((N + 256 / LANES - 1) / (256 / LANES)));
                 hipLaunchKernelGGL((logprob_short_error_kernel<T, COUNT, LANES>), grid, dim3(256), 0, stream, a);
