@@ -22,41 +22,76 @@ struct LookupArgs {
     void *out;
     const int *tokens;
     long N, table_stride, out_stride;
-    int V, D, lanes;  // lanes: threads that share a row
+    int V, D, lanes, lead;  // threads that share a row; values by which its rows may begin behind a line's begin
     float scale;
 };
 
-constexpr int kSlotsPerThread = 4;
+constexpr int kSlotsPerThread = 4, kLine = 128;
 
-// A thread has the same columns of several slots, whose tokens and then rows it asks for together.
-template <typename T, typename O>
+// A thread has the same columns of several slots, whose tokens and then rows it asks for together.  The output's rows are dealt to threads in vectors
+// from a cache line's begin on; not LINES: rows that begin inside a line (33222 rows of 1204, bf16 to fp32, 36 us, dealt from the rows' begins 44; the
+// questions that this asks are spared for the others, 16 rows of 4096 4.4 us and 6.2).
+template <typename T, typename O, bool LINES>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
     constexpr int W = kBoth<T, O>, U = kSlotsPerThread;
     const int rows = 256 / a.lanes;
     const long n = (long)blockIdx.x * (rows * U) + threadIdx.x / a.lanes;
+    const bool whole = a.D >= W;
     bool held[U];
     const T *from[U];
+    O *to[U];
+    int lead[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int token = n + u * rows < a.N ? a.tokens[n + u * rows] : -1;
         held[u] = token >= 0 && token < a.V;
         from[u] = static_cast<const T *>(a.table) + (held[u] ? token : 0) * a.table_stride;
+        to[u] = static_cast<O *>(a.out) + (n + u * rows) * a.out_stride;
+        lead[u] = LINES ? 0 : (int)(reinterpret_cast<uintptr_t>(to[u]) % kLine / sizeof(O));
     }
-    for (int d = (threadIdx.x % a.lanes) * W; d < a.D; d += a.lanes * W) {
-        const Columns c = columns_of<W>(d, a.D);
+    for (int k = (threadIdx.x % a.lanes) * W; k < a.D + a.lead; k += a.lanes * W) {
         Vector<T, W> x[U];
+        if (LINES) {
+            const Columns c = columns_of<W>(k, a.D);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                x[u].clear();
+                if (held[u]) x[u].load(from[u], c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (n + u * rows >= a.N) break;
+                float v[W];
+#pragma unroll
+                for (int q = 0; q < W; ++q) v[q] = x[u].value(q) * (held[u] ? a.scale : 0.0f);
+                put_columns<O, W, true>(to[u], c, v);
+            }
+            continue;
+        }
+        int at[U];  // the column read first: a row's first and last vectors are read where the row has whole ones
+        bool in[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            const int d = k - lead[u];
+            in[u] = d < a.D && d + W > 0 && n + u * rows < a.N;
+            at[u] = max(0, whole ? min(d, a.D - W) : d);
             x[u].clear();
-            if (held[u]) x[u].load(from[u], c);
+            if (in[u] && held[u]) x[u].load(from[u], Columns{at[u], min(W, a.D - at[u]), 0, whole});
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (n + u * rows >= a.N) break;
+            if (!in[u]) continue;
+            const int d = k - lead[u];
             float v[W];
 #pragma unroll
             for (int q = 0; q < W; ++q) v[q] = x[u].value(q) * (held[u] ? a.scale : 0.0f);
-            put_columns<O, W, true>(static_cast<O *>(a.out) + (n + u * rows) * a.out_stride, c, v);
+            if (at[u] == d && whole) {
+                put_elements<O, W, true>(to[u] + d, v);
+                continue;
+            }
+#pragma unroll
+            for (int q = 0; q < W; ++q)
+                if (at[u] + q >= d && at[u] + q < min(d + W, a.D)) to[u][at[u] + q] = (O)v[q];
         }
     }
 }
@@ -867,15 +902,20 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
     CNT_REQUIRE(std::isfinite(scale), "embed_forward: the scale has to be finite");
     if (N == 0) return CNT_OK;
     const int wide = table_type == CNT_F32 || out_type == CNT_F32 ? 4 : 8;
-    LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + wide - 1) / wide)), scale};
+    const long size = (long)element_size(out_type);
+    const bool lines = reinterpret_cast<uintptr_t>(out) % kLine == 0 && (N == 1 || out_stride * size % kLine == 0);
+    const int lead = lines ? 0 : kLine / (int)size - 1;
+    LookupArgs a = {table, out, tokens, N, table_stride, out_stride, V, D, std::min(256, power_of_two_from((D + lead + wide - 1) / wide)), lead, scale};
     const long slots = 256 / a.lanes * kSlotsPerThread, blocks = (N + slots - 1) / slots;
     CNT_REQUIRE(blocks < 1L << 24, "embed_forward: too many slots");
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "embed_forward");
     with_type(table_type, [&](auto t) {
         with_type(out_type, [&](auto o) {
-            hipLaunchKernelGGL((embed_lookup_kernel<typename decltype(t)::type, typename decltype(o)::type>), dim3((unsigned)blocks),
-                               dim3(256), 0, stream, a);
+            using T = typename decltype(t)::type;
+            using O = typename decltype(o)::type;
+            auto kernel = lines ? embed_lookup_kernel<T, O, true> : embed_lookup_kernel<T, O, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
         });
     });
     CNT_HIP(hipGetLastError());
