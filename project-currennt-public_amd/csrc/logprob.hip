@@ -1083,6 +1083,8 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
 constexpr int kSpan = 64 * 32;
 // Logits of a long row that a workgroup takes at a time: 16 for every lane.
 constexpr int kChunk = 16, kRound = 256 * kChunk;
+// Bytes of a row that the largest workgroup's registers hold with its errors' work.
+constexpr int kMostHeld = 1024 * 16 * 16;
 
 // Which kernel takes the rows; measured on 32000 rows of up to 1000 logits, 20000 of 1975, 16384 of 3000 and 8192 of 10000, us:
 //   a row in registers, K rounds (HELD) against a wave that streams a row (WAVE): 500 logits, K = 8 34 / 47, 16 55 / 52, 32 96 / 66;
@@ -1117,10 +1119,10 @@ void with_lanes(int V, F f) {
     else f(integral_constant<int, 32>(), integral_constant<int, 64>());
 }
 
-// The same for a row and its errors, which have no alternatives to look for: up to twice as long in 16 bits (values and gradient of 20000 rows of 4000
-// fp16 logits 62 us, 77 by a workgroup for each; of 4001 fp32 logits 118 and 108).
+// The same for a row's values and errors, which have no alternatives to look for: up to twice as long where there are many 16-bit ones (20000 rows of
+// 4000 fp16 logits 62 us, 77 by a workgroup for each; 400 of bf16 5.9 and 5.4; 20000 of 4001 fp32 logits 118 and 108).
 template <typename T>
-constexpr int kErrorSpan = sizeof(T) == 2 ? 2 * kSpan : kSpan;
+int most_in_wave(long N) { return sizeof(T) == 2 && N >= 2048 ? 2 * kSpan : kSpan; }
 template <typename T, typename F>
 void with_error_lanes(int V, F f) {
     using std::integral_constant;
@@ -1131,6 +1133,12 @@ void with_error_lanes(int V, F f) {
         }
     }
     with_lanes(V, f);
+}
+
+// Whether a row's values and errors are shared out among workgroups, in three launches: rows that no workgroup's registers hold, and the longest of
+// very few (one of 64000 fp32 logits 8.7 us, 10.5 by one workgroup; of 32000 8.8 and 6.8; 150 of 64000 25 and 18).
+bool shared_errors(long N, int V, int type) {
+    return parts_of(N, V, 0) > 1 && (V > kMostHeld / (int)element_size(type) - 128 || (V > 48 * 1024 && N < 64));
 }
 
 size_t scratch_of(long N, int V, int K) {
@@ -1179,8 +1187,8 @@ int gradient(hipStream_t stream, int type, RowArgs &a) {
     a.parts = (int)std::min({4096L, ((1L << 26) - 4) / a.N, (a.V + 63L + kSpan - 1) / kSpan});
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        if (a.V <= kErrorSpan<T>) {
-            with_error_lanes<T>(a.V, [&](auto count, auto lanes) {
+        if (a.V <= kSpan) {
+            with_lanes(a.V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((a.N + 256 / LANES - 1) / (256 / LANES)));
                 hipLaunchKernelGGL((logprob_short_gradient_kernel<T, COUNT, LANES>), grid, dim3(256), 0, stream, a);
@@ -1281,7 +1289,7 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
     a.logp_err = logp_err; a.entropy_err = entropy_err; a.err = err; a.err_stride = err_stride;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "logprob_error_backward");
-    if (parts_of(N, V, 0) > 1) {  // few long rows: shared out among workgroups
+    if (shared_errors(N, V, type)) {
         CNT_TRY(forward(stream, type, a, scratch));
         return gradient(stream, type, a);
     }
@@ -1292,7 +1300,7 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
         // what rows may begin inside a cache line by (lead_of)
         const bool lines = reinterpret_cast<uintptr_t>(logits) % 128 == 0 && (stride * (long)sizeof(T) % 128 == 0 || N == 1);
         const int lead = lines ? 0 : 127 / (int)sizeof(T);
-        if (V <= kErrorSpan<T>) {
+        if (V <= most_in_wave<T>(N)) {
             with_error_lanes<T>(V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((N + 256 / LANES - 1) / (256 / LANES)));

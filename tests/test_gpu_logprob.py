@@ -170,7 +170,7 @@ def _check_gradients(capi, x, tokens, scale, g, h):
 
 @pytest.mark.parametrize("dtype", S.TYPES)
 @pytest.mark.parametrize("N,V", [(1, 1), (2, 5), (3, 64), (5, 255), (9, 256), (4, 257), (3, 1024), (5, 1025), (3, 2048), (2, 2049), (7, 4001), (5, 4096), (6, 4097), (3, 9001),
-                                 (1, 131072), (520, 2500), (514, 8200), (600, 20001)])
+                                 (1, 131072), (64, 50001), (520, 2500), (514, 8200), (600, 20001)])
 def test_gradient(N, V, dtype):
     rng = np.random.default_rng(N + V)
     g, h = rng.standard_normal(N).astype(np.float32), (0.3 * rng.standard_normal(N)).astype(np.float32)
@@ -178,11 +178,12 @@ def test_gradient(N, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", S.TYPES)
-@pytest.mark.parametrize("V", [2049, 2500, 4096, 4097, 4090, 8150, 16350, 30001, 60001, 65540, 100003, 131072, 140001])
-def test_gradient_of_many_long_rows(V, dtype):
-    # every form that a row of its own workgroup takes; some of the rows are checked
+@pytest.mark.parametrize("N,V", [(513, V) for V in (2049, 2500, 4096, 4097, 4090, 8150, 16350, 30001, 60001, 65540, 100003, 131072, 140001)] +
+                         [(2100, 2049), (2100, 2500), (2100, 4096), (2100, 4097)])
+def test_gradient_of_many_long_rows(N, V, dtype):
+    # every form that a row of its own wave or workgroup takes; some of the rows are checked
     capi = PC.pkg().capi
-    N, rng, some = 513, np.random.default_rng(V), [0, 1, 2, 255, 511, 512]
+    rng, some = np.random.default_rng(V), [0, 1, 2, 255, 511, N - 1]
     x = torch.randn(N, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V)).mul_(2.5).to(dtype)
     g, h = rng.standard_normal(N).astype(np.float32), (0.3 * rng.standard_normal(N)).astype(np.float32)
     t = _tokens(rng, N, V)
