@@ -3,11 +3,12 @@
 //   out[n] = scale * table[token[n]]                       (zero where slot n has no token)
 //   grad[v] = scale * sum over the slots n of token v of err[n]    (+ what grad held, if asked)
 //
-// Both move rows and are bounded by memory.  Up to 128 slots, and tables that a workgroup's few hundred slots fill well, have kernels of their own
-// (see there).  Else the gradient is formed by sorted tokens: a stable counting sort of the slots' tokens (one or
-// two passes of at most ten bits) makes a token's slots neighbours in ascending order, so a row's sum has one order, is formed in 32 bits
-// and written once, without atomics and without clearing the table first.  Tokens are as skewed as in any text: a run that covers
-// whole pieces of the sorted list is added up piece by piece by workgroups of their own first.
+// Both move rows and are bounded by memory; small gradients by launches that wait for each other.  A gradient's sums are formed in 32 bits, in an
+// order that the tokens alone determine, and every row is written once, without atomics and without clearing the table first.  Three ways:
+//   up to 128 slots: every workgroup looks for its rows' slots among all of them
+//   slabs of 512 slots, sorted and added up by a workgroup each, for small and middle tables and lists
+//   else a stable counting sort of the slots by token (one or two passes of at most ten bits, three beyond 2^20 rows), which makes a token's slots
+//   neighbours; a run that covers whole pieces of the sorted list (tokens are as skewed as in any text) is added up piece by piece first
 #include "elements.hpp"
 
 #include <algorithm>
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const SumArgs a) {
         if (first + r < a.V && bounds[r] == bounds[r + 1]) write_row<G, W>(a, (int)(first + r), c, sum);
 }
 
-// ----- few slots: no sort ---------------------------------------------------------------------------------------------------------
+// ----- few slots ---------------------------------------------------------------------------------------------------------
 // Every workgroup looks through all tokens for those of its rows, which it keeps in the order of their slots; a group of threads has kept its
 // row's errors added up in that order.  One launch: 5 slots of 708 rows 13.5 us by the sorted list.
 constexpr int kFewSlots = 128;
@@ -629,25 +630,29 @@ int sum_few(hipStream_t stream, const FewArgs &args) {
     return CNT_OK;
 }
 
-// ----- slabs of the list, each with a table of its own -----------------------------------------------------------------------------------
-// A workgroup sorts the slots of a slab that are its rows' in LDS, adds their errors up and writes its rows of the slab's table.  One slab's
-// table is the gradient itself; those of several are added up in order by a second launch.
+// ----- slabs of the list ------------------------------------------------------------------------------------------------------------------
+// A workgroup sorts the slots of a slab that belong to its rows in LDS and adds their errors up.  One slab's sums are the gradient itself; those
+// of several are left in the place of their first slot and added up, in order, by a second launch, which goes by an index of the rows' runs; or, where
+// a slab has two places for every row, in the row's (256 x 64 from 32000 slots 15.3 us, by the index 16.4; half empty, 509 x 746 from 6737 26 and 19).
+constexpr unsigned short kNoRun = 0xffff;
 constexpr int kSlab = 512, kSlabRows = 1024, kSlabWaves = kSlab / 64, kSlabLanes = 16;
 // Against the sorted list, us.  One slab: 1000 x 64 from 300 slots 6.6 / 17.0, 100000 x 64 from 500 10 / 21, 50000 x 458 from 300 22 / 28; beyond
 // 65536 x 1024 from 500 54 / 47 (the zeros, in rows of 256 bytes here).
 constexpr long kOneSlabValues = 1 << 25;
-// Several: 256 x 64 from 32000 13.8 / 21.5, 5000 x 64 from 4000 13.6 / 24.5, 1100 x 256 from 4000 15.0 / 20.2, 2000 x 64 from 16000 16.6 / 26.2; beyond 1000
-// x 512 from 2000 15.8 / 14.5, 5000 x 512 from 1000 26 / 21, 20000 x 64 from 2000 21.0 / 23.7, 100 x 2048 from 16000 41 / 37.
-constexpr long kSlabValues = 3 << 17;    // of one table
-constexpr size_t kSlabBytes = 16 << 20;  // of all
+// Several: 256 x 64 from 32000 15.3 / 22.0, 1000 x 64 from 2000 10.0 / 14.5, 1665 x 594 from 943 12.5 / 20.6, 46356 x 13 from 7743 19 / 30, 2261 x 132 from
+// 17980 18.6 / 27.6, 3992 x 1135 from 3826 24 / 29; beyond 19473 x 367 from 4492 36 / 28, 577 x 801 from 26051 44 / 36, 100 x 2048 from 16000
+// 41 / 36.
+// More errors where little is left of them: 51 x 767 from 25518 26 / 34, 20 x 512 from 30000 19 / 41.
+constexpr long kSlabValues = 1 << 24, kSlabJoined = 5 << 23, kFewJoined = 1 << 21;  // errors; values of all slabs' tables
 
 struct SlabArgs {
     const int *tokens;
     const void *err;
-    void *out;    // tables side by side, or the gradient
-    int *counts;  // entries of the slabs' rows, may be NULL
+    void *out;              // the gradient, or the runs' sums of all slabs
+    unsigned short *index;  // of several slabs: the first slot of every row's run in every slab, kNoRun where there is none
     long err_stride, out_stride;
     int N, V, D, bits, lanes, tiles, parts, accumulate, once;  // parts: workgroups that share a slab's rows
+    int dense;  // every row has its own place in a slab and needs no index
     float scale;
 };
 
@@ -713,8 +718,10 @@ __global__ __launch_bounds__(kSlab) void embed_slab_kernel(const SlabArgs a) {
     const int groups = kSlab / a.lanes, x = threadIdx.x % a.lanes, g = threadIdx.x / a.lanes;
     const Columns c = columns_of<W>((tile * a.lanes + x) * W, a.D);
     const E *err = static_cast<const E *>(a.err) + base * a.err_stride;
-    G *out = static_cast<G *>(a.out) + ((long)slab * a.V + low) * a.out_stride;
-    auto write = [&](int row, const float (&total)[W]) { put_sums(out + row * a.out_stride, c, total, a.scale, a.accumulate, a.once); };
+    auto write = [&](int row, const float (&total)[W]) {
+        const int to = a.dense ? base + low + row : a.index ? base + (int)(list[starts[row]] & 0xffff) : low + row;
+        put_sums(static_cast<G *>(a.out) + to * a.out_stride, c, total, a.scale, a.accumulate, a.once);
+    };
     const int share = (n + groups - 1) / groups, begin = min(n, g * share), end = min(n, begin + share);
     const int others = begin > 0 && begin < end && list[begin] >> 16 == list[begin - 1] >> 16 ? (int)(list[begin] >> 16) : -1;
     Vector<E, W> v[U];
@@ -754,77 +761,90 @@ __global__ __launch_bounds__(kSlab) void embed_slab_kernel(const SlabArgs a) {
         }
         write(current, sum);
     }
-    if (!a.accumulate) {
+    if (a.index ? a.dense : !a.accumulate) {
 #pragma unroll
         for (int q = 0; q < W; ++q) sum[q] = 0.0f;
 #pragma unroll 8
         for (int row = g; row < rows; row += groups)
             if (starts[row] == starts[row + 1]) write(row, sum);
     }
-    if (a.counts && tile == 0)
-        for (int row = threadIdx.x; row < rows; row += kSlab) a.counts[slab * a.V + low + row] = starts[row + 1] - starts[row];
+    if (a.index && !a.dense && tile == 0)
+        for (int row = threadIdx.x; row < rows; row += kSlab)
+            a.index[(long)slab * a.V + low + row] = starts[row] < starts[row + 1] ? (unsigned short)list[starts[row]] : kNoRun;
 }
 
-// The slabs' tables, a wave for each fourth of them.
-template <typename G>
-__global__ __launch_bounds__(256) void embed_slab_join_kernel(const float *tables, const int *counts, int slabs, int V, int D, int vectors, void *grad,
-                                                              long grad_stride, int accumulate, int once, float scale) {
-    constexpr int W = kBoth<float, G>, U = 8;
+struct JoinArgs {
+    const float *sums;
+    const unsigned short *index;
+    void *grad;
+    long grad_stride;
+    int slabs, V, D, vectors, split, dense, accumulate, once;  // vectors of a row; split: waves that share a row's slabs, 1 or 4
+    float scale;
+};
+
+// The rows' runs of all slabs, W columns per thread; U slabs in flight (5000 x 8 from 65000 slots, by sixteens 24.9 us, by
+// eights 26.0; 30000 x 128 from 1000 18.7 and 15.5).
+template <typename G, int U>
+__global__ __launch_bounds__(256) void embed_slab_join_kernel(const JoinArgs a) {
+    constexpr int W = kBoth<float, G>;
     __shared__ float sums[3][W][64];
     __shared__ int found[3][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = (slabs + 3) / 4;
-    const long i = (long)blockIdx.x * 64 + lane;
-    const int row = (int)(i / vectors);
-    Columns c = columns_of<W>((int)(i % vectors) * W, D);
-    if (row >= V) c.count = 0;
-    const int begin = min(slabs, wave * each), end = min(slabs, begin + each);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % a.split, each = (a.slabs + a.split - 1) / a.split;
+    const unsigned i = (blockIdx.x * (4 / a.split) + wave / a.split) * 64 + lane, row = i / (unsigned)a.vectors;
+    Columns c = columns_of<W>((int)(i - row * a.vectors) * W, a.D);
+    if (row >= (unsigned)a.V) c.count = 0;
+    const int begin = min(a.slabs, part * each), end = min(a.slabs, begin + each);
     float sum[W] = {};
-    int entries = 0;
+    int any = 0;
     for (int s = begin; s < end; s += U) {
+        int run[U];
         Vector<float, W> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) run[u] = s + u >= end || c.count <= 0 ? kNoRun : a.dense ? (int)row : a.index[(long)(s + u) * a.V + row];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             v[u].clear();
-            if (s + u < end && c.count > 0) v[u].load(tables + ((long)(s + u) * V + row) * D, c);
-            if (accumulate && s + u < end && c.count > 0) entries += counts[(s + u) * V + row];
+            if (run[u] != kNoRun) v[u].load(a.sums + ((long)(s + u) * kSlab + run[u]) * a.D, c);
+            any |= run[u] != kNoRun;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int q = 0; q < W; ++q) sum[q] += v[u].value(q);
     }
-    if (wave > 0) {
+    if (a.split > 1) {
+        if (wave > 0) {
 #pragma unroll
-        for (int q = 0; q < W; ++q) sums[wave - 1][q][lane] = sum[q];
-        found[wave - 1][lane] = entries;
+            for (int q = 0; q < W; ++q) sums[wave - 1][q][lane] = sum[q];
+            found[wave - 1][lane] = any;
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int o = 0; o < 3; ++o) {
+            any |= found[o][lane];
+#pragma unroll
+            for (int q = 0; q < W; ++q) sum[q] += sums[o][q][lane];
+        }
     }
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int o = 0; o < 3; ++o) {
-        entries += found[o][lane];
-#pragma unroll
-        for (int q = 0; q < W; ++q) sum[q] += sums[o][q][lane];
-    }
-    if (accumulate && entries == 0) return;
-    put_sums(static_cast<G *>(grad) + row * grad_stride, c, sum, scale, accumulate, once);
+    if (row >= (unsigned)a.V || (a.accumulate && !any)) return;
+    put_sums(static_cast<G *>(a.grad) + (long)row * a.grad_stride, c, sum, a.scale, a.accumulate, a.once);
 }
 
-// Scratch of a gradient by slabs: their tables and counts.
+// Scratch of a gradient by slabs: their runs' sums, where these are.
 struct SlabPlan {
     int slabs;  // 0: by the sorted list
-    size_t counts, bytes;
+    size_t index, bytes;
 };
 SlabPlan slab_plan(int V, int D, long N) {
     SlabPlan p = {};
     const long slabs = (N + kSlab - 1) / kSlab;
-    const long values = (long)V * D;
-    if (N <= kFewSlots || values > (slabs > 1 ? kSlabValues : kOneSlabValues)) return p;
-    if (slabs > 1 && (size_t)(slabs * values) * sizeof(float) > kSlabBytes) return p;
+    if (N <= kFewSlots) return p;
+    if (slabs > 1 ? slabs * V * D > (N * D > kSlabValues ? kFewJoined : kSlabJoined) || N * D > 2 * kSlabValues : (long)V * D > kOneSlabValues) return p;
     p.slabs = (int)slabs;
     if (slabs > 1) {
-        p.counts = (size_t)slabs * V * D * sizeof(float);
-        p.bytes = p.counts + (size_t)slabs * V * sizeof(int);
+        p.index = (size_t)slabs * kSlab * D * sizeof(float);
+        p.bytes = p.index + (size_t)slabs * V * sizeof(unsigned short);
     }
     return p;
 }
@@ -955,23 +975,26 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     }
     char *mem = static_cast<char *>(scratch);
     if (slabs.slabs == 1) {
-        SlabArgs s = {tokens, err, grad, nullptr, err_stride, grad_stride, (int)N, V, D, 0, 0, 0, 0, accumulate, once, scale};
+        SlabArgs s = {tokens, err, grad, nullptr, err_stride, grad_stride, (int)N, V, D, 0, 0, 0, 0, accumulate, once, 0, scale};
         with_type(err_type, [&](auto e) {
             with_type(grad_type, [&](auto g) { status = sum_slab<typename decltype(e)::type, typename decltype(g)::type>(stream, s, 1); });
         });
         return status;
     }
     if (slabs.slabs) {
-        int *counts = reinterpret_cast<int *>(mem + slabs.counts);
-        SlabArgs s = {tokens, err, mem, accumulate ? counts : nullptr, err_stride, D, (int)N, V, D, 0, 0, 0, 0, 0, 0, 1.0f};
+        auto *index = reinterpret_cast<unsigned short *>(mem + slabs.index);
+        const int dense = V <= kSlab / 2 && !accumulate;
+        SlabArgs s = {tokens, err, mem, index, err_stride, D, (int)N, V, D, 0, 0, 0, 0, 0, 0, dense, 1.0f};
         with_type(err_type, [&](auto e) { status = sum_slab<typename decltype(e)::type, float>(stream, s, slabs.slabs); });
         CNT_TRY(status);
         with_type(grad_type, [&](auto g) {
             using G = typename decltype(g)::type;
             constexpr int W = kBoth<float, G>;
             const int vectors = (D + W - 1) / W;
-            hipLaunchKernelGGL((embed_slab_join_kernel<G>), dim3((unsigned)(((long)V * vectors + 63) / 64)), dim3(256), 0, stream,
-                               reinterpret_cast<const float *>(mem), counts, slabs.slabs, V, D, vectors, grad, grad_stride, accumulate, (int)once, scale);
+            const long waves = ((long)V * vectors + 63) / 64;
+            JoinArgs j = {reinterpret_cast<const float *>(mem), index, grad, grad_stride, slabs.slabs, V, D, vectors, waves < 2048 ? 4 : 1, dense, accumulate, once, scale};
+            auto kernel = slabs.slabs > 8 * j.split ? embed_slab_join_kernel<G, 16> : embed_slab_join_kernel<G, 8>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((waves * j.split + 3) / 4)), dim3(256), 0, stream, j);
         });
         CNT_HIP(hipGetLastError());
         return CNT_OK;

@@ -73,7 +73,7 @@ def _check_gradient(capi, V, D, t, err_type, grad_type, rng, accumulate=False, s
 @pytest.mark.parametrize("accumulate", [False, True])
 @pytest.mark.parametrize("grad", S.TYPES)
 @pytest.mark.parametrize("err", S.TYPES)
-@pytest.mark.parametrize("V,D,N", [(1, 1, 1), (3, 5, 64), (256, 64, 3000), (1000, 130, 700), (40, 1030, 301)])
+@pytest.mark.parametrize("V,D,N", [(1, 1, 1), (3, 5, 64), (256, 64, 3000), (1000, 130, 700), (40, 1030, 301), (110000, 130, 1500)])
 def test_gradient(V, D, N, err, grad, accumulate):
     rng = np.random.default_rng(V * 7 + D)
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V), err, grad, rng, accumulate)
@@ -83,8 +83,8 @@ def test_gradient(V, D, N, err, grad, accumulate):
     (1, 3, 1024), (1, 1, 1000), (2, 300, 1023), (9, 64, 1025), (50, 7, 513), (3000, 100, 1024), (100003, 33, 1000), (20000, 1030, 300), (5, 70, 49),
     (1, 3, 5000), (2, 4, 70001), (256, 8, 66000), (1024, 5, 9001), (1025, 5, 9001), (65536, 3, 5000), (65537, 3, 5000),
     (1 << 20, 1, 3000), ((1 << 20) + 1, 1, 3000), (700, 1, 600000), (5, 2, 0), (100003, 17, 1), (64, 513, 4097),
-    (600, 300, 9000), (1024, 1030, 1500), (64, 515, 33000), (1024, 400, 2000), (1025, 400, 2000), (65536, 7, 5000), (65537, 7, 5000), (3, 140000, 1000),
-    (16400, 2051, 512)])
+    (600, 300, 9000), (1024, 1030, 1500), (64, 515, 33000), (3, 140000, 1000), (16400, 2051, 512),
+    (600, 1100, 16000), (1024, 1030, 17000), (1025, 1030, 17000), (65536, 37, 9001), (65537, 37, 9001), (1 << 20, 1, 21000), ((1 << 20) + 1, 1, 21000), (100003, 400, 600)])
 def test_gradient_sizes(V, D, N):
     rng = np.random.default_rng(N + D)
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.float32, torch.float32, rng)
@@ -110,7 +110,7 @@ def test_gradient_of_tables_that_are_filled_on_the_way(V, D, N, grad, accumulate
     _check_gradient(PC.pkg().capi, V, D, _tokens(rng, N, V, 0.02), torch.bfloat16, grad, rng, accumulate)
 
 
-@pytest.mark.parametrize("N,D", [(100, 33), (500, 33), (1000, 33), (2500, 33), (1000, 1400), (2500, 1400)])
+@pytest.mark.parametrize("N,D", [(100, 33), (500, 33), (1000, 33), (2500, 33), (1000, 1400), (2500, 6800)])
 @pytest.mark.parametrize("kind", ["none", "one", "last", "ascending", "descending", "outside"])
 def test_gradient_orders_of_tokens(kind, N, D):
     rng = np.random.default_rng(3)
@@ -122,7 +122,7 @@ def test_gradient_orders_of_tokens(kind, N, D):
     _check_gradient(PC.pkg().capi, V, D, t, torch.float32, torch.bfloat16, rng, True)
 
 
-@pytest.mark.parametrize("V,N", [(50, 70), (50, 300), (50, 700), (7000, 700)])
+@pytest.mark.parametrize("V,N", [(50, 70), (50, 300), (50, 700), (7000, 700), (330000, 700)])
 def test_gradient_rows_anywhere_and_broadcast_errors(V, N):
     capi = PC.pkg().capi
     rng = np.random.default_rng(8)
@@ -177,7 +177,7 @@ def test_gradient_against_differences():
     S.assert_close(S.f64(grad), want, S.U * (count[:, None] + 1.0) * size + 1e-12)
 
 
-@pytest.mark.parametrize("V,N", [(500, 100), (500, 400), (500, 4000), (9000, 4000)])
+@pytest.mark.parametrize("V,N", [(500, 100), (500, 400), (500, 4000), (9000, 4000), (120000, 4000)])
 def test_on_another_stream_and_replayed_from_a_graph(V, N):
     capi = PC.pkg().capi
     rng = np.random.default_rng(5)
