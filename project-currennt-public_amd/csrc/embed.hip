@@ -644,6 +644,7 @@ constexpr long kOneSlabValues = 1 << 25;
 // 41 / 36.
 // More errors where little is left of them: 51 x 767 from 25518 26 / 34, 20 x 512 from 30000 19 / 41.
 constexpr long kSlabValues = 1 << 24, kSlabJoined = 5 << 23, kFewJoined = 1 << 21;  // errors; values of all slabs' tables
+constexpr int kMostSlabs = 512;  // (31 x 8 from 260000 41 / 42, from 1000000 141 / 72)
 
 struct SlabArgs {
     const int *tokens;
@@ -840,6 +841,7 @@ SlabPlan slab_plan(int V, int D, long N) {
     SlabPlan p = {};
     const long slabs = (N + kSlab - 1) / kSlab;
     if (N <= kFewSlots) return p;
+    if (slabs > kMostSlabs) return p;
     if (slabs > 1 ? slabs * V * D > (N * D > kSlabValues ? kFewJoined : kSlabJoined) || N * D > 2 * kSlabValues : (long)V * D > kOneSlabValues) return p;
     p.slabs = (int)slabs;
     if (slabs > 1) {
@@ -992,7 +994,8 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
             constexpr int W = kBoth<float, G>;
             const int vectors = (D + W - 1) / W;
             const long waves = ((long)V * vectors + 63) / 64;
-            JoinArgs j = {reinterpret_cast<const float *>(mem), index, grad, grad_stride, slabs.slabs, V, D, vectors, waves < 2048 ? 4 : 1, dense, accumulate, once, scale};
+            JoinArgs j = {reinterpret_cast<const float *>(mem), index, grad, grad_stride, slabs.slabs, V, D, vectors, waves < 2048 ? 4 : 1, dense,
+                          accumulate, once, scale};
             auto kernel = slabs.slabs > 8 * j.split ? embed_slab_join_kernel<G, 16> : embed_slab_join_kernel<G, 8>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)((waves * j.split + 3) / 4)), dim3(256), 0, stream, j);
         });
