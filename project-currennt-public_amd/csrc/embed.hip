@@ -4,7 +4,7 @@
 //   grad[v] = scale * sum over the slots n of token v of err[n]    (+ what grad held, if asked)
 //
 // Both move rows and are bounded by memory; small gradients by launches that wait for each other.  A gradient's sums are formed in 32 bits, in an
-// order that the tokens alone determine, and every row is written once, without atomics and without clearing the table first.  Three ways:
+// order that the tokens alone determine, without atomics and without clearing the table first.  Three ways:
 //   up to 128 slots: every workgroup looks for its rows' slots among all of them
 //   slabs of 512 slots, sorted and added up by a workgroup each, for small and middle tables and lists
 //   else a stable counting sort of the slots by token (one or two passes of at most ten bits, three beyond 2^20 rows), which makes a token's slots
@@ -300,9 +300,9 @@ __global__ __launch_bounds__(kSortThreads) void token_place_kernel(const SortArg
     }
 }
 
-// Whether rows of the gradient are written past the caches: rows of whole lines (53665 of 512 fp32 zeros 21 us, 22.5 through the caches), and
-// tables that the last-level cache has no room for (65536 rows of 1000 from 16384 slots 75 us and 97).  Other rows share lines, which are written twice
-// past the caches (53665 of 458: 27 us, 20 through them).
+// Whether rows of the gradient are written past the caches: rows of whole lines (53665 of 512 fp32 zeros 21.1 us, 21.8 through the caches), and tables
+// that the last-level cache has no room for (65536 rows of 1000 from 16384 slots 76 us and 86).  Other rows share lines, which are written twice
+// past the caches (53665 of 458: 28 us, 17 through them).
 inline bool past_caches(const void *grad, int V, int D, long stride, int type) {
     const long row = stride * (long)element_size(type);
     return (reinterpret_cast<uintptr_t>(grad) % 128 == 0 && row % 128 == 0) || V * (long)D * (long)element_size(type) > 128L << 20;
@@ -885,7 +885,7 @@ int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
     {
         constexpr int W = kWide<E>;
         share_columns(a, W);
-        // Few entries for the rows: gaps of hundreds of rows are not left to a wave each (10 slots of 41140 rows: 32 us for the gradient).
+        // Few entries for the rows: gaps of hundreds of rows are not left to a wave each (100003 x 400 from 600 slots: 65 us for the gradient, 36 so).
         a.searched = a.V / 4 > N;
         a.first_blocks = (int)((a.searched ? a.V : N) / 256 + 1);
         a.pieces = (int)pieces;
@@ -895,9 +895,8 @@ int sum_runs(hipStream_t stream, const SumArgs &args, long N) {
     }
     constexpr int W = kBoth<E, G>;
     share_columns(a, W);
-    // Few rows: a group's time is that of one run, and no rows are left to go through for their zeros (256 rows of 64, 32000 slots: 6.5 us
-    // for this launch, 10.6 by windows of the list).  Many rows: most are without entries, and the runs' groups are those of the list (65536 rows of
-    // 1024, 16384 slots: 32 us, 36 by rows).
+    // Few rows: a group's time is that of one run, and no rows are left to go through for their zeros (577 x 801 from 26051 slots 36 us, 41 by windows of
+    // the list).  Many rows: most are without entries, and the runs' groups are those of the list (65536 x 1024 from 16384 67 us, 96 by rows).
     a.by_rows = a.V <= N;
     const long groups = 256 / a.lanes, windows = a.by_rows ? 0 : (N + kWindow - 1) / kWindow;
     const long others = a.by_rows ? a.V : a.accumulate ? 0 : (a.V - a.filled + kZeroRows - 1) / kZeroRows;
