@@ -132,7 +132,7 @@ int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const 
 /* The table's gradient: grad[v] = scale * sum of err[n] over the slots n with tokens[n] = v, for all V rows (rows of zeros where
  * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
  * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
- * cnt_embed_scratch(V, D, N) bytes (0 for some sizes: NULL then), aligned to 16, with any content, which the call has for itself until it has run (two captured
+ * cnt_embed_scratch(V, D, N) bytes (enough for fewer slots as well), aligned to 16, with any content, which the call has for itself until it has run (two captured
  * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^33. */
 long cnt_embed_scratch(int V, int D, long N);
 int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
@@ -150,8 +150,8 @@ int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, fl
  * A logit of -inf is a token that is ruled out: its p is 0.  A row with nothing else has lse = -inf, logp = -inf, entropy 0 and the
  * tokens 0 .. K-1 as alternatives.  A row with a NaN or +inf has NaN in lse, logp, entropy and top_logp; NaN logits are never among the
  * alternatives (token -1 where fewer than K are left).  Any result may be NULL; K is 0 .. 64 and <= V.  N < 2^24, V <= 2^30.
- * scratch: device memory of cnt_logprob_scratch(N, V, K) bytes (0 for most sizes: NULL then), any content, the call's own until
- * it has run. */
+ * scratch: device memory of cnt_logprob_scratch(N, V, K) bytes (0 for most sizes: NULL then; fewer rows may need more, never more
+ * than 20 + 13 * K KB), any content, the call's own until it has run. */
 long cnt_logprob_scratch(long N, int V, int K);
 int cnt_logprob_forward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
                         float *logp, float *lse, float *entropy, int K, float *top_logp, int *top_tokens, void *scratch,

@@ -537,7 +537,7 @@ def embed_forward(table, tokens, out, scale=1.0, stream=None):
 
 
 def embed_scratch(V, D, N):
-    """Bytes of scratch memory that embed_backward needs."""
+    """Bytes of scratch memory that embed_backward needs for N slots or fewer."""
     need = lib().cnt_embed_scratch(V, D, N)
     if need < 0:
         raise ValueError("sizes out of range")

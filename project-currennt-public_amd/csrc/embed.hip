@@ -104,7 +104,7 @@ constexpr long kCountedTwice = 32768;
 constexpr int kFillVectors = 4;
 constexpr size_t kFillFrom = 16 << 20, kFillBytes = 48 << 20;  // tables that are filled on the way, bytes per launch
 
-// Scratch of a gradient: two lists of (token, slot), counts of every block and digit, the number of slots with a token, where the rows' runs
+// Scratch of a gradient, which is enough for shorter lists as well: two lists of (token, slot), counts of every block and digit, the number of slots with a token, where the rows' runs
 // begin, partial sums.
 struct SortPlan {
     int bits, passes, block, blocks, piece;  // slots per block, blocks; piece: entries of the sorted list that are added up together
@@ -132,10 +132,11 @@ SortPlan sort_plan(long V, int D, long N) {
     const size_t list = (size_t)N * sizeof(int);
     p.keys[0] = take(list); p.slots[0] = take(list);
     p.keys[1] = p.passes > 1 ? take(list) : 0; p.slots[1] = p.passes > 1 ? take(list) : 0;
-    p.counts = take(p.counted ? (size_t)p.blocks * (1 << p.bits) * sizeof(int) : 0);
+    p.counts = take(p.counted ? (size_t)std::min<long>(kMostSortBlocks, (N + kSortThreads - 1) / kSortThreads) * (1 << p.bits) * sizeof(int) : 0);
     p.total = take(sizeof(int));
     p.starts = take(((size_t)V + 1) * sizeof(int));
-    p.partial = take((size_t)(N / p.piece) * D * sizeof(float));
+    // (a list that has pieces of half the length has up to 64 p^2 entries in them, p being that half)
+    p.partial = take((size_t)std::max(N / p.piece, p.piece > 32 ? 32L * p.piece : 0L) * D * sizeof(float));
     p.bytes = at;
     return p;
 }
@@ -835,7 +836,7 @@ __global__ __launch_bounds__(256) void embed_slab_join_kernel(const JoinArgs a) 
 // Scratch of a gradient by slabs: their runs' sums, where these are.
 struct SlabPlan {
     int slabs;  // 0: by the sorted list
-    size_t index, bytes;
+    size_t index;
 };
 SlabPlan slab_plan(int V, int D, long N) {
     SlabPlan p = {};
@@ -844,11 +845,14 @@ SlabPlan slab_plan(int V, int D, long N) {
     if (slabs > kMostSlabs) return p;
     if (slabs > 1 ? slabs * V * D > (N * D > kSlabValues ? kFewJoined : kSlabJoined) || N * D > 2 * kSlabValues : (long)V * D > kOneSlabValues) return p;
     p.slabs = (int)slabs;
-    if (slabs > 1) {
-        p.index = (size_t)slabs * kSlab * D * sizeof(float);
-        p.bytes = p.index + (size_t)slabs * V * sizeof(unsigned short);
-    }
+    p.index = (size_t)slabs * kSlab * D * sizeof(float);
     return p;
+}
+
+size_t gradient_scratch(int V, int D, long N) {
+    // as many slabs as this list or a shorter one may have
+    const long slabs = std::min({(N + kSlab - 1) / kSlab, (long)kMostSlabs, kSlabJoined / ((long)V * D), 2 * kSlabValues / D / kSlab + 1});
+    return std::max(sort_plan(V, D, N).bytes, slabs > 1 ? (size_t)slabs * (kSlab * (size_t)D * sizeof(float) + V * sizeof(unsigned short)) : 0);
 }
 
 template <typename E, typename G>
@@ -945,8 +949,7 @@ int cnt_embed_forward(void *stream_, int V, int D, long N, int table_type, const
 
 long cnt_embed_scratch(int V, int D, long N) {
     if (!cnt::gradient_sizes(V, D, N)) return -1;
-    const cnt::SlabPlan slabs = cnt::slab_plan(V, D, N);
-    return (long)(slabs.slabs ? slabs.bytes : cnt::sort_plan(V, D, N).bytes);
+    return (long)cnt::gradient_scratch(V, D, N);
 }
 
 int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
@@ -959,8 +962,8 @@ int cnt_embed_backward(void *stream_, int V, int D, long N, const int *tokens, f
     CNT_REQUIRE(std::isfinite(scale), "embed_backward: the scale has to be finite");
     const SlabPlan slabs = slab_plan(V, D, N);
     const SortPlan plan = sort_plan(V, D, N);
-    const size_t need = slabs.slabs ? slabs.bytes : plan.bytes;
-    CNT_REQUIRE(grad && (scratch || need == 0) && (N == 0 || (tokens && err)), "embed_backward: null argument");
+    const size_t need = gradient_scratch(V, D, N);
+    CNT_REQUIRE(grad && scratch && (N == 0 || (tokens && err)), "embed_backward: null argument");
     CNT_REQUIRE(scratch_bytes >= need, "embed_backward: %zu bytes of scratch memory, %zu are needed", scratch_bytes, need);
     CNT_REQUIRE(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embed_backward: the scratch memory is not aligned to 16 bytes");
     hipStream_t stream = static_cast<hipStream_t>(stream_);

@@ -138,6 +138,20 @@ def test_gradient_rows_anywhere_and_broadcast_errors(V, N):
             assert torch.all(place[:, :1] == 3.0) and torch.all(place[:, 66:] == 3.0) and torch.all(scratch[-512:] == 0xAB)
 
 
+@pytest.mark.parametrize("V,D", [(300, 40), (9000, 700)])
+def test_scratch_of_the_longest_list_serves_the_others(V, D):
+    capi = PC.pkg().capi
+    rng = np.random.default_rng(6)
+    e = _dev(rng.standard_normal((20000, D)).astype(np.float32))
+    scratch = torch.full((capi.embed_scratch(V, D, 20000) + 512,), 0xAB, dtype=torch.uint8, device="cuda")
+    for N in (20000, 9000, 3000, 600, 300, 100):
+        t, grad = _tokens(rng, N, V), torch.empty(V, D, device="cuda")
+        capi.embed_backward(_dev(t), e[:N], grad, scratch=scratch[:-512])
+        want, size, count = S.embed_grad(t, S.f64(e[:N]), V, 1.0)
+        S.assert_close(S.f64(grad), want, S.U * (count[:, None] + 1.0) * size)
+        assert torch.all(scratch[-512:] == 0xAB)
+
+
 def test_more_than_two_to_the_31_values():
     # rows whose addresses are beyond 32 bits
     capi = PC.pkg().capi

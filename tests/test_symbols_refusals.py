@@ -52,6 +52,22 @@ def test_embedding_scales():
         _refused(L.cnt_embed_backward(None, 4, 4, 2, P, scale, 0, P, 4, 0, P, 4, 0, P, 2 ** 20), "finite")
 
 
+@pytest.mark.parametrize("V,D", [(1, 1), (31, 8), (256, 64), (1000, 130), (5000, 64), (46356, 13), (1 << 20, 1), (577, 801), (33005, 1602), (3, 140000)])
+def test_scratch_serves_fewer_slots(V, D):
+    # a caller keeps what its longest fraction needs
+    L = load_package().capi.lib()
+    sizes = sorted({n + d for k in range(1, 21) for n in (1 << k, 3 << k, 64 * k * k, 512 * k, 4096 * k) for d in (-1, 0, 1)} | {0, 524288, 524289, 1 << 20})
+    needs = [L.cnt_embed_scratch(V, D, n) for n in sizes if n * D <= 2 ** 33]
+    assert needs == sorted(needs) and needs[0] >= 0
+
+
+def test_scratch_of_shared_rows_is_bounded():
+    L = load_package().capi.lib()
+    for K in (0, 1, 2, 8, 31, 64):
+        for V in (2049, 5000, 40000, 131072, 1000000, 1 << 30):
+            assert all(0 <= L.cnt_logprob_scratch(n, V, K) <= (20 + 13 * K) * 1024 for n in range(0, 600))
+
+
 def test_sizes_that_no_launch_takes():
     L = load_package().capi.lib()
     _refused(L.cnt_embed_forward(None, 4, 2 ** 30 + 1, 2, 0, P, 2 ** 31, P, 1.0, 0, P, 2 ** 31), "sizes")
