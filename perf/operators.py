@@ -13,7 +13,6 @@ A case is a dict of plain values with an `op`:
 Tokens follow the usual skewed distribution (token k about as often as 1 / (k + 1)); a fiftieth of the slots holds no token (-1), as
 the padding behind a fraction's shorter sequences does.
 """
-import functools
 import importlib
 import math
 
@@ -25,7 +24,6 @@ TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 
 
-@functools.lru_cache(maxsize=None)
 def _capi():
     return importlib.import_module("project-currennt-public_amd").capi
 
