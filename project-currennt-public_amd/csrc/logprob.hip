@@ -30,7 +30,7 @@ struct RowArgs {
     float scale;
     float *logp, *lse, *entropy, *top_logp;
     int *top_tokens;
-    float *part_stats, *part_values;  // of a shared row: three statistics, K values, K tokens per part
+    float *part_stats, *part_values;  // of a shared row: three statistics, K values, K tokens per part; joined: maximum and log s in the first part's place
     int *part_tokens;
     const float *logp_err, *entropy_err;
     void *err;
@@ -746,7 +746,12 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const RowArgs a) {
     const Given given = given_logit(static_cast<const T *>(a.logits) + n * a.stride, given_one);
     s = join_lanes(s, c);
     const float log_s = logf(s.s);
-    if (lane == 0) write_stats(a, n, given, s, log_s);
+    if (lane == 0) {
+        write_stats(a, n, given, s, log_s);
+        // for the errors of the joint call (all lanes' statistics have been read: they are in these two)
+        a.part_stats[p * 3] = s.m;
+        a.part_stats[p * 3 + 1] = log_s;
+    }
     if (a.K == 0) return;
     unsigned key[Q];
 #pragma unroll
@@ -775,6 +780,7 @@ struct Slopes {
     float first, second, given;
     int token;
 };
+// (lse: what the row's log sum says of it, NaN: no numbers, -inf: nothing to choose from)
 __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse, float entropy) {
     int token = a.tokens ? a.tokens[n] : -1;
     if (token >= a.V || token < 0) token = -1;
@@ -826,8 +832,10 @@ __device__ __forceinline__ void put_gradient(T *row, int begin, int end, int lan
 // From saved statistics, `parts` waves for a row, neighbouring ones for neighbouring stretches (rows of 32000 16-bit logits dealt row by row
 // instead: 75 us for 3001; workgroups that have one row each: 55 us for
 // 6517 of 9819, 47 so).  A wave has one chunk but in very long rows.
-template <typename T, int NV>
-__global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) {
+// JOINED: the rows of a joint call that are shared out, from their maximum and log s apart, as the other forms of that call have them: rows far from zero
+// have a log sum that 32 bits round by more than its logits differ (a row of the type's lowest value: p = 1 for 1 / V).
+template <typename T, int NV, bool JOINED>
+__global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a, int forward_parts) {
     constexpr int SPAN = Chunk<T, NV>::SPAN, W = kWide<T>;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned id = blockIdx.x * 4 + wave;
@@ -836,9 +844,11 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) 
     if (n >= a.N) return;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
-    auto errors = [&](float (&t)[W], int at, float ref, const Slopes &s) {
+    const float *joined = JOINED ? a.part_stats + n * forward_parts * 3 : nullptr;
+    const float c = a.scale * kLog2e;
+    auto errors = [&](float (&t)[W], int at, float ref, float log2_s, const Slopes &s) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) t[i] = __builtin_fmaf(t[i], a.scale, -ref) * kLog2e;
+        for (int i = 0; i < W; ++i) t[i] = JOINED ? (t[i] - ref) * c - log2_s : __builtin_fmaf(t[i], a.scale, -ref) * kLog2e;
         errors_of<W>(at, s, t);
     };
     for (int at = stretch * SPAN - lead_of(row); at < a.V; at += a.parts * SPAN) {
@@ -846,14 +856,15 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a) 
         RawChunk<T, NV> x;  // (asked for in front of the row's values)
         if (whole) x.load(row + at, lane);
         else x.template load_within<true>(row, at, a.V, lane);
-        const float lse = a.lse[n], ref = lse == kMinusInfinity ? 0.0f : lse;
-        const Slopes s = slopes_of(a, n, lse, a.entropy ? a.entropy[n] : 0.0f);
+        // JOINED: log s is -inf where all logits are, and NaN where the log sum is
+        const float base = JOINED ? joined[0] : a.lse[n], log_s = JOINED ? joined[1] : base, ref = base == kMinusInfinity ? 0.0f : base;
+        const Slopes s = slopes_of(a, n, log_s, a.entropy ? a.entropy[n] : 0.0f);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int first = at + (j * 64 + lane) * W;
             float t[W];
             x.part[j].template values<0>(t);
-            errors(t, first, ref, s);
+            errors(t, first, ref, log_s * kLog2e, s);
             if (whole) put_elements<T, W, true>(to + first, t);
             else put_within(to, first, a.V, t);
         }
@@ -1183,11 +1194,12 @@ int forward(hipStream_t stream, int type, RowArgs &a, void *scratch) {
     return CNT_OK;
 }
 
-int gradient(hipStream_t stream, int type, RowArgs &a) {
+// forward_parts: of a joint call, the parts of a row whose statistics the forward launches have left in scratch; else 0
+int gradient(hipStream_t stream, int type, RowArgs &a, int forward_parts) {
     a.parts = (int)std::min({4096L, ((1L << 26) - 4) / a.N, (a.V + 63L + kSpan - 1) / kSpan});
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;
-        if (a.V <= kSpan) {
+        if (a.V <= kSpan) {  // (none of a joint call's shared rows)
             with_lanes(a.V, [&](auto count, auto lanes) {
                 constexpr int COUNT = decltype(count)::value, LANES = decltype(lanes)::value;
                 const dim3 grid((unsigned)((a.N + 256 / LANES - 1) / (256 / LANES)));
@@ -1195,7 +1207,8 @@ int gradient(hipStream_t stream, int type, RowArgs &a) {
             });
             return;
         }
-        hipLaunchKernelGGL((logprob_gradient_kernel<T, 32 / kWide<T>>), dim3((unsigned)((a.N * a.parts + 3) / 4)), dim3(256), 0, stream, a);
+        auto kernel = forward_parts ? logprob_gradient_kernel<T, 32 / kWide<T>, true> : logprob_gradient_kernel<T, 32 / kWide<T>, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.N * a.parts + 3) / 4)), dim3(256), 0, stream, a, forward_parts);
     });
     CNT_HIP(hipGetLastError());
     return CNT_OK;
@@ -1270,7 +1283,7 @@ int cnt_logprob_backward(void *stream_, long N, int V, int type, const void *log
     a.lse = const_cast<float *>(lse); a.entropy = const_cast<float *>(entropy);
     a.logp_err = logp_err; a.entropy_err = entropy_err; a.err = err; a.err_stride = err_stride;
     ProfileScope prof(static_cast<hipStream_t>(stream_), "logprob_backward");
-    return gradient(static_cast<hipStream_t>(stream_), type, a);
+    return gradient(static_cast<hipStream_t>(stream_), type, a, 0);
 }
 
 int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
@@ -1291,7 +1304,7 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
     ProfileScope prof(stream, "logprob_error_backward");
     if (shared_errors(N, V, type)) {
         CNT_TRY(forward(stream, type, a, scratch));
-        return gradient(stream, type, a);
+        return gradient(stream, type, a, a.parts);
     }
     with_type(type, [&](auto t) {
         using T = typename decltype(t)::type;

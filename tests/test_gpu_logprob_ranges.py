@@ -1,0 +1,71 @@
+"""Log probabilities and their gradients at the ends of what calls may ask for, in every form that a row's length and the number of rows choose:
+masks between ordinary logits and the type's lowest value, scales far from 1, rows far from zero.  Against 64 bits (through the C ABI)."""
+import numpy as np
+import pytest
+import torch
+
+import parity_cases as PC
+import symbols as S
+
+pytestmark = pytest.mark.gpu
+
+ROWS = 6
+# a V for each form: 16 lanes, a wave, a workgroup of growing size, shared or read twice (the last two: by the number of rows and their type)
+LENGTHS = [300, 1500, 3000, 9001, 30001, 70001, 140001]
+# a few rows, many
+TIMES = [1, 88]
+
+
+def _dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+def _joint(x, tokens, g, h, scale, times):
+    """Results of the joint call for `times` copies of the rows: those of the first, of a middle and of the last copy."""
+    N, V = x.shape
+    many = x.repeat(times, 1)
+    f = [torch.full((N * times,), 7.0, device="cuda") for _ in range(3)]
+    err = torch.full_like(many, 7.0)
+    tile = lambda a: _dev(np.tile(a, times))
+    PC.pkg().capi.logprob_error_backward(many, tile(tokens), tile(g), tile(h), *f, err, scale=scale)
+    return [[t[N * k:N * k + N] for t in f + [err]] for k in sorted({0, times // 2, times - 1})]
+
+
+def _check_joint(x, tokens, g, h, scale, times):
+    scale = float(np.float32(scale))
+    R = S.Rows(S.f64(x), scale)
+    want, tol = R.gradient(tokens, g.astype(np.float64), h.astype(np.float64), False)
+    # probabilities below 2^-126 may be flushed to zero: at most |log p| = 90 then, in front of which stand the scale and the errors
+    tol = tol + S.TINY[torch.float32] * scale * (np.abs(g) + np.abs(h) * (90 + np.where(R.bad, 0.0, R.entropy)))[:, None]
+    rows = np.arange(len(tokens))
+    held = (tokens >= 0) & (tokens < x.shape[1])
+    at = np.where(held, tokens, 0)
+    with np.errstate(over="ignore"):
+        lse = R.lse.astype(np.float32)  # infinite where 32 bits cannot hold it
+    for logp, got_lse, entropy, err in _joint(x, tokens, g, h, scale, times):
+        S.assert_close(S.f64(err), want, tol, x.dtype)
+        S.assert_close(S.f64(entropy), R.entropy, R.tol_entropy)
+        S.assert_close(S.f64(logp), np.where(held, R.logp[rows, at], 0.0), np.where(held, R.tol_logp[rows, at], 0.0))
+        S.assert_close(S.f64(got_lse), lse, R.tol_lse)
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("V", LENGTHS)
+def test_gradient_of_rows_far_from_zero(V, times, dtype):
+    """The joint call's probabilities come from the row's maximum: what 32 bits of the log sum cannot hold does not reach them."""
+    rng = np.random.default_rng(V + 1)
+    x = rng.standard_normal((ROWS, V)) * 2.5
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x[0] = low
+    x[1] += 1e4
+    x[2] -= 1e4
+    x[3] = low
+    x[3, 5] = -3.0
+    x[4] = high
+    x[5] = low
+    x[5, V // 3:V // 2] = -np.inf
+    tokens = np.array([1, 2, V - 1, 5, -1, V - 2], np.int32)
+    g, h = np.array([1.0, -1.0, 0.5, 1.0, 1.0, 2.0], np.float32), np.array([0.5, 1.0, -1.0, 0.0, 2.0, 0.5], np.float32)
+    _check_joint(_dev(x, dtype), tokens, g, h, 1.0, times)
