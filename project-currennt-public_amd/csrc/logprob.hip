@@ -1029,7 +1029,9 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
     // 16-bit errors take log2 p = x * c - z from one operation: below 64 z is rounded by 2^-18, the results by 2^-9 or 2^-12
     const float z = r + (log2_s + off);
     const int holder = (slopes.token + lead) / (THREADS * W);
-    for_vectors(std::integral_constant<int, 3>(), !ruled_out && (sizeof(T) == 4 || (fused && fabsf(z) <= 64.0f)),
+    // second * t, which has no bound on t here, has to be a number where the probability is 0: far masks, large scales, large errors
+    const bool numbers = __ballot(!(fabsf(slopes.second) * ((ref - low) * c + log2_s) < 1e38f)) == 0;
+    for_vectors(std::integral_constant<int, 3>(), !ruled_out && numbers && (sizeof(T) == 4 || (fused && fabsf(z) <= 64.0f)),
         [&](int j, int at, float (&t)[W]) {
 #pragma unroll
             for (int i = 0; i < W; ++i) {

@@ -50,6 +50,30 @@ def _check_joint(x, tokens, g, h, scale, times):
         S.assert_close(S.f64(got_lse), lse, R.tol_lse)
 
 
+# scale, value of the mask, error of the entropies
+VANISHING = [(1.0, -1e33, 1e6), (1.0, -1e36, 65536.0), (1.0, -1e37, 100.0), (1.0, -5e37, 7.0), (1.0, -7e37, 1e4), (1e19, -1e18, 10.0), (1e20, -30.0, 1.0),
+             (1e30, -30.0, 1e4)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,times", [(V, times) for V in LENGTHS for times in TIMES] + [(3000, 350)])
+def test_gradient_where_probabilities_vanish(V, times, dtype):
+    """A probability of 0 makes an error of 0, however large the logarithm and what stands in front of it."""
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((ROWS, V)) * 2.5
+    masked = rng.random((ROWS, V)) < 0.1
+    masked[:, 7] = False
+    masked[2] = np.arange(V) != 7      # one token left
+    masked[3] = np.arange(V) >= V // 2
+    masked[4] = False
+    masked[4, V - 5] = True            # one ruled out
+    tokens = np.array([7, -1, 7, 3, V - 5, 9], np.int32)
+    g = np.array([1.0, 1.0, -2.0, 0.0, 3.0, -1.0], np.float32)
+    for scale, low, error in VANISHING:
+        h = np.array([1.0, -1.0, 0.5, 1.0, -1.0, 1.0], np.float32) * np.float32(error)
+        _check_joint(_dev(np.where(masked, low, x), dtype), tokens, g, h, scale, times)
+
+
 @pytest.mark.parametrize("dtype", S.TYPES)
 @pytest.mark.parametrize("times", TIMES)
 @pytest.mark.parametrize("V", LENGTHS)
