@@ -780,8 +780,9 @@ struct Slopes {
     float first, second, given;
     int token;
 };
-// (lse: what the row's log sum says of it, NaN: no numbers, -inf: nothing to choose from)
-__device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse, float entropy) {
+// sum: log s of a row, or its saved log sum: -inf where there is nothing to choose from, NaN where there are no numbers.  (The log sum of a
+// row whose maximum is known says neither: it may be beyond 32 bits.)
+__device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float sum, float entropy) {
     int token = a.tokens ? a.tokens[n] : -1;
     if (token >= a.V || token < 0) token = -1;
     const float error = a.logp_err ? a.logp_err[n] : 0.0f;  // (not waiting for the token)
@@ -790,8 +791,8 @@ __device__ __forceinline__ Slopes slopes_of(const RowArgs &a, long n, float lse,
     s.first = -a.scale * (h == 0.0f ? g : g + h * entropy);
     s.second = -a.scale * h * kLn2;
     s.given = a.scale * g;
-    s.token = lse == kMinusInfinity ? -1 : token;  // nothing to choose from: no gradient
-    if (lse != lse) s.first = lse;
+    s.token = sum == kMinusInfinity ? -1 : token;  // nothing to choose from: no gradient
+    if (sum != sum) s.first = sum;
     return s;
 }
 // the given token's own error, if it is one of W from logit `at` on
@@ -856,15 +857,14 @@ __global__ __launch_bounds__(256) void logprob_gradient_kernel(const RowArgs a, 
         RawChunk<T, NV> x;  // (asked for in front of the row's values)
         if (whole) x.load(row + at, lane);
         else x.template load_within<true>(row, at, a.V, lane);
-        // JOINED: log s is -inf where all logits are, and NaN where the log sum is
-        const float base = JOINED ? joined[0] : a.lse[n], log_s = JOINED ? joined[1] : base, ref = base == kMinusInfinity ? 0.0f : base;
-        const Slopes s = slopes_of(a, n, log_s, a.entropy ? a.entropy[n] : 0.0f);
+        const float base = JOINED ? joined[0] : a.lse[n], sum = JOINED ? joined[1] : base, ref = base == kMinusInfinity ? 0.0f : base;
+        const Slopes s = slopes_of(a, n, sum, a.entropy ? a.entropy[n] : 0.0f);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int first = at + (j * 64 + lane) * W;
             float t[W];
             x.part[j].template values<0>(t);
-            errors(t, first, ref, log_s * kLog2e, s);
+            errors(t, first, ref, sum * kLog2e, s);
             if (whole) put_elements<T, W, true>(to + first, t);
             else put_within(to, first, a.V, t);
         }
@@ -910,7 +910,7 @@ __global__ __launch_bounds__(256) void logprob_short_error_kernel(const RowArgs 
     if (!here) return;
     const float log_s = logf(s.s), log2_s = log_s * kLog2e;
     if (l == 0) write_stats(a, n, given, s, log_s);
-    const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
+    const Slopes slopes = slopes_of(a, n, log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
     T *to = static_cast<T *>(a.err) + n * a.err_stride;
 #pragma unroll
@@ -1025,7 +1025,7 @@ __global__ __launch_bounds__(THREADS, GROUPS * THREADS / 256) void logprob_held_
         a.lse[n] = lse;
         a.entropy[n] = entropy;
     }
-    const Slopes slopes = slopes_of(a, n, lse, entropy);
+    const Slopes slopes = slopes_of(a, n, log_s, entropy);
     // 16-bit errors take log2 p = x * c - z from one operation: below 64 z is rounded by 2^-18, the results by 2^-9 or 2^-12
     const float z = r + (log2_s + off);
     const int holder = (slopes.token + lead) / (THREADS * W);
@@ -1081,7 +1081,7 @@ __global__ __launch_bounds__(1024) void logprob_long_error_kernel(const RowArgs 
     const float log_s = logf(s.s), log2_s = log_s * kLog2e;
     if (threadIdx.x == 0) write_stats(a, n, given, s, log_s);
     __syncthreads();  // the errors may take the logits' place: the given token's logit has been read
-    const Slopes slopes = slopes_of(a, n, s.m * a.scale + log_s, entropy_of(s, log_s));
+    const Slopes slopes = slopes_of(a, n, log_s, entropy_of(s, log_s));
     const float ref = s.m == kMinusInfinity ? 0.0f : s.m;
     for (int at = wave * SPAN - lead_of(row); at < a.V; at += WAVES * SPAN) {
         load_chunk<true>(row, at, a.V, lane, x);

@@ -93,3 +93,23 @@ def test_gradient_of_rows_far_from_zero(V, times, dtype):
     tokens = np.array([1, 2, V - 1, 5, -1, V - 2], np.int32)
     g, h = np.array([1.0, -1.0, 0.5, 1.0, 1.0, 2.0], np.float32), np.array([0.5, 1.0, -1.0, 0.0, 2.0, 0.5], np.float32)
     _check_joint(_dev(x, dtype), tokens, g, h, 1.0, times)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("V", LENGTHS)
+def test_gradient_of_rows_whose_log_sum_is_beyond_32_bits(V, times, dtype):
+    """A row is without choices if all of its logits are -inf, not if its log sum is -inf in 32 bits."""
+    x = np.zeros((ROWS, V))
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x[0] = low
+    x[1] = low
+    x[1, 4:V - 3] = -np.inf
+    x[2] = high
+    x[3] = -np.inf
+    x[4] = low
+    x[4, 7] = 0.5 * low
+    tokens = np.array([1, 2, V - 1, 5, 7, 2], np.int32)
+    g, h = np.array([1.0, -1.0, 0.5, 1.0, 2.0, 1.0], np.float32), np.array([0.5, 1.0, -1.0, 1.0, 2.0, 0.0], np.float32)
+    for scale in (1.5, 64.0, 1e30):
+        _check_joint(_dev(x, dtype), tokens, g, h, scale, times)
