@@ -159,12 +159,15 @@ int cnt_logprob_forward(void *stream, long N, int V, int type, const void *logit
 /* Errors of the logits from the errors of logp and entropy (either may be NULL: zeros):
  *   err[v] = scale * (logp_err[n] * ([v = t] - p_v) - entropy_err[n] * p_v * (log p_v + entropy[n]))
  * with the lse and entropy of the forward call, in the logits' type (rows err_stride apart).  err may be the logits themselves, with the
- * same stride, and overlaps them in no other way (CNT_ERR_ARG).  Rows where everything is ruled out get zeros, slots without a symbol the entropy's part alone. */
+ * same stride, and overlaps them in no other way (CNT_ERR_ARG).  Rows where everything is ruled out get zeros, slots without a symbol the entropy's part alone.
+ * scale * logp_err and scale * entropy_err are up to 1e34; a p of 0 gives an error of 0 then, whatever log p is.
+ * p is exp(z - lse) with the lse in 32 bits: off by a factor of up to exp(|lse| * 2^-23), and never above 1.  Rows whose |lse| is large (1e4: a
+ * thousandth; a row of nothing but the type's lowest value: p = 1 for 1 / V; an infinite lse: p = 0) have their errors from cnt_logprob_error_backward. */
 int cnt_logprob_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
                          const float *lse, const float *entropy, const float *logp_err, const float *entropy_err, void *err,
                          long err_stride);
 /* Both in one call, for losses whose errors do not depend on the results (a sum or mean over slots): logp (may be NULL), lse, entropy
- * and err.  scratch as for the forward call with K = 0. */
+ * and err.  p goes by the row's maximum here, so that rows far from zero are as exact as others.  scratch as for the forward call with K = 0. */
 int cnt_logprob_error_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
                                const float *logp_err, const float *entropy_err, float *logp, float *lse, float *entropy, void *err,
                                long err_stride, void *scratch, size_t scratch_bytes);

@@ -808,7 +808,8 @@ template <int W>
 __device__ __forceinline__ void errors_of(int at, const Slopes &s, float (&t)[W]) {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float u = at_least(t[i]);
+        // (a saved log sum in 32 bits may be off by more than 128: no probability is above 1)
+        const float u = __builtin_amdgcn_fmed3f(t[i], -1000.0f, 0.0f);
         t[i] = __builtin_amdgcn_exp2f(u) * __builtin_fmaf(s.second, u, s.first);
     }
     add_given<W>(at, s, t);

@@ -113,3 +113,27 @@ def test_gradient_of_rows_whose_log_sum_is_beyond_32_bits(V, times, dtype):
     g, h = np.array([1.0, -1.0, 0.5, 1.0, 2.0, 1.0], np.float32), np.array([0.5, 1.0, -1.0, 1.0, 2.0, 0.0], np.float32)
     for scale in (1.5, 64.0, 1e30):
         _check_joint(_dev(x, dtype), tokens, g, h, scale, times)
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+@pytest.mark.parametrize("scale", [1.0, 1e5, 1e20, 1e30])
+@pytest.mark.parametrize("V", [3, 300, 1500, 3000, 70001])
+def test_gradient_from_a_log_sum_that_is_off_stays_within_bounds(V, scale, dtype):
+    """A probability from a log sum in 32 bits is off by a factor exp(|lse| 2^-24), but none is above 1: with |log p| <= 1000 in front of one of
+    at least 2^-126, p |log p| <= 1 / e, an error is at most scale * (2 |g| + |h| (1 + H))."""
+    rng = np.random.default_rng(V)
+    N = 64
+    x = _dev(rng.standard_normal((N, V)) * 30, dtype)
+    x[5:9] = torch.finfo(dtype).min
+    x[9] = torch.finfo(dtype).max
+    g, h = rng.standard_normal(N).astype(np.float32), rng.standard_normal(N).astype(np.float32)
+    t = rng.integers(-1, V, N).astype(np.int32)
+    lse, entropy = torch.empty(N, device="cuda"), torch.empty(N, device="cuda")
+    capi, err = PC.pkg().capi, torch.full_like(x, 7.0)
+    capi.logprob_forward(x, lse=lse, entropy=entropy, scale=scale)
+    capi.logprob_backward(x, _dev(t), lse, entropy, _dev(g), _dev(h), err, scale=scale)
+    most = scale * (2 * np.abs(g) + np.abs(h) * (1 + S.f64(entropy)))
+    top = torch.finfo(dtype).max
+    got = S.f64(err)
+    assert not np.isnan(got).any()
+    assert np.all(np.abs(got) <= np.where(most < top, most * (1 + 4 * S.HALF[dtype]), np.inf)[:, None] + S.TINY[dtype])
