@@ -137,3 +137,35 @@ def test_gradient_from_a_log_sum_that_is_off_stays_within_bounds(V, scale, dtype
     got = S.f64(err)
     assert not np.isnan(got).any()
     assert np.all(np.abs(got) <= np.where(most < top, most * (1 + 4 * S.HALF[dtype]), np.inf)[:, None] + S.TINY[dtype])
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+@pytest.mark.parametrize("times", TIMES)
+@pytest.mark.parametrize("V", LENGTHS)
+def test_log_probabilities_of_rows_that_masks_leave_little_of(V, times, dtype):
+    rng = np.random.default_rng(V + 2)
+    x = rng.standard_normal((ROWS, V)) * 2.5
+    low, K = torch.finfo(dtype).min, 6
+    x[0] = low
+    x[1] += 1e4
+    x[2] = -np.inf
+    x[2, V - 1] = 1.5
+    x[3] = low
+    x[3, 5] = -3.0
+    x[4] = -np.inf
+    x[5, 3:V - 1] = low
+    x = _dev(x, dtype)
+    tokens = np.array([1, 2, V - 1, 4, 3, 9], np.int32)
+    out = {n: torch.full((ROWS * times,), 7.0, device="cuda") for n in ("logp", "lse", "entropy")}
+    out["top_logp"] = torch.full((ROWS * times, K), 7.0, device="cuda")
+    out["top_tokens"] = torch.full((ROWS * times, K), -7, dtype=torch.int32, device="cuda")
+    PC.pkg().capi.logprob_forward(x.repeat(times, 1), _dev(np.tile(tokens, times)), **out)
+    R, rows = S.Rows(S.f64(x), 1.0), np.arange(ROWS)
+    want = R.top(K)
+    for k in sorted({0, times // 2, times - 1}):
+        part = {n: t[ROWS * k:ROWS * k + ROWS] for n, t in out.items()}
+        assert np.array_equal(part["top_tokens"].cpu().numpy(), want)
+        S.assert_close(S.f64(part["top_logp"]), R.logp[rows[:, None], want], R.tol_logp[rows[:, None], want])
+        S.assert_close(S.f64(part["logp"]), R.logp[rows, tokens], R.tol_logp[rows, tokens])
+        S.assert_close(S.f64(part["lse"]), R.lse, R.tol_lse)
+        S.assert_close(S.f64(part["entropy"]), R.entropy, R.tol_entropy)
