@@ -610,8 +610,8 @@ float cnt_opt_next_beta_accum(float accum, int which);
  * place).  The three arrays are host memory and copied; the tensors have to stay where they are.  The create call allocates, the
  * others only enqueue work.  Calls with one handle share its sums: they have to follow each other, also those of captured
  * graphs.  No counterpart in the reference, which limits single error values only (helpers/limitedError.cuh).
- *   result[0] = norm = sqrt(sum of all squares), summed in 64 bits in a fixed order
- *   result[1] = factor = max_norm / norm if norm > max_norm, else 1; 0 if the norm is infinite or NaN
+ *   result[0] = norm = sqrt(sum of all squares), summed in 64 bits in a fixed order, rounded to 32
+ *   result[1] = factor = max_norm / norm if norm > max_norm, else 1; 0 if the norm is infinite, also by that rounding, or NaN
  * result: two floats of device memory; max_norm > 0.  cnt_opt_grad_norm writes these; cnt_opt_clip also multiplies every element
  * with the factor (zeros for the factor 0), rounded once. */
 typedef struct cnt_gradients cnt_gradients;

@@ -84,14 +84,14 @@ __global__ __launch_bounds__(256) void gradient_squares_kernel(const Piece *__re
     if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-// The factor, by all threads of a workgroup; the first workgroup's first thread writes norm and factor down.  A norm that is no finite number
-// gives the factor 0: gradients that hold infinities or NaN move no weight.
+// The factor, by all threads of a workgroup; the first workgroup's first thread writes norm and factor down.  A norm that is no finite number in
+// the 32 bits in which it is reported gives the factor 0, so that whoever looks at either decides the same.
 __device__ __forceinline__ float clip_factor(const double *__restrict__ sums, int count, float max_norm, float *__restrict__ result) {
     double s = 0.0;
     for (int i = threadIdx.x; i < count; i += 256) s += sums[i];
     s = block_sum(s);
     const double norm = sqrt(s);
-    const float factor = !(norm <= 1.7976931348623157e308) ? 0.0f : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.0f;
+    const float factor = !((float)norm <= 3.402823466e38f) ? 0.0f : norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.0f;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         result[0] = (float)norm;
         result[1] = factor;
