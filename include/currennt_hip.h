@@ -621,7 +621,7 @@ int cnt_gradients_destroy(cnt_gradients *set);
 int cnt_opt_grad_norm(cnt_gradients *set, void *stream, float max_norm, float *result);
 int cnt_opt_clip(cnt_gradients *set, void *stream, float max_norm, float *result);
 /* cnt_opt_step on clip[1] * layer_updates (zeros for the factor 0) with the result of cnt_opt_grad_norm: clipping without a pass over the
- * gradients of its own. */
+ * gradients of its own.  A step on zeros is a step all the same: momentum and Adam's moments move the weights. */
 int cnt_opt_step_clipped(void *stream, int option, long n, float *weights, const float *layer_updates, float *cur_updates,
                          float *stats, float *weight_deltas, const float *mask, float frac_length, float beta1_accum,
                          float beta2_accum, float learning_rate, float momentum, const float *clip);

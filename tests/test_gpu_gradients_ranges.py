@@ -35,3 +35,19 @@ def test_the_largest_norms_of_32_bits(n, value, limit):
     # the factor is rounded to 32 bits, by at most half of their smallest step, 2^-150, where it is below 2^-126
     S.assert_close(S.f64(result), [norm, limit / norm], [1e-12 * norm, 2.0 ** -150])
     S.assert_close(S.f64(g), before * (limit / norm), before * (2.0 ** -150 + S.U * limit / norm))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan"), 3.3e38])
+def test_a_fraction_without_a_norm_is_a_gradient_of_zeros(bad):
+    """Nothing of it comes to the weights; what earlier fractions have left in the momentum does."""
+    capi = PC.pkg().capi
+    n = 4099
+    g, w, delta = torch.randn(n, device="cuda"), torch.randn(n, device="cuda"), torch.randn(n, device="cuda")
+    g[5:9] = bad
+    clip, cur = torch.zeros(2, device="cuda"), torch.zeros(n, device="cuda")
+    capi.opt_grad_norm(capi.GradientSet([g]), 1.0, clip)
+    for start in (torch.zeros_like(delta), delta):
+        weights, deltas = w.clone(), start.clone()
+        capi.opt_step_clipped(0, weights, g, cur, None, deltas, None, 1.0, 0.0, 0.0, 0.125, 0.5, clip)
+        # products with 0.5 are exact: one rounding, that of the sum
+        assert torch.equal(deltas, 0.5 * start) and torch.equal(weights, w + 0.5 * start)
