@@ -671,10 +671,9 @@ def opt_step_clipped(option, weights, layer_updates, cur_updates, stats, deltas,
                      learning_rate, momentum, clip, stream=None):
     """opt_step on clip[1] * layer_updates, clip as opt_grad_norm has left it."""
     index = _index("weights", weights)
-    _vector("clip", clip, _Types.float32, 2, index)
-    check(lib().cnt_opt_step_clipped(stream_ptr(stream), option, weights.numel(), ptr(weights), ptr(layer_updates),
-                                     ptr(cur_updates), ptr(stats), ptr(deltas), ptr(mask), frac_length, beta1_accum,
-                                     beta2_accum, learning_rate, momentum, ptr(clip)))
+    address = _vector("clip", clip, _Types.float32, 2, index)
+    _enqueue(index, stream, lib().cnt_opt_step_clipped, option, weights.numel(), ptr(weights), ptr(layer_updates), ptr(cur_updates),
+             ptr(stats), ptr(deltas), ptr(mask), frac_length, beta1_accum, beta2_accum, learning_rate, momentum, address)
 
 
 def opt_next_beta_accum(accum, which):
@@ -927,10 +926,10 @@ class Network:
 
     def update_clipped(self, option, learning_rate, momentum, frac_length, max_norm, result, stream=None):
         """`update` with the gradients clipped to max_norm; result (two floats on the device) receives their norm and the factor."""
-        index = _index("result", result)
-        _vector("result", result, _Types.float32, 2, index)
-        check(lib().cnt_network_update_clipped(self.handle, stream_ptr(stream), option, learning_rate, momentum, frac_length, max_norm,
-                                               ptr(result)))
+        index = _index("loss", self.loss)  # the network's device
+        address = _vector("result", result, _Types.float32, 2, index)
+        _enqueue(index, stream, lambda raw: lib().cnt_network_update_clipped(self.handle, raw, option, learning_rate, momentum, frac_length,
+                                                                             max_norm, address))
 
     def export_json(self):
         need = C.c_size_t()

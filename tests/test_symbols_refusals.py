@@ -1,5 +1,6 @@
 """What the operators over symbols refuse, before any device call: runs without a GPU."""
 import ctypes as C
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -192,3 +193,35 @@ def test_the_binding_checks_tensors_on_the_device():
             capi.opt_clip(gset, bad, c(2))
     with pytest.raises(ValueError, match="2 contiguous values"):
         capi.opt_clip(gset, 1.0, c(3))
+
+
+class _Elsewhere:
+    """what a call looks at of a tensor on a GPU, and nothing behind it"""
+
+    def __init__(self, count):
+        self.dtype, self.shape, self.count = torch.float32, (count,), count
+
+    def get_device(self):
+        return 0
+
+    def numel(self):
+        return self.count
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 4096
+
+
+def test_clipped_steps_run_where_their_tensors_are():
+    # as the other calls with the norm's result: a stream of another device is refused
+    capi = load_package().capi
+    stream = SimpleNamespace(device_index=1, device="cuda:1", cuda_stream=0)
+    none, two = _Elsewhere(0), _Elsewhere(2)
+    with pytest.raises(ValueError, match="stream"):
+        capi.opt_step_clipped(0, none, none, none, none, none, None, 1.0, 0.0, 0.0, 0.1, 0.0, two, stream=stream)
+    net = capi.Network.__new__(capi.Network)
+    net.handle, net.loss = capi.VP(), _Elsewhere(1)
+    with pytest.raises(ValueError, match="stream"):
+        net.update_clipped(0, 0.1, 0.0, 1.0, 1.0, two, stream=stream)
