@@ -167,7 +167,8 @@ int cnt_logprob_backward(void *stream, long N, int V, int type, const void *logi
                          const float *lse, const float *entropy, const float *logp_err, const float *entropy_err, void *err,
                          long err_stride);
 /* Both in one call, for losses whose errors do not depend on the results (a sum or mean over slots): logp (may be NULL), lse, entropy
- * and err.  p goes by the row's maximum here, so that rows far from zero are as exact as others.  scratch as for the forward call with K = 0. */
+ * and err.  p goes by the row's maximum here, so that rows far from zero are as exact as others.  N < 2^23 for rows of
+ * more than 32640 bytes, < 2^22 of more than 65408.  scratch as for the forward call with K = 0. */
 int cnt_logprob_error_backward(void *stream, long N, int V, int type, const void *logits, long stride, float scale, const int *tokens,
                                const float *logp_err, const float *entropy_err, float *logp, float *lse, float *entropy, void *err,
                                long err_stride, void *scratch, size_t scratch_bytes);

@@ -1303,6 +1303,9 @@ int cnt_logprob_error_backward(void *stream_, long N, int V, int type, const voi
     a.logits = logits; a.stride = stride; a.tokens = tokens; a.N = N; a.V = V; a.scale = scale;
     a.logp = logp; a.lse = lse; a.entropy = entropy;
     a.logp_err = logp_err; a.entropy_err = entropy_err; a.err = err; a.err_stride = err_stride;
+    // a launch has fewer than 2^32 threads: 1024 for a row beyond 64 KB, 512 beyond 32 KB (less what it may begin by inside a cache line)
+    const long row_bytes = V * (long)element_size(type) + 128;
+    CNT_REQUIRE(N < 1L << (row_bytes > 1 << 16 ? 22 : row_bytes > 1 << 15 ? 23 : 24), "logprob_error_backward: too many rows of this length");
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     ProfileScope prof(stream, "logprob_error_backward");
     if (shared_errors(N, V, type)) {

@@ -225,3 +225,11 @@ def test_clipped_steps_run_where_their_tensors_are():
     net.handle, net.loss = capi.VP(), _Elsewhere(1)
     with pytest.raises(ValueError, match="stream"):
         net.update_clipped(0, 0.1, 0.0, 1.0, 1.0, two, stream=stream)
+
+
+@pytest.mark.parametrize("code,size", [(0, 4), (1, 2), (2, 2)])
+def test_rows_that_no_launch_has_threads_for(code, size):
+    # (no refused call may touch the addresses; in the logits' place, as rows of this number leave no room for others)
+    L = load_package().capi.lib()
+    for V, N in ((32641 // size + 1, 1 << 23), (65409 // size + 1, 1 << 22), (131072, 1 << 22)):
+        _refused(L.cnt_logprob_error_backward(None, N, V, code, P, V, 1.0, P, P, P, P, P, P, P, V, None, 0), "too many rows")
