@@ -133,7 +133,8 @@ int cnt_embed_forward(void *stream, int V, int D, long N, int table_type, const 
  * there is no such slot); accumulate != 0 adds to grad instead and leaves rows without a slot untouched.  The sums are
  * formed in 32 bits in an order that the tokens alone determine: the same call gives the same bits.  scratch: device memory of
  * cnt_embed_scratch(V, D, N) bytes (enough for fewer slots as well), aligned to 16, with any content, which the call has for itself until it has run (two captured
- * graphs that may run at the same time need one each).  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^33. */
+ * graphs that may run at the same time need one each).  It is asked for whatever the sizes, also where a call uses none (lists of up to 128 slots, most of
+ * up to 512); small tables' sums on the way take as much of it as the errors in 32 bits, up to 135 MB.  V <= 2^23, D <= 2^21, N <= 2^30, V * D and N * D <= 2^33. */
 long cnt_embed_scratch(int V, int D, long N);
 int cnt_embed_backward(void *stream, int V, int D, long N, const int *tokens, float scale, int err_type, const void *err,
                        long err_stride, int grad_type, void *grad, long grad_stride, int accumulate, void *scratch,
@@ -608,9 +609,9 @@ float cnt_opt_next_beta_accum(float accum, int which);
 /* ---- norm of all gradients, and clipping -------------------------------------------------------------
  * A cnt_gradients handle is a list of tensors: tensor i has sizes[i] elements of types[i] (CNT_F32, CNT_BF16, CNT_F16) at
  * gradients[i] (device memory, aligned to its elements), and cnt_opt_clip writes to clipped[i] (same size and type; clipped = NULL: in
- * place).  The three arrays are host memory and copied; the tensors have to stay where they are.  The create call allocates, the
- * others only enqueue work.  Calls with one handle share its sums: they have to follow each other, also those of captured
- * graphs.  No counterpart in the reference, which limits single error values only (helpers/limitedError.cuh).
+ * place).  The arrays are host memory and copied; the tensors have to stay where they are: a set is made once, for buffers that a program keeps.
+ * The create call allocates and copies, for which it waits, and the destroy call waits for the device; the others only enqueue work.  Calls with one
+ * handle share its sums: they have to follow each other, also those of captured graphs.  No counterpart in the reference, which limits single error values only (helpers/limitedError.cuh).
  *   result[0] = norm = sqrt(sum of all squares), summed in 64 bits in a fixed order, rounded to 32
  *   result[1] = factor = max_norm / norm if norm > max_norm, else 1; 0 if the norm is infinite, also by that rounding, or NaN
  * result: two floats of device memory; max_norm > 0.  cnt_opt_grad_norm writes these; cnt_opt_clip also multiplies every element

@@ -99,10 +99,16 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const LookupArgs a) {
 
 // ----- sort of the slots by token ---------------------------------------------------------------------------------------------
 constexpr int kMostBits = 10, kMostBins = 1 << kMostBits, kMostSortBlocks = 512, kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-// Up to here every workgroup counts the whole list's digits for itself, which takes less than a launch of its own for the counts.
+// Up to here every workgroup counts the whole list's digits for itself, which takes about as long as a launch of its own for the counts, and less in
+// short lists (gradient of 65536 x 128 in bf16, counted by every workgroup / by a launch: 8000 slots 31.5 us / 33.1, 16384 37.0 / 36.1, 30000
+// 41.6 / 39.6; 45000 48.1 / 41.1, 120000 76.7 / 53.3).
 constexpr long kCountedTwice = 32768;
 constexpr int kFillVectors = 4;
-constexpr size_t kFillFrom = 16 << 20, kFillBytes = 48 << 20;  // tables that are filled on the way, bytes per launch
+// Tables that are filled on the way, bytes per launch.  Filled / not, us: 65536 x 1024 fp32 from 16384 slots 65.9 / 75.0, 30000 x 768 from 8192
+// 37.8 / 38.7; tables of 16 to 40 MB are up to two us slower so (8192 x 512 from 20000 34.3 / 33.3, 20000 x 512 from 16384 35.7 / 33.8).
+// 24, 32, 48, 64 and 80 MB per launch: 65536 x 1024 fp32 from 16384 slots 71.0, 68.7, 66.1, 63.4 and 65.0, from 8192 61.8, 59.7, 56.4, 55.6 and
+// 60.1; 131072 x 512 bf16 from 16384 42.0, 42.2, 44.6, 44.8 and 46.3; 131072 x 1024 bf16 from 4000 59.1, 56.5, 52.3, 52.6 and 59.3.
+constexpr size_t kFillFrom = 16 << 20, kFillBytes = 48 << 20;
 
 // Scratch of a gradient, which is enough for shorter lists as well: two lists of (token, slot), counts of every block and digit, the number of slots with a token, where the rows' runs
 // begin, partial sums.
@@ -634,16 +640,16 @@ int sum_few(hipStream_t stream, const FewArgs &args) {
 // ----- slabs of the list ------------------------------------------------------------------------------------------------------------------
 // A workgroup sorts the slots of a slab that belong to its rows in LDS and adds their errors up.  One slab's sums are the gradient itself; those
 // of several are left in the place of their first slot and added up, in order, by a second launch, which goes by an index of the rows' runs; or, where
-// a slab has two places for every row, in the row's (256 x 64 from 32000 slots 15.3 us, by the index 16.4; half empty, 509 x 746 from 6737 26 and 19).
+// a slab has two places for every row, in the row's (256 x 64 from 32000 slots 16.7 us, by the index 17.6; 31 x 8 from 260000 41.9 and 46.0; half empty, 509 x 746 from 6737 26 and 19).
 constexpr unsigned short kNoRun = 0xffff;
 constexpr int kSlab = 512, kSlabRows = 1024, kSlabWaves = kSlab / 64, kSlabLanes = 16;
-// Against the sorted list, us.  One slab: 1000 x 64 from 300 slots 6.6 / 17.0, 100000 x 64 from 500 10 / 21, 50000 x 458 from 300 22 / 28; beyond
-// 65536 x 1024 from 500 54 / 47 (the zeros, in rows of 256 bytes here).
+// Against the sorted list, fp32, us.  One slab: 1000 x 64 from 300 slots 7.0 / 18.2, 100000 x 64 from 500 10.7 / 22.1, 50000 x 458 from 300 24.6 / 28.7;
+// beyond 65536 x 1024 from 500 54 / 47 (the zeros, in rows of 256 bytes here).
 constexpr long kOneSlabValues = 1 << 25;
-// Several: 256 x 64 from 32000 15.3 / 22.0, 1000 x 64 from 2000 10.0 / 14.5, 1665 x 594 from 943 12.5 / 20.6, 46356 x 13 from 7743 19 / 30, 2261 x 132 from
-// 17980 18.6 / 27.6, 3992 x 1135 from 3826 24 / 29; beyond 19473 x 367 from 4492 36 / 28, 577 x 801 from 26051 44 / 36, 100 x 2048 from 16000
-// 41 / 36.
-// More errors where little is left of them: 51 x 767 from 25518 26 / 34, 20 x 512 from 30000 19 / 41.
+// Several: 256 x 64 from 32000 16.7 / 23.3, 1000 x 64 from 2000 10.8 / 15.3, 1665 x 594 from 943 13.5 / 21.4, 46356 x 13 from 7743 19.4 / 29.5, 2261 x 132
+// from 17980 19.4 / 30.9, 3992 x 1135 from 3826 25.3 / 29.5; beyond 19473 x 367 from 4492 36 / 28, 577 x 801 from 26051 44 / 36, 100 x 2048 from
+// 16000 41 / 36.
+// More errors where little is left of them: 51 x 767 from 25518 35.5 / 40.1, 20 x 512 from 30000 21.4 / 41.1.
 constexpr long kSlabValues = 1 << 24, kSlabJoined = 5 << 23, kFewJoined = 1 << 21;  // errors; values of all slabs' tables
 constexpr int kMostSlabs = 512;  // (31 x 8 from 260000 41 / 42, from 1000000 141 / 72)
 
