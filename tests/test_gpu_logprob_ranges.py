@@ -169,3 +169,26 @@ def test_log_probabilities_of_rows_that_masks_leave_little_of(V, times, dtype):
         S.assert_close(S.f64(part["logp"]), R.logp[rows, tokens], R.tol_logp[rows, tokens])
         S.assert_close(S.f64(part["lse"]), R.lse, R.tol_lse)
         S.assert_close(S.f64(part["entropy"]), R.entropy, R.tol_entropy)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_shared_rows_on_two_streams_at_once(dtype):
+    """What the three launches of a call hand on is in the call's own scratch memory."""
+    capi, N, V = PC.pkg().capi, 5, 140001
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for k in range(2):
+        x = (torch.randn(N, V, device="cuda") * 2.5 + 1e4 * k).to(dtype)
+        x[3] = torch.finfo(dtype).min
+        t = torch.randint(0, V, (N,), device="cuda", dtype=torch.int32)
+        new = lambda: [torch.zeros(N, device="cuda") for _ in range(3)] + [torch.zeros_like(x)]
+        sets.append((x, t, torch.randn(N, device="cuda"), torch.randn(N, device="cuda"), new(), new()))
+    for x, t, g, h, alone, _ in sets:
+        capi.logprob_error_backward(x, t, g, h, *alone)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for stream, (x, t, g, h, _, out) in zip(streams, sets):
+            capi.logprob_error_backward(x, t, g, h, *out, stream=stream)
+    torch.cuda.synchronize()
+    for _, _, _, _, alone, out in sets:
+        assert all(torch.equal(a, b) for a, b in zip(alone, out))
